@@ -191,6 +191,114 @@ size_t lsvd_attn_decode_static_scratch_bytes(void);
 int lsvd_attn_decode_static(const lsvd_attn_decode_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Slots of the tokens that a step adds, on the device (no counterpart in the reference, whose harness fixes its slots on
+ * the host; the field names are those of its MockInferState, kernels/layer_bench/ffn_kernel/baseline_kernel.py:38-53).
+ * The cache is cut into pages of page_size slots; row r of block_table lists the pages of request row r.  Entry b of the
+ * batch stands for row b_req_idx[b], holds `ready` = b_ready_cache_len[b] tokens and gets n = b_new_len[b] more:
+ *   b_start_loc[b]  = sum of n over the entries before b       (b_start_loc[batch] = all of them)
+ *   b_seq_len[b]    = ready + n
+ *   pages           : columns ceil(ready / page_size) .. ceil((ready + n) / page_size) - 1 of its block_table row are
+ *                     taken, in batch order, from free_pages[*free_head ..]; *free_head_out = the first one left
+ *   slot(pos)       = block_table[row][pos / page_size] * page_size + pos % page_size
+ *   mem_index[b_start_loc[b] + i] = req_to_token[row][ready + i] = slot(ready + i),  position_ids[..] = ready + i
+ *   rebuild != 0    : req_to_token[row][0 .. ready) is written as well (pages taken over from elsewhere)
+ * Entries of mem_index / position_ids behind the last token, up to num_tokens, become -1 / 0.  b_seq_len may be the array
+ * b_ready_cache_len and free_head_out the word free_head (a captured step then advances the lengths at every replay).
+ * An entry is refused -- it takes no page, its length stays `ready`, its tokens get slot -1 and position 0, LSVD_ERR_BOUNDS
+ * is reported -- when its row, a length or its tokens do not fit the tables or num_tokens, when an earlier entry adds tokens to the same
+ * row, or when the free pages run out (with every later entry that needs a page).  A page outside the cache gives slot -1.
+ * ------------------------------------------------------------------------------------------- */
+#define LSVD_MAX_BATCH 4096     /* entries of a batch in lsvd_chunk_maps */
+typedef struct lsvd_chunk_maps_args {
+  int32_t batch, page_size;
+  int32_t num_tokens;            /* capacity of mem_index and position_ids                                          */
+  int32_t num_slots;             /* rows in the cache                                                               */
+  const int32_t* b_req_idx;      /* device int32 [batch]                                                            */
+  const int32_t* b_ready_cache_len;   /* device int32 [batch]                                                       */
+  const int32_t* b_new_len;      /* device int32 [batch]                                                            */
+  int32_t* block_table;          /* device int32 [table_rows][block_table_stride], max_blocks columns used          */
+  int64_t block_table_stride;
+  int32_t max_blocks, table_rows;
+  int32_t* req_to_token;         /* device int32 [table_rows][req_to_token_stride], max_len columns used            */
+  int64_t req_to_token_stride;
+  int32_t max_len, rebuild;
+  const int32_t* free_pages;     /* device int32 [num_free], or NULL: block_table already lists every page          */
+  const int32_t* free_head;      /* device int32 [1]: entries of free_pages taken so far (NULL without free_pages)  */
+  int32_t num_free;
+  int32_t* free_head_out;        /* device int32 [1]                                                                */
+  int32_t* b_start_loc;          /* device int32 [batch + 1]                                                        */
+  int32_t* b_seq_len;            /* device int32 [batch]                                                            */
+  int32_t* mem_index;            /* device int32 [num_tokens]                                                       */
+  int32_t* position_ids;         /* device int32 [num_tokens]                                                       */
+  int32_t* status_word;          /* device int32 or NULL                                                            */
+} lsvd_chunk_maps_args;
+int lsvd_chunk_maps(const lsvd_chunk_maps_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention of new tokens over the paged int8 latent cache ("absorb" form, see lsvd_attn_decode), any number of query
+ * tokens per request: a prompt, a piece of one, drafted tokens to verify, or a single token.  No counterpart in the
+ * reference, whose kernels are decode-only.  The tokens' own latents are in the cache already (lsvd_cache_append).
+ * Request b owns the rows b_start_loc[b] .. b_start_loc[b+1]-1 of q and out, its LAST n tokens: row i of them stands at
+ * position pos = b_seq_len[b] - n + i and sees the keys t with lo <= t < hi,
+ *   hi = causal ? min(len, max(pos + 1, b_prefix_len[b])) : window > 0 ? min(len, pos + window) : len
+ *   lo = max(0, key_begin[row], window > 0 ? pos + 1 - window : 0)
+ *   x  = sm_scale * scale_k[t,h] * (z_k[t,h] . B_k q),   softcap > 0: x = softcap * tanh(x / softcap),
+ *   alibi_slopes: x -= alibi_slopes[h] * |pos - t|,      p = softmax_t(x),
+ *   o_lat = sum_t p_t scale_v[t,h] z_v[t,h],             o = B_v^T o_lat
+ * A row that sees nothing (or only scores of minus infinity) gets zeros.  Cached tokens whose slot is negative are not
+ * seen.  Rows behind b_start_loc[batch] are left as they were.  num_q_heads == num_kv_heads only.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct lsvd_attn_chunk_args {
+  int32_t batch, num_heads;
+  int32_t head_dim;              /* multiple of 8, <= 256                                                          */
+  int32_t max_len_in_batch;      /* upper bound of b_seq_len; a longer one is treated as this and reported          */
+  int32_t num_tokens;            /* rows of q and of the outputs (capacity)                                        */
+  int32_t max_new_in_batch;      /* upper bound of the new tokens of one request; a request with more is skipped   */
+                                 /* (its rows are left as they were) and reported as LSVD_ERR_BOUNDS               */
+  float sm_scale;                /* <= 0 selects 1/sqrt(head_dim)                                                  */
+  int32_t num_slots;
+  const void* q;                 /* device fp16 (row, h, d) at q[row*q_stride_t + h*q_stride_h + d]                */
+  int64_t q_stride_t, q_stride_h;
+  const int32_t* k_off;          /* HOST [num_heads+1], as in lsvd_attn_decode_args                                */
+  const int32_t* v_off;
+  const int8_t* cache_k;
+  int64_t cache_k_row_stride;
+  const void* scale_k;
+  int64_t scale_k_row_stride;
+  const int8_t* cache_v;
+  int64_t cache_v_row_stride;
+  const void* scale_v;
+  int64_t scale_v_row_stride;
+  const void* up_k;              /* device fp16 [sum r_k, head_dim]                                                */
+  int64_t up_k_row_stride;
+  const void* up_v;              /* device fp16 [sum r_v, head_dim]; may be NULL when out is NULL                  */
+  int64_t up_v_row_stride;
+  const int32_t* req_to_token;   /* device int32, at least max_len_in_batch columns                                */
+  int64_t req_to_token_stride;
+  const int32_t* b_req_idx;      /* device int32 [batch]                                                           */
+  const int32_t* b_seq_len;      /* device int32 [batch]: length with the new tokens                               */
+  const int32_t* b_start_loc;    /* device int32 [batch + 1], not decreasing                                       */
+  void* out;                     /* device fp16 (row, h, d), or NULL                                               */
+  int64_t out_stride_t, out_stride_h;
+  void* out_latent;              /* device fp16 (row, v_off[h]+i), or NULL                                         */
+  int64_t out_latent_stride_t;
+  void* workspace;               /* device, 256-byte aligned                                                       */
+  size_t workspace_bytes;
+  int32_t* status_word;          /* device int32 or NULL                                                           */
+  int32_t cache_layout;          /* LSVD_CACHE_*                                                                   */
+  int32_t req_to_token_rows;     /* a b_req_idx outside [0, rows) makes the request an empty one and is reported   */
+  int32_t causal, window;        /* window <= 0: none                                                              */
+  float softcap;                 /* <= 0: none                                                                     */
+  const float* alibi_slopes;     /* device fp32 [num_heads] or NULL                                                */
+  const int32_t* b_prefix_len;   /* device int32 [batch] or NULL                                                   */
+  const int32_t* key_begin;      /* device int32 [num_tokens] or NULL                                              */
+} lsvd_attn_chunk_args;
+/* Bytes of workspace for this problem on the current device (0: bad sizes). */
+size_t lsvd_attn_chunk_workspace_bytes(int32_t batch, int32_t num_heads, int32_t sum_rank_v, int32_t num_tokens,
+                                       int32_t max_new_in_batch, int32_t max_len_in_batch);
+int lsvd_attn_chunk(const lsvd_attn_chunk_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Decode attention in the reference's own form ("rope_recon"): int8 K up-factor, keys rebuilt per token and
  * rotated at their logical position, uniform ranks, grouped-query heads.  Replaces
  * token_decode_attention_flash_int8_latent_per_head_decoding_rope (kernels/layer_bench/fd_kernel/flash_decoding.py:3-57),

@@ -9,6 +9,7 @@ from ._lib import LsvdError
 from .attention import (LatentCacheLayout, destindex_copy_quantize_latent, cache_append,
                         token_decode_attention_int8_latent_absorb,
                         token_decode_attention_flash_int8_latent_per_head_decoding_rope, LatentDecodeAttention, InferState)
+from .chunk import ChunkMaps, ChunkState, chunk_maps, chunk_attention_int8_latent_absorb
 from .block import Int8AttentionBlock
 from .mixffn import MixedFFNGateUpDenseLatentFused, b200_mixffn
 from .ffn import (HybridFFN, quantize_weight_rtn, act_quant, hadamard_pack, hadamard_quant, heads_hadamard_quant, w8a8_gemv,
@@ -21,5 +22,6 @@ __all__ = ["ActQuantizer", "ActQuantWrapper", "SVDLinear", "add_actquant", "find
            "resolve_channel_group", "load_qmodel", "hybrid_ffn_weights", "load_hybrid_ffn", "int8_from_fake_quant",
            "LsvdError", "LatentCacheLayout", "destindex_copy_quantize_latent", "cache_append",
            "token_decode_attention_int8_latent_absorb", "token_decode_attention_flash_int8_latent_per_head_decoding_rope",
-           "LatentDecodeAttention", "InferState", "Int8AttentionBlock", "MixedFFNGateUpDenseLatentFused", "b200_mixffn", "HybridFFN", "quantize_weight_rtn", "act_quant", "hadamard_pack",
+           "LatentDecodeAttention", "InferState",
+           "ChunkMaps", "ChunkState", "chunk_maps", "chunk_attention_int8_latent_absorb", "Int8AttentionBlock", "MixedFFNGateUpDenseLatentFused", "b200_mixffn", "HybridFFN", "quantize_weight_rtn", "act_quant", "hadamard_pack",
            "hadamard_quant", "heads_hadamard_quant", "w8a8_gemv", "i8gemm"]

@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(HERE, "liblsvd_b200.so")
 
 LSVD_MAX_HEADS = 128
 LSVD_MAX_RANK = 128
+LSVD_MAX_BATCH = 4096
 ROUND_TORCH, ROUND_TRITON = 0, 1
 CACHE_SLOT_MAJOR, CACHE_HEAD_MAJOR = 0, 1
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_TIMEOUT, ERR_BOUNDS = range(7)
@@ -60,6 +61,40 @@ class AttnDecodeArgs(C.Structure):
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("status_word", C.c_void_p), ("ev_stream_begin", C.c_void_p), ("ev_stream_end", C.c_void_p),
         ("cache_layout", C.c_int32), ("req_to_token_rows", C.c_int32),
+    ]
+
+
+class ChunkMapsArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("page_size", C.c_int32), ("num_tokens", C.c_int32), ("num_slots", C.c_int32),
+        ("b_req_idx", C.c_void_p), ("b_ready_cache_len", C.c_void_p), ("b_new_len", C.c_void_p),
+        ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("max_blocks", C.c_int32), ("table_rows", C.c_int32),
+        ("req_to_token", C.c_void_p), ("req_to_token_stride", C.c_int64), ("max_len", C.c_int32), ("rebuild", C.c_int32),
+        ("free_pages", C.c_void_p), ("free_head", C.c_void_p), ("num_free", C.c_int32), ("free_head_out", C.c_void_p),
+        ("b_start_loc", C.c_void_p), ("b_seq_len", C.c_void_p), ("mem_index", C.c_void_p), ("position_ids", C.c_void_p),
+        ("status_word", C.c_void_p),
+    ]
+
+
+class AttnChunkArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("num_heads", C.c_int32), ("head_dim", C.c_int32), ("max_len_in_batch", C.c_int32),
+        ("num_tokens", C.c_int32), ("max_new_in_batch", C.c_int32), ("sm_scale", C.c_float), ("num_slots", C.c_int32),
+        ("q", C.c_void_p), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64),
+        ("k_off", C.POINTER(C.c_int32)), ("v_off", C.POINTER(C.c_int32)),
+        ("cache_k", C.c_void_p), ("cache_k_row_stride", C.c_int64),
+        ("scale_k", C.c_void_p), ("scale_k_row_stride", C.c_int64),
+        ("cache_v", C.c_void_p), ("cache_v_row_stride", C.c_int64),
+        ("scale_v", C.c_void_p), ("scale_v_row_stride", C.c_int64),
+        ("up_k", C.c_void_p), ("up_k_row_stride", C.c_int64),
+        ("up_v", C.c_void_p), ("up_v_row_stride", C.c_int64),
+        ("req_to_token", C.c_void_p), ("req_to_token_stride", C.c_int64),
+        ("b_req_idx", C.c_void_p), ("b_seq_len", C.c_void_p), ("b_start_loc", C.c_void_p),
+        ("out", C.c_void_p), ("out_stride_t", C.c_int64), ("out_stride_h", C.c_int64),
+        ("out_latent", C.c_void_p), ("out_latent_stride_t", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status_word", C.c_void_p),
+        ("cache_layout", C.c_int32), ("req_to_token_rows", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32),
+        ("softcap", C.c_float), ("alibi_slopes", C.c_void_p), ("b_prefix_len", C.c_void_p), ("key_begin", C.c_void_p),
     ]
 
 
@@ -186,6 +221,9 @@ SIGNATURES = {
     "lsvd_attn_decode": (C.c_int, [C.POINTER(AttnDecodeArgs), C.c_void_p]),
     "lsvd_attn_decode_static_scratch_bytes": (C.c_size_t, []),
     "lsvd_attn_decode_static": (C.c_int, [C.POINTER(AttnDecodeArgs), C.c_void_p]),
+    "lsvd_chunk_maps": (C.c_int, [C.POINTER(ChunkMapsArgs), C.c_void_p]),
+    "lsvd_attn_chunk_workspace_bytes": (C.c_size_t, [C.c_int32] * 6),
+    "lsvd_attn_chunk": (C.c_int, [C.POINTER(AttnChunkArgs), C.c_void_p]),
     "lsvd_heads_hadamard_quant": (C.c_int, [C.POINTER(HeadsHadamardQuantArgs), C.c_void_p]),
     "lsvd_ffn_decode_workspace_bytes": (C.c_size_t, [C.c_int32] * 5),
     "lsvd_ffn_decode_is_fused": (C.c_int, [C.POINTER(FfnDecodeArgs)]),

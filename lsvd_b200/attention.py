@@ -389,15 +389,16 @@ class LatentDecodeAttention(nn.Module):
     are given, then attends.
     """
 
-    def __init__(self, layout: LatentCacheLayout, head_dim: int, up_k: torch.Tensor, up_v: torch.Tensor,
+    def __init__(self, layout: LatentCacheLayout, head_dim: int, up_k: torch.Tensor, up_v: Optional[torch.Tensor],
                  rounding: str = "torch"):
         super().__init__()
         self.layout = layout
         self.head_dim = head_dim
         self.rounding = rounding
         self.register_buffer("up_k", up_k.to(torch.float16).contiguous())
-        self.register_buffer("up_v", up_v.to(torch.float16).contiguous())
+        self.register_buffer("up_v", None if up_v is None else up_v.to(torch.float16).contiguous())
         self._workspace = None
+        self._chunk_workspaces = []
 
     def _ws(self, batch, max_len, device):
         need = attn_decode_workspace_bytes(batch, self.layout, max_len)
@@ -420,6 +421,32 @@ class LatentDecodeAttention(nn.Module):
         return token_decode_attention_int8_latent_absorb(
             q, infer_state, self.layout.num_heads, self.head_dim, cache_k, scale_k, cache_v, scale_v,
             self.up_k, self.up_v, layout=self.layout, out=out, workspace=ws)
+
+    @torch.no_grad()
+    def forward_chunk(self, q, cache_k, scale_k, cache_v, scale_v, state, latent_k=None, latent_v=None, out=None, out_latent=None,
+                      **scores):
+        """A step with any number of new tokens per request (``state``: a ``ChunkState``): appends their latents ``[T, sum r]``
+        at ``state.mem_index`` when they are given, then attends from ``q [T, H, D]``.  ``scores``: ``causal``, ``window``,
+        ``b_prefix_len``, ``key_begin``, ``softcap``, ``alibi_slopes``, ``sm_scale`` as in ``chunk_attention_int8_latent_absorb``."""
+        from .chunk import attn_chunk_workspace_bytes, chunk_attention_int8_latent_absorb
+        if self.up_v is None and out is not None:
+            raise ValueError("without up_v the result is out_latent")
+        hm = self.layout.head_major
+        if not hm:
+            cache_k, cache_v = cache_k.view(cache_k.shape[0], -1), cache_v.view(cache_v.shape[0], -1)
+        if latent_k is not None or latent_v is not None:
+            cache_append(self.layout, latent_k, latent_v, state.mem_index, cache_k, scale_k, cache_v, scale_v, rounding=self.rounding)
+        with torch.cuda.device(q.device):
+            need = attn_chunk_workspace_bytes(state, self.layout, q.shape[0])
+        kept = self._chunk_workspaces
+        if not kept or kept[-1].numel() < need or kept[-1].device != q.device:
+            # an outgrown workspace stays: a captured step may still point to it (each is twice the last, so all of them
+            # together are at most twice the largest)
+            size = max(need, 2 * kept[-1].numel() if kept and kept[-1].device == q.device else 0)
+            kept.append(torch.empty(size, dtype=torch.uint8, device=q.device))
+        return chunk_attention_int8_latent_absorb(
+            q, state, self.layout.num_heads, self.head_dim, cache_k, scale_k, cache_v, scale_v, self.up_k, self.up_v,
+            layout=self.layout, out=out, out_latent=out_latent, workspace=kept[-1], **scores)
 
 
 @torch.no_grad()

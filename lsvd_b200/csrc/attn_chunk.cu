@@ -1,0 +1,673 @@
+// Attention of new tokens over the paged int8 latent cache ("absorb" form): entry points, the stream form, the merge.
+//
+// The query is folded into the per-head K up-factor once per row (q~ = B_k q), so that a score is a dot product of r_k int8
+// latents with q~, and the values stay in the latent space until the end:
+//   x_t = sm_scale scale_k[t] (z_k[t] . q~) [capped, biased],  o_lat = sum_t softmax(x)_t scale_v[t] z_v[t],  o = B_v^T o_lat.
+//
+// Stream form (up to 16 query rows of a request share one pass over its cache): a block owns (request, head, 16 query rows,
+// split of the keys); each of its four warps walks its own 32-key tiles.  The rows arrive by 16-byte asynchronous copies in
+// a ring of shared memory per warp (gathered slot by slot: any page table, both cache layouts); codes become fp16 exactly
+// (|code| <= 128) and meet q~ and the weights on the tensor cores (mma m16n8k16, fp32 accumulators).  With few rows the bytes
+// of the cache bound it: r_k + r_v + 4 bytes per key and head.
+//
+// Roundings.  q~ is kept in fp16 relative to its row's largest entry (a power of two taken out, so no entry overflows and
+// small ones keep their bits down to 2^-23 of the largest), the weights p * scale_v in fp16 relative to the largest V scale
+// seen: 2^-11 of each term, the size of the rounding of the fp16 result.  Maxima, sums and accumulators are fp32.  Scales are
+// applied in fp32 to scores and weights, never to the codes: a masked key's scale, were it infinite or NaN, touches nothing.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "attn_chunk.cuh"
+#include "devfn.cuh"
+
+namespace lsvd {
+
+constexpr int kChunkWarps = 4;
+constexpr int kChunkThreads = kChunkWarps * 32;
+constexpr int kRingBytes = 16 * 1024;         // per warp: 2 to 8 stages of 32 keys x (r_k + r_v) bytes
+constexpr int kMaxStages = 8;
+constexpr int kWeightShift = 10;              // weights are held as p * scale_v * 2^(10 - E), 2^E <= largest scale < 2^(E+1)
+
+// Absorbed query row `row` [128] fp32: four rows in the last 2 KB of every warp's ring, which no copy reaches before the
+// first tile is consumed (stages 0 .. n - 2 are requested ahead of that; the last stage, or what lies behind it, is free).
+__device__ __forceinline__ float* absorbed_row(uint8_t* ring_mem, int row) {
+  return reinterpret_cast<float*>(ring_mem + ((row >> 2) + 1) * kRingBytes - 2048 + (row & 3) * 512);
+}
+
+struct __align__(16) ChunkShared {
+  float sk[kChunkWarps][32], sv[kChunkWarps][32];             // scales of the tile in hand
+  int32_t slot[kChunkWarps][kMaxStages][32];                  // slot of every key in the ring, -1: none
+  float m[kChunkWarps][kStreamRows], l[kChunkWarps][kStreamRows];
+  int32_t lo[kStreamRows], hi[kStreamRows];
+};
+
+template <int kN>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// 16 bytes global -> shared, or 16 zero bytes (nothing is read).
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
+// Four consecutive halves, zero beyond `n` of them.
+__device__ __forceinline__ uint2 load_halves4(const __half* src, int n, bool vec) {
+  uint2 v = make_uint2(0u, 0u);
+  if (n >= 4 && vec) return __ldg(reinterpret_cast<const uint2*>(src));
+  __half* h = reinterpret_cast<__half*>(&v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) h[e] = src[e];
+  return v;
+}
+
+// q~ of up to 16 rows into shared memory, by all warps of the block: warp w takes the 8-rank tiles w, w + 4, ...
+// (mma lane (g, t): rows g and g + 8, k = halves 4t .. 4t + 3 of a 16-wide step, ranks 8 j + g).
+__device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int row0, int rows,
+                                            uint8_t* ring_mem) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const __half* qa = p.q + static_cast<int64_t>(r.start + row0 + min(g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+  const __half* qb = p.q + static_cast<int64_t>(r.start + row0 + min(g + 8, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+  const int tiles = H.nk * 2;
+  for (int j = warp; j < tiles; j += kChunkWarps) {
+    const __half* up = p.up_k + static_cast<int64_t>(H.k_col + j * 8 + g) * p.up_k_row_stride;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int d0 = 0; d0 < p.head_dim; d0 += 64) {
+      uint2 a0[4], a1[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = d0 + 16 * i + 4 * t;
+        a0[i] = load_halves4(qa + d, p.head_dim - d, p.q_vec);
+        a1[i] = load_halves4(qb + d, p.head_dim - d, p.q_vec);
+        b[i] = load_halves4(up + d, p.head_dim - d, p.up_k_vec);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mma_f16_16x8x16(acc, a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
+    }
+    *reinterpret_cast<float2*>(absorbed_row(ring_mem, g) + j * 8 + 2 * t) = make_float2(acc[0], acc[1]);
+    *reinterpret_cast<float2*>(absorbed_row(ring_mem, g + 8) + j * 8 + 2 * t) = make_float2(acc[2], acc[3]);
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// grid: (heads, batch * row tiles of 16, splits)
+template <bool kCap, bool kBias>
+__global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __grid_constant__ ChunkParams p, int row_tiles) {
+  extern __shared__ __align__(16) uint8_t ring_mem[];
+  __shared__ ChunkShared s;
+  grid_dependency_release();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+  const int h = blockIdx.x, b = blockIdx.y / row_tiles, row0 = (blockIdx.y % row_tiles) * kStreamRows, split = blockIdx.z;
+  const ChunkRequest r = chunk_request(p, b, h == 0 && row0 == 0 && split == 0 && threadIdx.x == 0);
+  const int rows = min(kStreamRows, r.n - row0);
+  if (rows <= 0) return;
+  const ChunkHead H = p.head[h];
+  const int rk = H.nk * 16, rv = H.nv * 16;
+
+  // the rows' visible keys, and the block's: from the smallest lo to the largest hi, cut to the split
+  if (threadIdx.x < kStreamRows) {
+    KeyRange k;
+    k.lo = k.hi = 0;
+    if (static_cast<int>(threadIdx.x) < rows)
+      k = visible_keys(p, r, p.b_prefix_len != nullptr ? p.b_prefix_len[b] : 0, row0 + threadIdx.x);
+    s.lo[threadIdx.x] = k.lo;
+    s.hi[threadIdx.x] = k.hi;
+  }
+  __syncthreads();
+  int kbeg = 0x7fffffff, kend = 0, inner_lo = 0, inner_hi = 0x7fffffff;    // inner: keys that every live row sees
+  for (int i = 0; i < rows; ++i) {
+    if (s.hi[i] > s.lo[i]) kbeg = min(kbeg, s.lo[i]);
+    kend = max(kend, s.hi[i]);
+    inner_lo = max(inner_lo, s.lo[i]);
+    inner_hi = min(inner_hi, s.hi[i]);
+  }
+  kbeg = max(kbeg & ~31, split * p.split_len);
+  if (p.splits > 1) kend = static_cast<int>(min(static_cast<int64_t>(kend), (static_cast<int64_t>(split) + 1) * p.split_len));
+  const int ntiles = kend > kbeg ? (kend - kbeg + 31) / 32 : 0;
+
+  if (ntiles == 0 && p.partials) {      // the merge reads no sums where the weights' sum is zero
+    if (static_cast<int>(threadIdx.x) < rows)
+      p.part_ml[(static_cast<int64_t>(split) * p.num_tokens + r.start + row0 + threadIdx.x) * p.num_heads + h] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+
+  const int32_t* r2t = p.req_to_token + static_cast<int64_t>(r.req) * p.req_to_token_stride;
+  const int8_t* kbase = p.cache_k + (p.head_major ? static_cast<int64_t>(H.k_col) * p.num_slots : H.k_col);
+  const int8_t* vbase = p.cache_v + (p.head_major ? static_cast<int64_t>(H.v_col) * p.num_slots : H.v_col);
+  const int64_t kstride = p.head_major ? rk : p.cache_k_row_stride, vstride = p.head_major ? rv : p.cache_v_row_stride;
+  const __half* ksc = p.scale_k + (p.head_major ? static_cast<int64_t>(h) * p.num_slots : h);
+  const __half* vsc = p.scale_v + (p.head_major ? static_cast<int64_t>(h) * p.num_slots : h);
+  const int64_t kss = p.head_major ? 1 : p.scale_k_row_stride, vss = p.head_major ? 1 : p.scale_v_row_stride;
+
+  const int stage_bytes = 32 * (rk + rv);
+  const int stages = stage_bytes * 8 <= kRingBytes ? 8 : (stage_bytes * 4 <= kRingBytes ? 4 : 2);
+  uint8_t* ring = ring_mem + warp * kRingBytes;
+  const int mine = ntiles > warp ? (ntiles - warp + kChunkWarps - 1) / kChunkWarps : 0;
+
+  // slot of this lane's key in tile `i` of the warp (-1: behind the end, unmapped or out of range)
+  auto fetch_slot = [&](int i) {
+    int slot = -1;
+    const int key = kbeg + (warp + i * kChunkWarps) * 32 + lane;
+    if (i < mine && key < kend) slot = r2t[key];
+    return slot;
+  };
+  const uint32_t inv_k = 65536u / H.nk + 1, inv_v = 65536u / H.nv + 1;     // x / n = x * inv >> 16 for x < 256, n <= 8
+  auto request = [&](int i, int slot) {
+    if (slot >= p.num_slots) {
+      report_status(p.status_word, LSVD_ERR_BOUNDS);
+      slot = -1;
+    }
+    const int st = i & (stages - 1);
+    s.slot[warp][st][lane] = slot;
+    uint8_t* kd = ring + st * stage_bytes;
+    uint8_t* vd = kd + 32 * rk;
+    for (int x = lane; x < 32 * H.nk; x += 32) {
+      const int tok = (x * inv_k) >> 16, piece = x - tok * H.nk;
+      const int sl = __shfl_sync(0xffffffffu, slot, tok);
+      // K rows lie in the order of the score columns (below), V rows in the order of the keys
+      const int row = (tok & ~7) | ((tok & 3) << 1) | ((tok >> 2) & 1);
+      cp_async16_or_zero(kd + row * rk + piece * 16, kbase + static_cast<int64_t>(max(sl, 0)) * kstride + piece * 16, sl >= 0);
+    }
+    for (int x = lane; x < 32 * H.nv; x += 32) {
+      const int tok = (x * inv_v) >> 16, piece = x - tok * H.nv;
+      const int sl = __shfl_sync(0xffffffffu, slot, tok);
+      cp_async16_or_zero(vd + tok * rv + piece * 16, vbase + static_cast<int64_t>(max(sl, 0)) * vstride + piece * 16, sl >= 0);
+    }
+  };
+  auto load_scales = [&](int i, float& a, float& c) {
+    a = c = 0.f;
+    if (i >= mine) return;
+    const int sl = s.slot[warp][i & (stages - 1)][lane];
+    if (sl >= 0) {
+      a = __half2float(ksc[sl * kss]);
+      c = __half2float(vsc[sl * vss]);
+    }
+  };
+
+  // the first stages are on their way while the query rows are absorbed
+  int slot_next = fetch_slot(0);
+  for (int i = 0; i < stages - 1; ++i) {
+    const int slot = slot_next;
+    slot_next = fetch_slot(i + 1);
+    if (i < mine) request(i, slot);
+    cp_async_commit();
+  }
+  float sk_next, sv_next;
+  load_scales(0, sk_next, sv_next);
+
+  absorb_rows(p, H, h, r, row0, rows, ring_mem);
+  __syncthreads();
+  const float *qt_a = absorbed_row(ring_mem, g), *qt_b = absorbed_row(ring_mem, g + 8);
+  // q~ as fp16 A fragments: step (mb, i) of a 64-rank block holds ranks 64 mb + 16 t + 4 i .. + 3 of lane (g, t)
+  uint32_t qa[2][4][4];
+  float fa, fb;                       // score scale of rows g and g + 8, with the power of two that was taken out
+  {
+    float ma = 0.f, mb_ = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int rank = 64 * mb + 16 * t4 + 4 * i;
+        if (rank < rk) {
+          const float4 x = *reinterpret_cast<const float4*>(qt_a + rank), y = *reinterpret_cast<const float4*>(qt_b + rank);
+          ma = fmaxf(ma, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+          mb_ = fmaxf(mb_, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+        }
+      }
+    ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
+    ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, 2));
+    mb_ = fmaxf(mb_, __shfl_xor_sync(0xffffffffu, mb_, 1));
+    mb_ = fmaxf(mb_, __shfl_xor_sync(0xffffffffu, mb_, 2));
+    const int ea = exponent_of(ma) - 8, eb = exponent_of(mb_) - 8;       // entries end up below 2^9
+    const float xa = pow2i(-ea), xb = pow2i(-eb);
+    fa = p.score_scale * pow2i(ea);
+    fb = p.score_scale * pow2i(eb);
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int rank = 64 * mb + 16 * t4 + 4 * i;
+        qa[mb][i][0] = qa[mb][i][1] = qa[mb][i][2] = qa[mb][i][3] = 0u;
+        if (rank < rk) {
+          const float4 x = *reinterpret_cast<const float4*>(qt_a + rank), y = *reinterpret_cast<const float4*>(qt_b + rank);
+          qa[mb][i][0] = pack_half2(x.x * xa, x.y * xa);
+          qa[mb][i][1] = pack_half2(y.x * xb, y.y * xb);
+          qa[mb][i][2] = pack_half2(x.z * xa, x.w * xa);
+          qa[mb][i][3] = pack_half2(y.z * xb, y.w * xb);
+        }
+      }
+  }
+  __syncthreads();                    // the rings' last stages may be written from here on
+  const float cap_log2e = p.softcap * kChunkLog2e;
+  if (kCap) {
+    fa *= 2.f * kChunkLog2e / p.softcap;
+    fb *= 2.f * kChunkLog2e / p.softcap;
+  } else {
+    fa *= kChunkLog2e;
+    fb *= kChunkLog2e;
+  }
+  const int lo_a = s.lo[g], hi_a = s.hi[g], lo_b = s.lo[g + 8], hi_b = s.hi[g + 8];
+  const int pos_a = r.len - r.n + row0 + g, pos_b = pos_a + 8;
+  const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
+
+  float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+  int E = -200;                       // exponent of the largest V scale so far
+  float o[2][8][4];
+#pragma unroll
+  for (int vb = 0; vb < 2; ++vb)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[vb][j][0] = o[vb][j][1] = o[vb][j][2] = o[vb][j][3] = 0.f;
+
+  for (int i = 0; i < mine; ++i) {
+    {
+      const int slot = slot_next;
+      slot_next = fetch_slot(i + stages);
+      __syncwarp();                   // every lane is done with the stage that is refilled now
+      if (i + stages - 1 < mine) request(i + stages - 1, slot);
+      cp_async_commit();
+    }
+    const float sk = sk_next, sv = sv_next;
+    const int st = i & (stages - 1);
+    const int my_slot = s.slot[warp][st][lane];
+    const uint32_t valid = __ballot_sync(0xffffffffu, my_slot >= 0);
+    load_scales(i + 1, sk_next, sv_next);
+    // V scales relative to the largest one: a larger one than before moves the accumulators' exponent
+    int e_new = E;
+    {
+      const float av = fabsf(sv);
+      const int e = (av > 0.f && av < INFINITY) ? exponent_of(av) : -200;
+      e_new = max(E, __reduce_max_sync(0xffffffffu, e));
+    }
+    s.sk[warp][lane] = sk;
+    s.sv[warp][lane] = sv * pow2i(kWeightShift - e_new);
+    if (stages == 8) cp_async_wait<7>();
+    else if (stages == 4) cp_async_wait<3>();
+    else cp_async_wait<1>();
+    __syncwarp();
+    const uint8_t* kd = ring + st * stage_bytes;
+    const uint8_t* vd = kd + 32 * rk;
+
+    // scores of 32 keys in four 8-key tiles; column c = 2 t' + e of tile j = 2 m + jj is key 16 m + 8 jj + t' + 4 e
+    float x[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+        if (mb * 4 < H.nk) {
+          uint4 w = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+          if (mb * 4 + t4 < H.nk) {
+            w = *reinterpret_cast<const uint4*>(kd + (8 * j + g) * rk + (mb * 4 + t4) * 16);
+            w.x ^= 0x80808080u; w.y ^= 0x80808080u; w.z ^= 0x80808080u; w.w ^= 0x80808080u;
+          }
+          uint32_t b0, b1;
+          codes_to_half(w.x, b0, b1);
+          mma_f16_16x8x16(x[j], qa[mb][0][0], qa[mb][0][1], qa[mb][0][2], qa[mb][0][3], b0, b1);
+          codes_to_half(w.y, b0, b1);
+          mma_f16_16x8x16(x[j], qa[mb][1][0], qa[mb][1][1], qa[mb][1][2], qa[mb][1][3], b0, b1);
+          codes_to_half(w.z, b0, b1);
+          mma_f16_16x8x16(x[j], qa[mb][2][0], qa[mb][2][1], qa[mb][2][2], qa[mb][2][3], b0, b1);
+          codes_to_half(w.w, b0, b1);
+          mma_f16_16x8x16(x[j], qa[mb][3][0], qa[mb][3][1], qa[mb][3][2], qa[mb][3][3], b0, b1);
+        }
+      }
+    }
+    const int key0 = kbeg + (warp + i * kChunkWarps) * 32;
+    const bool masked = key0 < inner_lo || key0 + 32 > inner_hi || valid != 0xffffffffu;
+    float top_a = -INFINITY, top_b = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int k = 8 * j + t4 + 4 * e;
+        const float c = s.sk[warp][k];
+        float xa = x[j][e] * (c * fa), xb = x[j][2 + e] * (c * fb);
+        if (kCap) {
+          xa = capped_log2(xa, cap_log2e);
+          xb = capped_log2(xb, cap_log2e);
+        }
+        if (kBias) {
+          xa -= slope * fabsf(static_cast<float>(pos_a - key0 - k));
+          xb -= slope * fabsf(static_cast<float>(pos_b - key0 - k));
+        }
+        if (masked) {
+          const bool live = (valid >> k) & 1u;
+          if (!live || key0 + k < lo_a || key0 + k >= hi_a) xa = -INFINITY;
+          if (!live || key0 + k < lo_b || key0 + k >= hi_b) xb = -INFINITY;
+        }
+        x[j][e] = xa;
+        x[j][2 + e] = xb;
+        top_a = fmaxf(top_a, xa);
+        top_b = fmaxf(top_b, xb);
+      }
+    }
+    top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, 1));
+    top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, 2));
+    top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 1));
+    top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 2));
+    const float n_a = fmaxf(m_a, top_a), n_b = fmaxf(m_b, top_b);
+    const float base_a = n_a == -INFINITY ? 0.f : n_a, base_b = n_b == -INFINITY ? 0.f : n_b;
+    if (__any_sync(0xffffffffu, n_a != m_a || n_b != m_b || e_new != E)) {
+      const float c_a = ex2(m_a - base_a), c_b = ex2(m_b - base_b);       // a first maximum: 2^-inf = 0
+      l_a *= c_a;
+      l_b *= c_b;
+      const float shift = pow2i(max(E - e_new, -126));
+      const float s_a = c_a * shift, s_b = c_b * shift;
+#pragma unroll
+      for (int vb = 0; vb < 2; ++vb)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          o[vb][j][0] *= s_a;
+          o[vb][j][1] *= s_a;
+          o[vb][j][2] *= s_b;
+          o[vb][j][3] *= s_b;
+        }
+      m_a = n_a;
+      m_b = n_b;
+      E = e_new;
+    }
+    uint32_t w[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float p0 = ex2(x[j][0] - base_a), p1 = ex2(x[j][1] - base_a), p2 = ex2(x[j][2] - base_b), p3 = ex2(x[j][3] - base_b);
+      l_a += p0 + p1;
+      l_b += p2 + p3;
+      const float v0 = s.sv[warp][8 * j + t4], v1 = s.sv[warp][8 * j + t4 + 4];
+      // a masked key's weight is zero whatever its scale holds
+      w[j][0] = pack_half2(p0 == 0.f ? 0.f : p0 * v0, p1 == 0.f ? 0.f : p1 * v1);
+      w[j][1] = pack_half2(p2 == 0.f ? 0.f : p2 * v0, p3 == 0.f ? 0.f : p3 * v1);
+    }
+    // values: rank 64 vb + 8 g + n of lane (g, t) is column g of tile n; the keys of step m are the score columns' keys
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int vb = 0; vb < 2; ++vb) {
+        if (vb * 4 < H.nv) {
+          uint2 ra = make_uint2(0x80808080u, 0x80808080u), rb = ra, rc = ra, rd = ra;
+          if (64 * vb + 8 * g < rv) {
+            const uint8_t* at = vd + (16 * m + t4) * rv + 64 * vb + 8 * g;
+            ra = *reinterpret_cast<const uint2*>(at);
+            rb = *reinterpret_cast<const uint2*>(at + 4 * rv);
+            rc = *reinterpret_cast<const uint2*>(at + 8 * rv);
+            rd = *reinterpret_cast<const uint2*>(at + 12 * rv);
+            ra.x ^= 0x80808080u; ra.y ^= 0x80808080u; rb.x ^= 0x80808080u; rb.y ^= 0x80808080u;
+            rc.x ^= 0x80808080u; rc.y ^= 0x80808080u; rd.x ^= 0x80808080u; rd.y ^= 0x80808080u;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {       // two ranks at a time: bytes 2 (q & 1), + 1 of word q >> 1
+            const uint32_t sel = (q & 1) ? 0x7362u : 0x5140u;
+            const uint32_t u = __byte_perm(q < 2 ? ra.x : ra.y, q < 2 ? rb.x : rb.y, sel);
+            const uint32_t v = __byte_perm(q < 2 ? rc.x : rc.y, q < 2 ? rd.x : rd.y, sel);
+            uint32_t b0, b1, c0, c1;
+            codes_to_half(u, b0, c0);         // {key t, key t + 4} of the first rank, of the second
+            codes_to_half(v, b1, c1);         // {key t + 8, key t + 12}
+            mma_f16_16x8x16(o[vb][2 * q], w[2 * m][0], w[2 * m][1], w[2 * m + 1][0], w[2 * m + 1][1], b0, b1);
+            mma_f16_16x8x16(o[vb][2 * q + 1], w[2 * m][0], w[2 * m][1], w[2 * m + 1][0], w[2 * m + 1][1], c0, c1);
+          }
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+
+  // join the four warps: common maximum per row, sums in shared memory (the rings are done with)
+  l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
+  l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
+  l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
+  l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
+  if (t4 == 0) {
+    s.m[warp][g] = m_a;
+    s.m[warp][g + 8] = m_b;
+    s.l[warp][g] = l_a;
+    s.l[warp][g + 8] = l_b;
+  }
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(ring_mem) + warp * (kStreamRows * LSVD_MAX_RANK);
+  float top_a = s.m[0][g], top_b = s.m[0][g + 8];
+#pragma unroll
+  for (int w = 1; w < kChunkWarps; ++w) {
+    top_a = fmaxf(top_a, s.m[w][g]);
+    top_b = fmaxf(top_b, s.m[w][g + 8]);
+  }
+  const float back = E > -200 ? pow2i(E - kWeightShift) : 1.f;
+  const float s_a = ex2(m_a - (top_a == -INFINITY ? 0.f : top_a)) * back, s_b = ex2(m_b - (top_b == -INFINITY ? 0.f : top_b)) * back;
+#pragma unroll
+  for (int vb = 0; vb < 2; ++vb)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int rank = 64 * vb + 16 * t4 + 8 * e;
+      if (rank < rv) {
+        float4* da = reinterpret_cast<float4*>(sums + g * LSVD_MAX_RANK + rank);
+        float4* db = reinterpret_cast<float4*>(sums + (g + 8) * LSVD_MAX_RANK + rank);
+        da[0] = make_float4(o[vb][0][e] * s_a, o[vb][1][e] * s_a, o[vb][2][e] * s_a, o[vb][3][e] * s_a);
+        da[1] = make_float4(o[vb][4][e] * s_a, o[vb][5][e] * s_a, o[vb][6][e] * s_a, o[vb][7][e] * s_a);
+        db[0] = make_float4(o[vb][0][2 + e] * s_b, o[vb][1][2 + e] * s_b, o[vb][2][2 + e] * s_b, o[vb][3][2 + e] * s_b);
+        db[1] = make_float4(o[vb][4][2 + e] * s_b, o[vb][5][2 + e] * s_b, o[vb][6][2 + e] * s_b, o[vb][7][2 + e] * s_b);
+      }
+    }
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(ring_mem);
+  for (int x = threadIdx.x; x < rows * rv; x += kChunkThreads) {
+    const int row = x / rv, rank = x - row * rv;
+    const int token = r.start + row0 + row;
+    float top = s.m[0][row], sum = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 1; w < kChunkWarps; ++w) top = fmaxf(top, s.m[w][row]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < kChunkWarps; ++w) {
+      sum += s.l[w][row] * ex2(s.m[w][row] - base);
+      v += all[w * (kStreamRows * LSVD_MAX_RANK) + row * LSVD_MAX_RANK + rank];
+    }
+    if (p.partials) {
+      const int64_t at = static_cast<int64_t>(split) * p.num_tokens + token;
+      p.part_o[at * p.sum_rv + H.v_col + rank] = v;
+      if (rank == 0) p.part_ml[at * p.num_heads + h] = make_float2(top, sum);
+    } else {
+      p.out_latent[token * p.out_latent_stride_t + H.v_col + rank] = __float2half_rn(sum == 0.f ? 0.f : v / sum);
+    }
+  }
+}
+
+// Joins the splits of a row and applies the V up-factor: grid (heads, tiles of 8 rows).
+constexpr int kMergeRows = 8;
+__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
+  __shared__ float lat[kMergeRows][LSVD_MAX_RANK];
+  __shared__ bool live[kMergeRows];
+  grid_dependency_release();
+  grid_dependency_wait();
+  const int h = blockIdx.x, token0 = blockIdx.y * kMergeRows;
+  const ChunkHead H = p.head[h];
+  const int rv = H.nv * 16;
+  if (threadIdx.x < kMergeRows) {
+    const int token = token0 + threadIdx.x;
+    int lo = 0, hi = p.batch - 1;               // last request whose first row is not behind the token
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (p.b_start_loc[mid] <= token) lo = mid; else hi = mid - 1;
+    }
+    const ChunkRequest r = chunk_request(p, lo, false);
+    live[threadIdx.x] = token < p.num_tokens && token >= r.start && token < r.start + r.n;
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < kMergeRows * rv; x += blockDim.x) {
+    const int row = x / rv, rank = x - row * rv, token = token0 + row;
+    if (!live[row]) continue;
+    float top = -INFINITY;
+    for (int s = 0; s < p.splits; ++s)
+      top = fmaxf(top, p.part_ml[(static_cast<int64_t>(s) * p.num_tokens + token) * p.num_heads + h].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, v = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const int64_t at = static_cast<int64_t>(s) * p.num_tokens + token;
+      const float2 ml = p.part_ml[at * p.num_heads + h];
+      if (ml.y == 0.f) continue;                // nothing seen in this split
+      const float c = ex2(ml.x - base);
+      sum += ml.y * c;
+      v += p.part_o[at * p.sum_rv + H.v_col + rank] * c;
+    }
+    v = sum == 0.f ? 0.f : v / sum;
+    lat[row][rank] = v;
+    if (p.out_latent != nullptr) p.out_latent[token * p.out_latent_stride_t + H.v_col + rank] = __float2half_rn(v);
+  }
+  if (p.out == nullptr) return;
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.head_dim; d += blockDim.x) {
+    float acc[kMergeRows];
+#pragma unroll
+    for (int i = 0; i < kMergeRows; ++i) acc[i] = 0.f;
+    for (int rank = 0; rank < rv; ++rank) {
+      const float w = __half2float(p.up_v[static_cast<int64_t>(H.v_col + rank) * p.up_v_row_stride + d]);
+#pragma unroll
+      for (int i = 0; i < kMergeRows; ++i) acc[i] = fmaf(w, lat[i][rank], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kMergeRows; ++i)
+      if (live[i]) p.out[(token0 + i) * p.out_stride_t + h * p.out_stride_h + d] = __float2half_rn(acc[i]);
+  }
+}
+
+struct ChunkPlan {
+  int row_tiles, splits, split_len;
+};
+
+// The stream form's split of the keys: enough blocks for six rounds of the resident ones (three per SM), no piece shorter
+// than 256 keys.
+static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_new, int max_len) {
+  ChunkPlan c;
+  c.row_tiles = std::max(1, (std::min(max_new, num_tokens) + kStreamRows - 1) / kStreamRows);
+  const int64_t blocks = static_cast<int64_t>(num_heads) * std::min<int64_t>(static_cast<int64_t>(batch) * c.row_tiles, batch + num_tokens / kStreamRows);
+  const int64_t want = 6LL * 3 * std::max(1, device_sm_count());
+  const int64_t most = std::max(1, max_len / 256);
+  c.splits = static_cast<int>(std::max<int64_t>(1, std::min(most, std::min<int64_t>(want / std::max<int64_t>(1, blocks), 128))));
+  c.split_len = std::max(128, (max_len + c.splits - 1) / c.splits);
+  c.split_len = (c.split_len + 127) / 128 * 128;
+  c.splits = std::max(1, (max_len + c.split_len - 1) / c.split_len);
+  return c;
+}
+
+static size_t chunk_align(size_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace lsvd
+
+extern "C" size_t lsvd_attn_chunk_workspace_bytes(int32_t batch, int32_t num_heads, int32_t sum_rank_v, int32_t num_tokens,
+                                                  int32_t max_new_in_batch, int32_t max_len_in_batch) {
+  using namespace lsvd;
+  if (batch <= 0 || num_heads <= 0 || sum_rank_v <= 0 || num_tokens < 0 || max_new_in_batch < 0 || max_len_in_batch < 0) return 0;
+  const ChunkPlan c = chunk_plan(batch, num_heads, num_tokens, max_new_in_batch, max_len_in_batch);
+  const size_t rows = static_cast<size_t>(c.splits) * std::max(1, num_tokens);
+  return chunk_align(rows * num_heads * sizeof(float2)) + chunk_align(rows * sum_rank_v * sizeof(float));
+}
+
+extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
+  using namespace lsvd;
+  if (a == nullptr) return LSVD_ERR_INVALID_ARG;
+  if (a->batch <= 0 || a->num_heads <= 0 || a->num_heads > LSVD_MAX_HEADS) return LSVD_ERR_INVALID_ARG;
+  if (a->head_dim <= 0 || a->head_dim > 256 || (a->head_dim % 8) != 0) return LSVD_ERR_INVALID_ARG;
+  if (a->num_slots <= 0 || a->max_len_in_batch < 0 || a->num_tokens < 0 || a->max_new_in_batch < 0) return LSVD_ERR_INVALID_ARG;
+  if (!a->k_off || !a->v_off || a->k_off[0] != 0 || a->v_off[0] != 0) return LSVD_ERR_INVALID_ARG;
+  ChunkParams p{};
+  for (int h = 0; h < a->num_heads; ++h) {
+    const int rk = a->k_off[h + 1] - a->k_off[h], rv = a->v_off[h + 1] - a->v_off[h];
+    if (rk <= 0 || rv <= 0 || rk > LSVD_MAX_RANK || rv > LSVD_MAX_RANK || (rk % 16) != 0 || (rv % 16) != 0) return LSVD_ERR_INVALID_ARG;
+    p.head[h] = {a->k_off[h], a->v_off[h], static_cast<int16_t>(rk / 16), static_cast<int16_t>(rv / 16)};
+  }
+  const int sum_rk = a->k_off[a->num_heads], sum_rv = a->v_off[a->num_heads];
+  if (a->num_tokens == 0) return LSVD_OK;
+  if (!a->q || !a->cache_k || !a->cache_v || !a->scale_k || !a->scale_v || !a->up_k || !a->req_to_token || !a->b_req_idx ||
+      !a->b_seq_len || !a->b_start_loc)
+    return LSVD_ERR_INVALID_ARG;
+  if ((a->out == nullptr && a->out_latent == nullptr) || (a->out != nullptr && a->up_v == nullptr)) return LSVD_ERR_INVALID_ARG;
+  if (a->cache_layout != LSVD_CACHE_SLOT_MAJOR && a->cache_layout != LSVD_CACHE_HEAD_MAJOR) return LSVD_ERR_INVALID_ARG;
+  if (!aligned(a->cache_k, 16) || !aligned(a->cache_v, 16)) return LSVD_ERR_INVALID_ARG;
+  if (a->cache_layout == LSVD_CACHE_SLOT_MAJOR &&
+      ((a->cache_k_row_stride % 16) != 0 || (a->cache_v_row_stride % 16) != 0 || a->cache_k_row_stride < sum_rk ||
+       a->cache_v_row_stride < sum_rv || a->scale_k_row_stride < a->num_heads || a->scale_v_row_stride < a->num_heads))
+    return LSVD_ERR_INVALID_ARG;
+  const void* halves[] = {a->q, a->up_k, a->up_v, a->scale_k, a->scale_v, a->out, a->out_latent};
+  for (const void* x : halves)
+    if (!aligned(x, 2)) return LSVD_ERR_INVALID_ARG;
+  const void* words[] = {a->req_to_token, a->b_req_idx, a->b_seq_len, a->b_start_loc, a->alibi_slopes, a->b_prefix_len, a->key_begin,
+                         a->status_word};
+  for (const void* x : words)
+    if (!aligned(x, 4)) return LSVD_ERR_INVALID_ARG;
+  if (a->up_k_row_stride < a->head_dim || (a->out != nullptr && a->up_v_row_stride < a->head_dim)) return LSVD_ERR_INVALID_ARG;
+  if (a->req_to_token_rows <= 0 || (a->req_to_token_rows > 1 && a->req_to_token_stride < a->max_len_in_batch)) return LSVD_ERR_INVALID_ARG;
+  if (std::isnan(a->softcap) || std::isinf(a->softcap)) return LSVD_ERR_INVALID_ARG;
+  const ChunkPlan c = chunk_plan(a->batch, a->num_heads, a->num_tokens, a->max_new_in_batch, a->max_len_in_batch);
+  const int64_t row_blocks = static_cast<int64_t>(a->batch) * c.row_tiles;
+  if (row_blocks > 65535 || (a->num_tokens + kMergeRows - 1) / kMergeRows > 65535) return LSVD_ERR_UNSUPPORTED;
+  const bool partials = c.splits > 1 || a->out != nullptr;
+  const size_t need = lsvd_attn_chunk_workspace_bytes(a->batch, a->num_heads, sum_rv, a->num_tokens, a->max_new_in_batch, a->max_len_in_batch);
+  if (partials && (a->workspace == nullptr || a->workspace_bytes < need || !aligned(a->workspace, 256))) return LSVD_ERR_WORKSPACE;
+
+  p.q = static_cast<const __half*>(a->q);
+  p.q_stride_t = a->q_stride_t;
+  p.q_stride_h = a->q_stride_h;
+  p.cache_k = a->cache_k;
+  p.cache_v = a->cache_v;
+  p.scale_k = static_cast<const __half*>(a->scale_k);
+  p.scale_v = static_cast<const __half*>(a->scale_v);
+  p.cache_k_row_stride = a->cache_k_row_stride;
+  p.cache_v_row_stride = a->cache_v_row_stride;
+  p.scale_k_row_stride = a->scale_k_row_stride;
+  p.scale_v_row_stride = a->scale_v_row_stride;
+  p.up_k = static_cast<const __half*>(a->up_k);
+  p.up_v = static_cast<const __half*>(a->up_v);
+  p.up_k_row_stride = a->up_k_row_stride;
+  p.up_v_row_stride = a->up_v_row_stride;
+  p.req_to_token = a->req_to_token;
+  p.req_to_token_stride = a->req_to_token_stride;
+  p.b_req_idx = a->b_req_idx;
+  p.b_seq_len = a->b_seq_len;
+  p.b_start_loc = a->b_start_loc;
+  p.out = static_cast<__half*>(a->out);
+  p.out_stride_t = a->out_stride_t;
+  p.out_stride_h = a->out_stride_h;
+  p.out_latent = static_cast<__half*>(a->out_latent);
+  p.out_latent_stride_t = a->out_latent_stride_t;
+  p.status_word = a->status_word;
+  p.alibi_slopes = a->alibi_slopes;
+  p.b_prefix_len = a->b_prefix_len;
+  p.key_begin = a->key_begin;
+  p.score_scale = a->sm_scale > 0.f ? a->sm_scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
+  p.softcap = a->softcap;
+  p.batch = a->batch;
+  p.num_heads = a->num_heads;
+  p.head_dim = a->head_dim;
+  p.max_len = a->max_len_in_batch;
+  p.num_tokens = a->num_tokens;
+  p.max_new = a->max_new_in_batch;
+  p.num_slots = a->num_slots;
+  p.r2t_rows = a->req_to_token_rows;
+  p.causal = a->causal;
+  p.window = a->window;
+  p.head_major = a->cache_layout == LSVD_CACHE_HEAD_MAJOR ? 1 : 0;
+  p.sum_rv = sum_rv;
+  p.q_vec = aligned(a->q, 8) && (a->q_stride_t % 4) == 0 && (a->q_stride_h % 4) == 0;
+  p.up_k_vec = aligned(a->up_k, 8) && (a->up_k_row_stride % 4) == 0;
+  p.splits = c.splits;
+  p.split_len = c.split_len;
+  p.partials = partials;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.part_ml = reinterpret_cast<float2*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + chunk_align(static_cast<size_t>(c.splits) * a->num_tokens * a->num_heads * sizeof(float2)));
+
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool cap = a->softcap > 0.f, bias = a->alibi_slopes != nullptr;
+  void (*kern)(ChunkParams, int) = cap ? (bias ? chunk_stream_kernel<true, true> : chunk_stream_kernel<true, false>)
+                                       : (bias ? chunk_stream_kernel<false, true> : chunk_stream_kernel<false, false>);
+  const int smem = kChunkWarps * kRingBytes;
+  LSVD_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem));
+  LSVD_CUDA_TRY(launch_chained(kern, dim3(a->num_heads, static_cast<unsigned>(row_blocks), c.splits), dim3(kChunkThreads), smem, st, 1, true,
+                               p, c.row_tiles));
+  if (partials)
+    LSVD_CUDA_TRY(launch_chained(chunk_merge_kernel, dim3(a->num_heads, (a->num_tokens + kMergeRows - 1) / kMergeRows), dim3(128), 0, st, 1,
+                                 true, p));
+  return LSVD_OK;
+}

@@ -1,0 +1,128 @@
+// Shared by the kernels of the chunk attention (attn_chunk.cu, attn_chunk_tile.cu): parameters, the visible range of a
+// query token, the scores' cap and bias.
+#pragma once
+
+#include "common.cuh"
+
+namespace lsvd {
+
+constexpr float kChunkLog2e = 1.4426950408889634f;
+constexpr int kStreamRows = 16;      // query rows of a block of the stream form
+
+struct ChunkHead {
+  int32_t k_col, v_col;      // byte offsets of the head inside a K / V cache row
+  int16_t nk, nv;            // 16-entry pieces of K and V
+};
+
+struct ChunkParams {
+  const __half* q;
+  int64_t q_stride_t, q_stride_h;
+  const int8_t* cache_k;
+  const int8_t* cache_v;
+  const __half* scale_k;
+  const __half* scale_v;
+  int64_t cache_k_row_stride, cache_v_row_stride, scale_k_row_stride, scale_v_row_stride;
+  const __half* up_k;
+  const __half* up_v;
+  int64_t up_k_row_stride, up_v_row_stride;
+  const int32_t* req_to_token;
+  int64_t req_to_token_stride;
+  const int32_t* b_req_idx;
+  const int32_t* b_seq_len;
+  const int32_t* b_start_loc;
+  __half* out;
+  int64_t out_stride_t, out_stride_h;
+  __half* out_latent;
+  int64_t out_latent_stride_t;
+  float2* part_ml;           // [split][row][head]: running maximum (log2 domain) and sum
+  float* part_o;             // [split][row][sum r_v]: unnormalised sums
+  int32_t* status_word;
+  const float* alibi_slopes;
+  const int32_t* b_prefix_len;
+  const int32_t* key_begin;
+  float score_scale;         // sm_scale
+  float softcap;
+  int32_t batch, num_heads, head_dim, max_len, num_tokens, max_new, num_slots, r2t_rows;
+  int32_t causal, window, head_major, sum_rv;
+  int32_t q_vec, up_k_vec;   // rows of q / up_k can be read in 8-byte pieces
+  int32_t splits, split_len; // keys [s * split_len, (s + 1) * split_len) of the stream form's split s
+  int32_t partials;          // results go to part_ml / part_o, for the merge
+  ChunkHead head[LSVD_MAX_HEADS];
+};
+
+#ifdef __CUDACC__
+// A request, checked: its first row, its new tokens (0: skip it), its length and its row of the slot table.
+struct ChunkRequest {
+  int start, n, len, req;
+};
+
+// `report`: one thread per request says what was wrong.
+__device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int b, bool report) {
+  ChunkRequest r;
+  r.start = min(max(p.b_start_loc[b], 0), p.num_tokens);
+  const int end = min(max(p.b_start_loc[b + 1], 0), p.num_tokens);
+  r.n = max(end - r.start, 0);
+  r.len = p.b_seq_len[b];
+  r.req = p.b_req_idx[b];
+  bool bad = r.len > p.max_len || r.n > p.max_new;
+  if (r.len > p.max_len) r.len = p.max_len;
+  if (r.n > p.max_new) r.n = 0;
+  if (r.len < 0) r.len = 0;
+  if (static_cast<uint32_t>(r.req) >= static_cast<uint32_t>(p.r2t_rows)) {
+    bad = true;
+    r.req = 0;
+    r.len = 0;
+  }
+  if (bad && report) report_status(p.status_word, LSVD_ERR_BOUNDS);
+  return r;
+}
+
+struct KeyRange {
+  int lo, hi;      // keys lo <= t < hi are seen; lo >= hi: none
+};
+
+// Causal, sliding-window, prefix and document masks all leave a query token one run of keys.
+__device__ __forceinline__ KeyRange visible_keys(const ChunkParams& p, const ChunkRequest& r, int prefix, int i) {
+  const int pos = r.len - r.n + i;
+  KeyRange k;
+  k.lo = 0;
+  k.hi = r.len;
+  if (p.causal) k.hi = min(r.len, max(pos + 1, prefix));
+  if (p.window > 0) {
+    k.lo = max(0, static_cast<int>(max(static_cast<int64_t>(pos) + 1 - p.window, static_cast<int64_t>(0))));
+    if (!p.causal) k.hi = static_cast<int>(min(static_cast<int64_t>(r.len), static_cast<int64_t>(pos) + p.window));
+  }
+  if (p.key_begin != nullptr) k.lo = max(k.lo, p.key_begin[r.start + i]);
+  if (k.hi <= k.lo) k.lo = k.hi = 0;
+  return k;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// cap * tanh(x / cap) * log2(e) of u = x * 2 log2(e) / cap: tanh(y) = 1 - 2 / (1 + e^(2y)), off by a few 2^-24 of the cap
+// (the hardware's tanh is off by 2^-11 of it, half a unit of a score at a cap of 1000, 2 % of a weight at 50).
+__device__ __forceinline__ float capped_log2(float u, float cap_log2e) {
+  return fmaf(__fdividef(-2.f, 1.f + ex2(u)), cap_log2e, cap_log2e);
+}
+
+// Exponent e with 2^e <= x < 2^(e+1) for a positive normal x (0 for what is not positive and finite).
+__device__ __forceinline__ int exponent_of(float x) {
+  return (x > 0.f && x < INFINITY) ? static_cast<int>((__float_as_uint(x) >> 23) & 255u) - 127 : 0;
+}
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23); }
+
+// Four int8 codes (already xored with 0x80808080, i.e. code + 128) as two fp16 pairs: 0x6400 | u is 1024 + u, exactly.
+__device__ __forceinline__ void codes_to_half(uint32_t u, uint32_t& lo, uint32_t& hi) {
+  const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 off = __floats2half2_rn(-1152.f, -1152.f);
+  const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&a), off), y = __hadd2(*reinterpret_cast<const __half2*>(&b), off);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+#endif
+
+}  // namespace lsvd

@@ -159,3 +159,109 @@ def decode_rope_recon(q16, cache_k, scale_k, cache_v, scale_v, wk_q, wk_scale16,
             v = cache_v[rows, hk].float() * scale_v[rows, hk].float()[:, None]
             out[b, h] = p @ v
     return out.half()
+
+
+def chunk_maps(req, ready, new, table, page, r2t, num_tokens, num_slots, free=None, head=0, rebuild=False):
+    """Slots of a step's new tokens, entry by entry (lists of Python integers; ``table`` and ``r2t`` are changed in place).
+
+    Returns (start, seq, mem_index, position_ids, head, refused) with ``refused`` the entries that got nothing: their row or
+    length does not fit the tables, their tokens do not fit ``num_tokens``, an earlier entry adds tokens to the same row, or
+    the free pages have run out.
+    """
+    up = lambda tokens: -(-tokens // page)
+    start, seq, refused, seen, dry = [0], [], [], set(), False
+    mem, pos = [-1] * num_tokens, [0] * num_tokens
+    h = head
+    for b, (row, old, n) in enumerate(zip(req, ready, new)):
+        first = start[-1]
+        start.append(first + max(n, 0))
+        ok = 0 <= row < len(table) and old >= 0 and n >= 0 and old + n <= len(r2t[0]) and old + n <= len(table[0]) * page
+        ok = ok and start[-1] <= num_tokens
+        if ok and n > 0:
+            ok = row not in seen
+            seen.add(row)
+        need = up(old + n) - up(old) if ok and free is not None else 0
+        if need and (dry or not 0 <= head <= len(free) or h + need > len(free)):
+            dry, ok = True, False
+        if not ok:
+            refused.append(b)
+            seq.append(max(old, 0))
+            continue
+        for j in range(need):
+            table[row][up(old) + j] = free[h + j]
+        h += need
+        slot = lambda t: table[row][t // page] * page + t % page if 0 <= table[row][t // page] * page <= num_slots - page else -1
+        for t in range(0 if rebuild else old, old + n):
+            r2t[row][t] = slot(t)
+        for i in range(n):
+            mem[first + i], pos[first + i] = slot(old + i), old + i
+        seq.append(old + n)
+    return [min(x, num_tokens) for x in start], seq, mem, pos, h, refused
+
+
+def chunk_absorb(q16, cache_k, scale_k, cache_v, scale_v, up_k16, up_v16, k_off, v_off, req_to_token, b_req_idx, b_seq_len,
+                 b_start_loc, sm_scale=None, causal=True, window=0, prefix=None, key_begin=None, softcap=0.0, slopes=None):
+    """Attention of several new tokens per request in 64 bits, and how far a kernel may be off.
+
+    Keys are rebuilt (no absorbed query): x = sm_scale s_k (z_k B_k) . q, capped, biased, masked; o_lat = sum p s_v z_v,
+    o = B_v^T o_lat.  Returns (o [T, H, D], o_lat [T, sum r_v], their bounds); rows of no request are NaN.
+
+    The bounds follow from the kernels' roundings, each half a step: the absorbed query in fp16 (2^-11 of every term of a
+    score: dx), fp32 arithmetic on scores (2^-21 of the largest score or bias, or of the cap), weights p s_v in fp16 (2^-11 of
+    every term), sums in fp32 (2^-20), the result in fp16 (2^-11, or half a step of 2^-24 below the normal range).  A score
+    off by dx changes a weight by e^dx and the sum of weights by as much: 2 dx of every term.
+    """
+    T, H, D = q16.shape
+    sm = 1.0 / math.sqrt(D) if sm_scale is None else sm_scale
+    f = lambda t: t.double()
+    nan = float("nan")
+    o, lat = torch.full((T, H, D), nan, dtype=torch.float64), torch.full((T, v_off[-1]), nan, dtype=torch.float64)
+    o_tol, lat_tol = torch.zeros_like(o), torch.zeros_like(lat)
+    half = lambda v, e: e + 2.0 ** -11 * (v.abs() + e) + 2.0 ** -25
+    for b in range(len(b_seq_len)):
+        a, e = int(b_start_loc[b]), int(b_start_loc[b + 1])
+        n, L = e - a, int(b_seq_len[b])
+        rows = req_to_token[int(b_req_idx[b]), :L].long()
+        real = rows >= 0
+        rows = rows.clamp_min(0)
+        i = torch.arange(L - n, L)[:, None]
+        t = torch.arange(L)[None, :]
+        sees = (t <= i) | ((t < int(prefix[b])) if prefix is not None else torch.zeros(1, L, dtype=torch.bool)) if causal \
+            else ((t - i < window) if window > 0 else torch.ones(n, L, dtype=torch.bool))
+        if window > 0:
+            sees = sees & (i - t < window)
+        if key_begin is not None:
+            sees = sees & (t >= key_begin[a:e, None])
+        sees = sees & real[None, :]
+        for h in range(H):
+            kb, zk, sk = f(up_k16[k_off[h]:k_off[h + 1]]), f(cache_k[rows, k_off[h]:k_off[h + 1]]), f(scale_k[rows, h])
+            zv, sv = f(cache_v[rows, v_off[h]:v_off[h + 1]]), f(scale_v[rows, h])
+            x = (f(q16[a:e, h]) @ (zk @ kb).t()) * sk * sm
+            dx = 2.0 ** -11 * ((f(q16[a:e, h]) @ kb.t()).abs() @ zk.abs().t()) * sk.abs() * sm
+            big = x.abs()
+            if softcap > 0:
+                x = softcap * torch.tanh(x / softcap)
+                big = big.clamp_min(softcap)
+            if slopes is not None:
+                bias = float(slopes[h]) * (i - t).abs().double()
+                x = x - bias
+                big = torch.maximum(big, bias)
+            none = torch.zeros((), dtype=torch.float64)
+            dx = torch.where(sees, dx + 2.0 ** -21 * big, none).amax(1, keepdim=True) if L else torch.zeros(n, 1, dtype=torch.float64)
+            x = x.masked_fill(~sees, float("-inf"))
+            if L:
+                x = x - x.amax(1, keepdim=True).clamp_min(-1e300)
+            p = torch.exp(x)
+            total = p.sum(1, keepdim=True)
+            p = torch.where(total > 0, p / total, none)
+            w = torch.where(p > 0, p * sv, none)
+            y = w @ zv
+            off = (w.abs() @ zv.abs()) * (2 * dx * torch.exp(2 * dx) + 2.0 ** -11 + 2.0 ** -20)
+            lat[a:e, v_off[h]:v_off[h + 1]] = y
+            lat_tol[a:e, v_off[h]:v_off[h + 1]] = half(y, off)
+            if up_v16 is not None:
+                bv = f(up_v16[v_off[h]:v_off[h + 1]])
+                o[a:e, h] = y @ bv
+                # the latent result may pass through fp16 on its way
+                o_tol[a:e, h] = half(y @ bv, (off + 2.0 ** -11 * (y.abs() + off) + 2.0 ** -25) @ bv.abs() * (1 + 2.0 ** -20))
+    return o, lat, o_tol, lat_tol
