@@ -42,32 +42,13 @@ struct __align__(16) ChunkShared {
   int32_t lo[kStreamRows], hi[kStreamRows];
 };
 
-template <int kN>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// 16 bytes global -> shared, or 16 zero bytes (nothing is read).
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-
-// Four consecutive halves, zero beyond `n` of them.
-__device__ __forceinline__ uint2 load_halves4(const __half* src, int n, bool vec) {
-  uint2 v = make_uint2(0u, 0u);
-  if (n >= 4 && vec) return __ldg(reinterpret_cast<const uint2*>(src));
-  __half* h = reinterpret_cast<__half*>(&v);
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (e < n) h[e] = src[e];
-  return v;
-}
-
 // q~ of up to 16 rows into shared memory, by all warps of the block: warp w takes the 8-rank tiles w, w + 4, ...
 // (mma lane (g, t): rows g and g + 8, k = halves 4t .. 4t + 3 of a 16-wide step, ranks 8 j + g).
-__device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int row0, int rows,
+__device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int rows,
                                             uint8_t* ring_mem) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const __half* qa = p.q + static_cast<int64_t>(r.start + row0 + min(g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
-  const __half* qb = p.q + static_cast<int64_t>(r.start + row0 + min(g + 8, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+  const __half* qa = p.q + static_cast<int64_t>(r.start + min(g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+  const __half* qb = p.q + static_cast<int64_t>(r.start + min(g + 8, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
   const int tiles = H.nk * 2;
   for (int j = warp; j < tiles; j += kChunkWarps) {
     const __half* up = p.up_k + static_cast<int64_t>(H.k_col + j * 8 + g) * p.up_k_row_stride;
@@ -89,23 +70,18 @@ __device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHea
   }
 }
 
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// grid: (heads, batch * row tiles of 16, splits)
+// grid: (heads, batch, splits)
 template <bool kCap, bool kBias>
-__global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __grid_constant__ ChunkParams p, int row_tiles) {
+__global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __grid_constant__ ChunkParams p) {
   extern __shared__ __align__(16) uint8_t ring_mem[];
   __shared__ ChunkShared s;
   grid_dependency_release();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-  const int h = blockIdx.x, b = blockIdx.y / row_tiles, row0 = (blockIdx.y % row_tiles) * kStreamRows, split = blockIdx.z;
-  const ChunkRequest r = chunk_request(p, b, h == 0 && row0 == 0 && split == 0 && threadIdx.x == 0);
-  const int rows = min(kStreamRows, r.n - row0);
-  if (rows <= 0) return;
+  const int h = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
+  const ChunkRequest r = chunk_request(p, b, h == 0 && split == 0 && threadIdx.x == 0);
+  const int rows = r.n;
+  if (rows <= 0 || rows > kStreamRows) return;      // none, or the tile form's
   const ChunkHead H = p.head[h];
   const int rk = H.nk * 16, rv = H.nv * 16;
 
@@ -114,7 +90,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     KeyRange k;
     k.lo = k.hi = 0;
     if (static_cast<int>(threadIdx.x) < rows)
-      k = visible_keys(p, r, p.b_prefix_len != nullptr ? p.b_prefix_len[b] : 0, row0 + threadIdx.x);
+      k = visible_keys(p, r, p.b_prefix_len != nullptr ? p.b_prefix_len[b] : 0, threadIdx.x);
     s.lo[threadIdx.x] = k.lo;
     s.hi[threadIdx.x] = k.hi;
   }
@@ -126,13 +102,14 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     inner_lo = max(inner_lo, s.lo[i]);
     inner_hi = min(inner_hi, s.hi[i]);
   }
-  kbeg = max(kbeg & ~31, split * p.split_len);
-  if (p.splits > 1) kend = static_cast<int>(min(static_cast<int64_t>(kend), (static_cast<int64_t>(split) + 1) * p.split_len));
+  kbeg = max(kbeg & ~31, split * p.stream_split_len);
+  if (p.stream_splits > 1) kend = static_cast<int>(min(static_cast<int64_t>(kend), (static_cast<int64_t>(split) + 1) * p.stream_split_len));
   const int ntiles = kend > kbeg ? (kend - kbeg + 31) / 32 : 0;
 
-  if (ntiles == 0 && p.partials) {      // the merge reads no sums where the weights' sum is zero
+  if (ntiles == 0 && p.stream_partials) {      // the merge reads no sums where the weights' sum is zero
     if (static_cast<int>(threadIdx.x) < rows)
-      p.part_ml[(static_cast<int64_t>(split) * p.num_tokens + r.start + row0 + threadIdx.x) * p.num_heads + h] = make_float2(-INFINITY, 0.f);
+      p.stream_ml[(static_cast<int64_t>(split) * p.batch * p.stream_stride + b * p.stream_stride + threadIdx.x) * p.num_heads + h] =
+          make_float2(-INFINITY, 0.f);
     return;
   }
 
@@ -169,14 +146,13 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     for (int x = lane; x < 32 * H.nk; x += 32) {
       const int tok = (x * inv_k) >> 16, piece = x - tok * H.nk;
       const int sl = __shfl_sync(0xffffffffu, slot, tok);
-      // K rows lie in the order of the score columns (below), V rows in the order of the keys
-      const int row = (tok & ~7) | ((tok & 3) << 1) | ((tok >> 2) & 1);
-      cp_async16_or_zero(kd + row * rk + piece * 16, kbase + static_cast<int64_t>(max(sl, 0)) * kstride + piece * 16, sl >= 0);
+      const int row = k_row_of(tok);
+      copy16_or_zero(kd + row * rk + k_piece_at(row, piece, H.nk) * 16, kbase + static_cast<int64_t>(max(sl, 0)) * kstride + piece * 16, sl >= 0);
     }
     for (int x = lane; x < 32 * H.nv; x += 32) {
       const int tok = (x * inv_v) >> 16, piece = x - tok * H.nv;
       const int sl = __shfl_sync(0xffffffffu, slot, tok);
-      cp_async16_or_zero(vd + tok * rv + piece * 16, vbase + static_cast<int64_t>(max(sl, 0)) * vstride + piece * 16, sl >= 0);
+      copy16_or_zero(vd + tok * rv + v_piece_at(tok, piece, H.nv) * 16, vbase + static_cast<int64_t>(max(sl, 0)) * vstride + piece * 16, sl >= 0);
     }
   };
   auto load_scales = [&](int i, float& a, float& c) {
@@ -195,12 +171,12 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     const int slot = slot_next;
     slot_next = fetch_slot(i + 1);
     if (i < mine) request(i, slot);
-    cp_async_commit();
+    copy_commit();
   }
   float sk_next, sv_next;
   load_scales(0, sk_next, sv_next);
 
-  absorb_rows(p, H, h, r, row0, rows, ring_mem);
+  absorb_rows(p, H, h, r, rows, ring_mem);
   __syncthreads();
   const float *qt_a = absorbed_row(ring_mem, g), *qt_b = absorbed_row(ring_mem, g + 8);
   // q~ as fp16 A fragments: step (mb, i) of a 64-rank block holds ranks 64 mb + 16 t + 4 i .. + 3 of lane (g, t)
@@ -252,7 +228,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     fb *= kChunkLog2e;
   }
   const int lo_a = s.lo[g], hi_a = s.hi[g], lo_b = s.lo[g + 8], hi_b = s.hi[g + 8];
-  const int pos_a = r.len - r.n + row0 + g, pos_b = pos_a + 8;
+  const int pos_a = r.len - r.n + g, pos_b = pos_a + 8;
   const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
 
   float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
@@ -269,7 +245,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       slot_next = fetch_slot(i + stages);
       __syncwarp();                   // every lane is done with the stage that is refilled now
       if (i + stages - 1 < mine) request(i + stages - 1, slot);
-      cp_async_commit();
+      copy_commit();
     }
     const float sk = sk_next, sv = sv_next;
     const int st = i & (stages - 1);
@@ -285,9 +261,9 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     }
     s.sk[warp][lane] = sk;
     s.sv[warp][lane] = sv * pow2i(kWeightShift - e_new);
-    if (stages == 8) cp_async_wait<7>();
-    else if (stages == 4) cp_async_wait<3>();
-    else cp_async_wait<1>();
+    if (stages == 8) copy_wait<7>();
+    else if (stages == 4) copy_wait<3>();
+    else copy_wait<1>();
     __syncwarp();
     const uint8_t* kd = ring + st * stage_bytes;
     const uint8_t* vd = kd + 32 * rk;
@@ -302,7 +278,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
         if (mb * 4 < H.nk) {
           uint4 w = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
           if (mb * 4 + t4 < H.nk) {
-            w = *reinterpret_cast<const uint4*>(kd + (8 * j + g) * rk + (mb * 4 + t4) * 16);
+            w = *reinterpret_cast<const uint4*>(kd + (8 * j + g) * rk + k_piece_at(8 * j + g, mb * 4 + t4, H.nk) * 16);
             w.x ^= 0x80808080u; w.y ^= 0x80808080u; w.z ^= 0x80808080u; w.w ^= 0x80808080u;
           }
           uint32_t b0, b1;
@@ -390,7 +366,8 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
         if (vb * 4 < H.nv) {
           uint2 ra = make_uint2(0x80808080u, 0x80808080u), rb = ra, rc = ra, rd = ra;
           if (64 * vb + 8 * g < rv) {
-            const uint8_t* at = vd + (16 * m + t4) * rv + 64 * vb + 8 * g;
+            // (keys four apart share their swizzle)
+            const uint8_t* at = vd + (16 * m + t4) * rv + v_piece_at(t4, 4 * vb + (g >> 1), H.nv) * 16 + 8 * (g & 1);
             ra = *reinterpret_cast<const uint2*>(at);
             rb = *reinterpret_cast<const uint2*>(at + 4 * rv);
             rc = *reinterpret_cast<const uint2*>(at + 8 * rv);
@@ -413,7 +390,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       }
     }
   }
-  cp_async_wait<0>();
+  copy_wait<0>();
 
   // join the four warps: common maximum per row, sums in shared memory (the rings are done with)
   l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
@@ -454,7 +431,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   const float* all = reinterpret_cast<const float*>(ring_mem);
   for (int x = threadIdx.x; x < rows * rv; x += kChunkThreads) {
     const int row = x / rv, rank = x - row * rv;
-    const int token = r.start + row0 + row;
+    const int token = r.start + row;
     float top = s.m[0][row], sum = 0.f, v = 0.f;
 #pragma unroll
     for (int w = 1; w < kChunkWarps; ++w) top = fmaxf(top, s.m[w][row]);
@@ -464,10 +441,10 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       sum += s.l[w][row] * ex2(s.m[w][row] - base);
       v += all[w * (kStreamRows * LSVD_MAX_RANK) + row * LSVD_MAX_RANK + rank];
     }
-    if (p.partials) {
-      const int64_t at = static_cast<int64_t>(split) * p.num_tokens + token;
-      p.part_o[at * p.sum_rv + H.v_col + rank] = v;
-      if (rank == 0) p.part_ml[at * p.num_heads + h] = make_float2(top, sum);
+    if (p.stream_partials) {
+      const int64_t at = (static_cast<int64_t>(split) * p.batch + b) * p.stream_stride + row;
+      p.stream_o[at * p.sum_rv + H.v_col + rank] = v;
+      if (rank == 0) p.stream_ml[at * p.num_heads + h] = make_float2(top, sum);
     } else {
       p.out_latent[token * p.out_latent_stride_t + H.v_col + rank] = __float2half_rn(sum == 0.f ? 0.f : v / sum);
     }
@@ -478,7 +455,8 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
 constexpr int kMergeRows = 8;
 __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
   __shared__ float lat[kMergeRows][LSVD_MAX_RANK];
-  __shared__ bool live[kMergeRows];
+  __shared__ int64_t first[kMergeRows], step[kMergeRows];      // row of the first split, rows between splits
+  __shared__ int splits[kMergeRows];                            // 0: not a row for the merge; < 0: of the tile form
   grid_dependency_release();
   grid_dependency_wait();
   const int h = blockIdx.x, token0 = blockIdx.y * kMergeRows;
@@ -492,24 +470,41 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
       if (p.b_start_loc[mid] <= token) lo = mid; else hi = mid - 1;
     }
     const ChunkRequest r = chunk_request(p, lo, false);
-    live[threadIdx.x] = token < p.num_tokens && token >= r.start && token < r.start + r.n;
+    int n = 0;
+    if (token < p.num_tokens && token >= r.start && token < r.start + r.n) {
+      if (r.n > p.tile_min) {
+        n = p.tile_splits > 1 ? -p.tile_splits : 0;
+        first[threadIdx.x] = token;
+        step[threadIdx.x] = p.num_tokens;
+      } else {
+        n = p.stream_partials ? p.stream_splits : 0;
+        first[threadIdx.x] = static_cast<int64_t>(lo) * p.stream_stride + token - r.start;
+        step[threadIdx.x] = static_cast<int64_t>(p.batch) * p.stream_stride;
+      }
+    }
+    splits[threadIdx.x] = n;
   }
   __syncthreads();
+  bool any = false;
+  for (int i = 0; i < kMergeRows; ++i) any = any || splits[i] != 0;
+  if (!any) return;
   for (int x = threadIdx.x; x < kMergeRows * rv; x += blockDim.x) {
     const int row = x / rv, rank = x - row * rv, token = token0 + row;
-    if (!live[row]) continue;
+    if (splits[row] == 0) continue;
+    const bool tile = splits[row] < 0;
+    const int n = abs(splits[row]);
+    const float2* ml = (tile ? p.tile_ml : p.stream_ml) + first[row] * p.num_heads + h;
+    const float* po = (tile ? p.tile_o : p.stream_o) + first[row] * p.sum_rv + H.v_col + rank;
     float top = -INFINITY;
-    for (int s = 0; s < p.splits; ++s)
-      top = fmaxf(top, p.part_ml[(static_cast<int64_t>(s) * p.num_tokens + token) * p.num_heads + h].x);
+    for (int s = 0; s < n; ++s) top = fmaxf(top, ml[s * step[row] * p.num_heads].x);
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f, v = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const int64_t at = static_cast<int64_t>(s) * p.num_tokens + token;
-      const float2 ml = p.part_ml[at * p.num_heads + h];
-      if (ml.y == 0.f) continue;                // nothing seen in this split
-      const float c = ex2(ml.x - base);
-      sum += ml.y * c;
-      v += p.part_o[at * p.sum_rv + H.v_col + rank] * c;
+    for (int s = 0; s < n; ++s) {
+      const float2 part = ml[s * step[row] * p.num_heads];
+      if (part.y == 0.f) continue;                // nothing seen in this split
+      const float c = ex2(part.x - base);
+      sum += part.y * c;
+      v += po[s * step[row] * p.sum_rv] * c;
     }
     v = sum == 0.f ? 0.f : v / sum;
     lat[row][rank] = v;
@@ -528,30 +523,62 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
     }
 #pragma unroll
     for (int i = 0; i < kMergeRows; ++i)
-      if (live[i]) p.out[(token0 + i) * p.out_stride_t + h * p.out_stride_h + d] = __float2half_rn(acc[i]);
+      if (splits[i] != 0) p.out[(token0 + i) * p.out_stride_t + h * p.out_stride_h + d] = __float2half_rn(acc[i]);
   }
 }
 
 struct ChunkPlan {
-  int row_tiles, splits, split_len;
+  bool stream, tile;                       // which forms are launched
+  int stream_splits, stream_split_len, stream_stride;
+  int tiles, tile_splits, tile_split_len, tile_min;
 };
 
-// The stream form's split of the keys: enough blocks for six rounds of the resident ones (three per SM), no piece shorter
-// than 256 keys.
+static void chunk_split(int64_t blocks, int64_t want, int least, int unit, int max_len, int* splits, int* len) {
+  const int64_t most = std::max(1, max_len / least);
+  const int64_t n = std::max<int64_t>(1, std::min(most, std::min<int64_t>(want / std::max<int64_t>(1, blocks), 128)));
+  const int64_t piece = std::max<int64_t>(unit, (max_len + n - 1) / n);
+  *len = static_cast<int>((piece + unit - 1) / unit * unit);
+  *splits = std::max(1, (max_len + *len - 1) / *len);
+}
+
+// Requests of up to 16 new tokens go to the stream form, longer ones to the tile form; a single request of a step that may
+// bring more than 16 always goes to the tile form (one launch).  The keys are split where the rows alone are too few
+// blocks: stream form, six rounds of the resident blocks (three per SM), pieces of 256 keys or more; tile form, two
+// rounds (two per SM), 512 keys or more.
 static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_new, int max_len) {
-  ChunkPlan c;
-  c.row_tiles = std::max(1, (std::min(max_new, num_tokens) + kStreamRows - 1) / kStreamRows);
-  const int64_t blocks = static_cast<int64_t>(num_heads) * std::min<int64_t>(static_cast<int64_t>(batch) * c.row_tiles, batch + num_tokens / kStreamRows);
-  const int64_t want = 6LL * 3 * std::max(1, device_sm_count());
-  const int64_t most = std::max(1, max_len / 256);
-  c.splits = static_cast<int>(std::max<int64_t>(1, std::min(most, std::min<int64_t>(want / std::max<int64_t>(1, blocks), 128))));
-  c.split_len = std::max(128, (max_len + c.splits - 1) / c.splits);
-  c.split_len = (c.split_len + 127) / 128 * 128;
-  c.splits = std::max(1, (max_len + c.split_len - 1) / c.split_len);
+  ChunkPlan c{};
+  const int64_t sms = std::max(1, device_sm_count());
+  const int longest = std::max(1, std::min(max_new, num_tokens));
+  c.tile = longest > kStreamRows;
+  c.stream = !c.tile || batch > 1;
+  c.tile_min = c.stream ? kStreamRows : 0;
+  c.stream_stride = std::min(kStreamRows, longest);
+  chunk_split(static_cast<int64_t>(num_heads) * batch, 6 * 3 * sms, 256, 128, max_len, &c.stream_splits, &c.stream_split_len);
+  const int64_t of_tokens = num_tokens / 128 + std::min<int64_t>(batch, num_tokens / (c.tile_min + 1));
+  const int64_t of_requests = static_cast<int64_t>(batch) * ((longest + 127) / 128);
+  c.tiles = static_cast<int>(std::max<int64_t>(1, std::min(of_tokens, of_requests)));
+  chunk_split(static_cast<int64_t>(num_heads) * c.tiles, 2 * 2 * sms, 512, 64, max_len, &c.tile_splits, &c.tile_split_len);
+  if (!c.stream) c.stream_splits = 0;
+  if (!c.tile) c.tile_splits = 0;
   return c;
 }
 
-static size_t chunk_align(size_t x) { return (x + 255) / 256 * 256; }
+struct ChunkWorkspace {
+  size_t stream_ml, stream_o, tile_ml, tile_o, total;
+};
+
+// The stream form always has room for partial results (its up-projection is the merge's), the tile form when it is split.
+static ChunkWorkspace chunk_workspace(const ChunkPlan& c, int batch, int num_heads, int sum_rv, int num_tokens) {
+  auto align = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t srows = static_cast<size_t>(c.stream_splits) * batch * c.stream_stride;
+  const size_t trows = c.tile_splits > 1 ? static_cast<size_t>(c.tile_splits) * num_tokens : 0;
+  ChunkWorkspace w{};
+  w.stream_o = align(srows * num_heads * sizeof(float2));
+  w.tile_ml = w.stream_o + align(srows * sum_rv * sizeof(float));
+  w.tile_o = w.tile_ml + align(trows * num_heads * sizeof(float2));
+  w.total = w.tile_o + align(trows * sum_rv * sizeof(float));
+  return w;
+}
 
 }  // namespace lsvd
 
@@ -559,9 +586,9 @@ extern "C" size_t lsvd_attn_chunk_workspace_bytes(int32_t batch, int32_t num_hea
                                                   int32_t max_new_in_batch, int32_t max_len_in_batch) {
   using namespace lsvd;
   if (batch <= 0 || num_heads <= 0 || sum_rank_v <= 0 || num_tokens < 0 || max_new_in_batch < 0 || max_len_in_batch < 0) return 0;
-  const ChunkPlan c = chunk_plan(batch, num_heads, num_tokens, max_new_in_batch, max_len_in_batch);
-  const size_t rows = static_cast<size_t>(c.splits) * std::max(1, num_tokens);
-  return chunk_align(rows * num_heads * sizeof(float2)) + chunk_align(rows * sum_rank_v * sizeof(float));
+  const ChunkWorkspace w = chunk_workspace(chunk_plan(batch, num_heads, num_tokens, max_new_in_batch, max_len_in_batch), batch, num_heads,
+                                           sum_rank_v, num_tokens);
+  return w.total;
 }
 
 extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
@@ -598,13 +625,14 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
     if (!aligned(x, 4)) return LSVD_ERR_INVALID_ARG;
   if (a->up_k_row_stride < a->head_dim || (a->out != nullptr && a->up_v_row_stride < a->head_dim)) return LSVD_ERR_INVALID_ARG;
   if (a->req_to_token_rows <= 0 || (a->req_to_token_rows > 1 && a->req_to_token_stride < a->max_len_in_batch)) return LSVD_ERR_INVALID_ARG;
+  if (a->max_len_in_batch > (1 << 30)) return LSVD_ERR_UNSUPPORTED;
   if (std::isnan(a->softcap) || std::isinf(a->softcap)) return LSVD_ERR_INVALID_ARG;
   const ChunkPlan c = chunk_plan(a->batch, a->num_heads, a->num_tokens, a->max_new_in_batch, a->max_len_in_batch);
-  const int64_t row_blocks = static_cast<int64_t>(a->batch) * c.row_tiles;
-  if (row_blocks > 65535 || (a->num_tokens + kMergeRows - 1) / kMergeRows > 65535) return LSVD_ERR_UNSUPPORTED;
-  const bool partials = c.splits > 1 || a->out != nullptr;
-  const size_t need = lsvd_attn_chunk_workspace_bytes(a->batch, a->num_heads, sum_rv, a->num_tokens, a->max_new_in_batch, a->max_len_in_batch);
-  if (partials && (a->workspace == nullptr || a->workspace_bytes < need || !aligned(a->workspace, 256))) return LSVD_ERR_WORKSPACE;
+  if (a->batch > 65535 || c.tiles > 65535 || (a->num_tokens + kMergeRows - 1) / kMergeRows > 65535) return LSVD_ERR_UNSUPPORTED;
+  const bool stream_partials = c.stream && (c.stream_splits > 1 || a->out != nullptr);
+  const bool merge = stream_partials || c.tile_splits > 1;
+  const ChunkWorkspace w = chunk_workspace(c, a->batch, a->num_heads, sum_rv, a->num_tokens);
+  if (merge && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned(a->workspace, 256))) return LSVD_ERR_WORKSPACE;
 
   p.q = static_cast<const __half*>(a->q);
   p.q_stride_t = a->q_stride_t;
@@ -651,22 +679,33 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   p.sum_rv = sum_rv;
   p.q_vec = aligned(a->q, 8) && (a->q_stride_t % 4) == 0 && (a->q_stride_h % 4) == 0;
   p.up_k_vec = aligned(a->up_k, 8) && (a->up_k_row_stride % 4) == 0;
-  p.splits = c.splits;
-  p.split_len = c.split_len;
-  p.partials = partials;
+  p.up_v_vec = aligned(a->up_v, 8) && (a->up_v_row_stride % 4) == 0;
+  p.out_vec2 = aligned(a->out, 4) && (a->out_stride_t % 2) == 0 && (a->out_stride_h % 2) == 0;
+  p.out_lat_vec16 = aligned(a->out_latent, 16) && (a->out_latent_stride_t % 8) == 0;
+  p.stream_splits = c.stream_splits;
+  p.stream_split_len = c.stream_split_len;
+  p.stream_stride = c.stream_stride;
+  p.tile_splits = c.tile_splits;
+  p.tile_split_len = c.tile_split_len;
+  p.tile_min = c.tile_min;
+  p.stream_partials = stream_partials;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  p.part_ml = reinterpret_cast<float2*>(ws);
-  p.part_o = reinterpret_cast<float*>(ws + chunk_align(static_cast<size_t>(c.splits) * a->num_tokens * a->num_heads * sizeof(float2)));
+  p.stream_ml = reinterpret_cast<float2*>(ws + w.stream_ml);
+  p.stream_o = reinterpret_cast<float*>(ws + w.stream_o);
+  p.tile_ml = reinterpret_cast<float2*>(ws + w.tile_ml);
+  p.tile_o = reinterpret_cast<float*>(ws + w.tile_o);
 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool cap = a->softcap > 0.f, bias = a->alibi_slopes != nullptr;
-  void (*kern)(ChunkParams, int) = cap ? (bias ? chunk_stream_kernel<true, true> : chunk_stream_kernel<true, false>)
-                                       : (bias ? chunk_stream_kernel<false, true> : chunk_stream_kernel<false, false>);
-  const int smem = kChunkWarps * kRingBytes;
-  LSVD_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem));
-  LSVD_CUDA_TRY(launch_chained(kern, dim3(a->num_heads, static_cast<unsigned>(row_blocks), c.splits), dim3(kChunkThreads), smem, st, 1, true,
-                               p, c.row_tiles));
-  if (partials)
+  if (c.stream) {
+    const bool cap = a->softcap > 0.f, bias = a->alibi_slopes != nullptr;
+    void (*kern)(ChunkParams) = cap ? (bias ? chunk_stream_kernel<true, true> : chunk_stream_kernel<true, false>)
+                                    : (bias ? chunk_stream_kernel<false, true> : chunk_stream_kernel<false, false>);
+    const int smem = kChunkWarps * kRingBytes;
+    LSVD_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem));
+    LSVD_CUDA_TRY(launch_chained(kern, dim3(a->num_heads, a->batch, c.stream_splits), dim3(kChunkThreads), smem, st, 1, true, p));
+  }
+  if (c.tile) LSVD_CUDA_TRY(launch_chunk_rows(p, c.tiles, st));
+  if (merge)
     LSVD_CUDA_TRY(launch_chained(chunk_merge_kernel, dim3(a->num_heads, (a->num_tokens + kMergeRows - 1) / kMergeRows), dim3(128), 0, st, 1,
                                  true, p));
   return LSVD_OK;

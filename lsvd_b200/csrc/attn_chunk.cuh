@@ -1,4 +1,4 @@
-// Shared by the kernels of the chunk attention (attn_chunk.cu, attn_chunk_tile.cu): parameters, the visible range of a
+// Shared by the kernels of the chunk attention (attn_chunk.cu, attn_chunk_rows.cu): parameters, the visible range of a
 // query token, the scores' cap and bias.
 #pragma once
 
@@ -34,8 +34,12 @@ struct ChunkParams {
   int64_t out_stride_t, out_stride_h;
   __half* out_latent;
   int64_t out_latent_stride_t;
-  float2* part_ml;           // [split][row][head]: running maximum (log2 domain) and sum
-  float* part_o;             // [split][row][sum r_v]: unnormalised sums
+  // partial results, for the merge: running maximum (log2 domain) and sum [split][row][head], unnormalised sums
+  // [split][row][sum r_v]; a row is request * stream_stride + i in the stream form, the token's row in the tile form
+  float2* stream_ml;
+  float* stream_o;
+  float2* tile_ml;
+  float* tile_o;
   int32_t* status_word;
   const float* alibi_slopes;
   const int32_t* b_prefix_len;
@@ -45,10 +49,16 @@ struct ChunkParams {
   int32_t batch, num_heads, head_dim, max_len, num_tokens, max_new, num_slots, r2t_rows;
   int32_t causal, window, head_major, sum_rv;
   int32_t q_vec, up_k_vec;   // rows of q / up_k can be read in 8-byte pieces
-  int32_t splits, split_len; // keys [s * split_len, (s + 1) * split_len) of the stream form's split s
-  int32_t partials;          // results go to part_ml / part_o, for the merge
+  int32_t up_v_vec, out_vec2, out_lat_vec16;     // rows of up_v in 8-byte, of out in 4-byte, of out_latent in 16-byte pieces
+  // split s takes the keys [s * split_len, (s + 1) * split_len)
+  int32_t stream_splits, stream_split_len, stream_stride;
+  int32_t tile_splits, tile_split_len;
+  int32_t stream_partials;   // the stream form leaves its results to the merge (the tile form: when it is split)
+  int32_t tile_min;          // the tile form takes requests of more rows than this
   ChunkHead head[LSVD_MAX_HEADS];
 };
+
+cudaError_t launch_chunk_rows(const ChunkParams& p, int tiles, cudaStream_t st);
 
 #ifdef __CUDACC__
 // A request, checked: its first row, its new tokens (0: skip it), its length and its row of the slot table.
@@ -122,6 +132,52 @@ __device__ __forceinline__ void codes_to_half(uint32_t u, uint32_t& lo, uint32_t
   const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&a), off), y = __hadd2(*reinterpret_cast<const __half2*>(&b), off);
   lo = *reinterpret_cast<const uint32_t*>(&x);
   hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four consecutive halves, zero beyond `n` of them.
+__device__ __forceinline__ uint2 load_halves4(const __half* src, int n, bool vec) {
+  uint2 v = make_uint2(0u, 0u);
+  if (n >= 4 && vec) return __ldg(reinterpret_cast<const uint2*>(src));
+  uint32_t h[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) h[e] = __half_as_ushort(src[e]);
+  v.x = h[0] | (h[1] << 16);
+  v.y = h[2] | (h[3] << 16);
+  return v;
+}
+
+__device__ __forceinline__ void store_halves8(__half* dst, uint4 v, bool vec) {
+  if (vec) {
+    *reinterpret_cast<uint4*>(dst) = v;
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dst[e] = __ushort_as_half(static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1))));
+}
+
+template <int kN>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// 16 bytes global -> shared, or 16 zero bytes (nothing is read).
+__device__ __forceinline__ void copy16_or_zero(void* dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
+// Where codes lie in shared memory (32 keys a group).  Column c = 2 t + e of the 8-key score tile j = 2 m + jj stands for key
+// 16 m + 8 jj + t + 4 e, so that lane (g, t)'s weights are those of keys t, t + 4, t + 8, t + 12 of a 16-key step and its V
+// operand comes from rows four apart.  K rows are stored in column order (lane (g, t) reads row 8 j + g), V rows in key order.
+// The 16-byte pieces of rows of 64 and 128 bytes are swizzled so that the rows read together lie in different banks.
+__device__ __forceinline__ int k_row_of(int key) { return (key & ~7) | ((key & 3) << 1) | ((key >> 2) & 1); }
+__device__ __forceinline__ int k_piece_at(int row, int piece, int nk) { return nk == 8 ? piece ^ ((row & 1) << 2) : piece; }
+__device__ __forceinline__ int v_piece_at(int key, int piece, int nv) {
+  return nv == 8 ? piece ^ ((key & 3) << 1) : (nv == 4 ? piece ^ (key & 2) : piece);
 }
 #endif
 
