@@ -544,7 +544,7 @@ static void chunk_split(int64_t blocks, int64_t want, int least, int unit, int m
 // Requests of up to 16 new tokens go to the stream form, longer ones to the tile form; a single request of a step that may
 // bring more than 16 always goes to the tile form (one launch).  The keys are split where the rows alone are too few
 // blocks: stream form, six rounds of the resident blocks (three per SM), pieces of 256 keys or more; tile form, two
-// rounds (two per SM), 512 keys or more.
+// rounds (one per SM), 512 keys or more.
 static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_new, int max_len) {
   ChunkPlan c{};
   const int64_t sms = std::max(1, device_sm_count());
@@ -554,10 +554,10 @@ static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_ne
   c.tile_min = c.stream ? kStreamRows : 0;
   c.stream_stride = std::min(kStreamRows, longest);
   chunk_split(static_cast<int64_t>(num_heads) * batch, 6 * 3 * sms, 256, 128, max_len, &c.stream_splits, &c.stream_split_len);
-  const int64_t of_tokens = num_tokens / 128 + std::min<int64_t>(batch, num_tokens / (c.tile_min + 1));
-  const int64_t of_requests = static_cast<int64_t>(batch) * ((longest + 127) / 128);
+  const int64_t of_tokens = num_tokens / kChunkTileRows + std::min<int64_t>(batch, num_tokens / (c.tile_min + 1));
+  const int64_t of_requests = static_cast<int64_t>(batch) * ((longest + kChunkTileRows - 1) / kChunkTileRows);
   c.tiles = static_cast<int>(std::max<int64_t>(1, std::min(of_tokens, of_requests)));
-  chunk_split(static_cast<int64_t>(num_heads) * c.tiles, 2 * 2 * sms, 512, 64, max_len, &c.tile_splits, &c.tile_split_len);
+  chunk_split(static_cast<int64_t>(num_heads) * c.tiles, 2 * sms, 512, 64, max_len, &c.tile_splits, &c.tile_split_len);
   if (!c.stream) c.stream_splits = 0;
   if (!c.tile) c.tile_splits = 0;
   return c;
@@ -704,7 +704,7 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
     LSVD_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem));
     LSVD_CUDA_TRY(launch_chained(kern, dim3(a->num_heads, a->batch, c.stream_splits), dim3(kChunkThreads), smem, st, 1, true, p));
   }
-  if (c.tile) LSVD_CUDA_TRY(launch_chunk_rows(p, c.tiles, st));
+  if (c.tile) LSVD_CUDA_TRY(launch_chunk_tile(p, c.tiles, st));
   if (merge)
     LSVD_CUDA_TRY(launch_chained(chunk_merge_kernel, dim3(a->num_heads, (a->num_tokens + kMergeRows - 1) / kMergeRows), dim3(128), 0, st, 1,
                                  true, p));

@@ -1,4 +1,4 @@
-// Shared by the kernels of the chunk attention (attn_chunk.cu, attn_chunk_rows.cu): parameters, the visible range of a
+// Shared by the kernels of the chunk attention (attn_chunk.cu, attn_chunk_tile.cu): parameters, the visible range of a
 // query token, the scores' cap and bias.
 #pragma once
 
@@ -8,6 +8,7 @@ namespace lsvd {
 
 constexpr float kChunkLog2e = 1.4426950408889634f;
 constexpr int kStreamRows = 16;      // query rows of a block of the stream form
+constexpr int kChunkTileRows = 256;  // and of the tile form
 
 struct ChunkHead {
   int32_t k_col, v_col;      // byte offsets of the head inside a K / V cache row
@@ -58,7 +59,7 @@ struct ChunkParams {
   ChunkHead head[LSVD_MAX_HEADS];
 };
 
-cudaError_t launch_chunk_rows(const ChunkParams& p, int tiles, cudaStream_t st);
+cudaError_t launch_chunk_tile(const ChunkParams& p, int tiles, cudaStream_t st);
 
 #ifdef __CUDACC__
 // A request, checked: its first row, its new tokens (0: skip it), its length and its row of the slot table.

@@ -1,0 +1,776 @@
+// Attention of new tokens over the paged int8 latent cache, tile form: 128 query rows of one request and head per block, on
+// tcgen05.  (The mathematics and the stream form, for requests of few rows, are in attn_chunk.cu.)
+//
+// Per 64 keys a block does two products with the weights' softmax between them:
+//   S[128 x 64] = q~[128 x r_k] . z_k^T     A and B from shared memory, accumulator in tensor memory (two buffers)
+//   O[128 x r_v] += P[128 x 64] . z_v       A = P, fp16, written over S in tensor memory; B = the codes, ranks contiguous
+// 16384 exponentials per 128 x 128 scores take 1024 cycles of an SM (16 a cycle) while the products take 512 at ranks of
+// 64 + 64: the exponentials bound it, then the issue slots of the softmax (about six per score).  So the softmax warps must never
+// wait.  Eight warps: four for the softmax (thread = row, no exchange between threads), three that gather the rows by slot,
+// widen the int8 codes to fp16 (exact) and store them in the 128-byte-swizzled layouts that the products read, one that issues
+// the products.  The score product of tile j + 2 runs while the softmax is at tile j + 1, and two blocks share an SM (256 tensor
+// memory columns and at most 113 KB of shared memory each), so that one's waits are the other's cycles.
+//
+// The prologue computes q~ = B_k q with the same unit; the epilogue applies the V up-factor likewise (o_lat rounded to fp16,
+// as in the latent result).  O is rescaled only when a row's maximum has grown by more than 2^8 since its last
+// reference, or when a larger V scale arrives: weights are held as p * scale_v * 2^(6 - E) with p < 2^8 and 2^E the power of
+// two below the largest V scale seen, so fp16 neither overflows (< 2^15) nor loses bits above 2^-20 of the reference.
+#include <algorithm>
+
+#include "attn_chunk.cuh"
+#include "devfn.cuh"
+#include "tc5.cuh"
+
+namespace lsvd {
+
+constexpr int kGroupRows = 128;                  // rows of one product: a softmax warpgroup's, thread = row
+constexpr int kGroups = 2;
+constexpr int kTileRows = kChunkTileRows;
+static_assert(kTileRows == kGroups * kGroupRows, "two products' rows");
+constexpr int kTileKeys = 64;
+constexpr int kSoftmaxWarps = 4 * kGroups, kLoadWarps = 3;
+constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
+constexpr int kTileThreads = (kMmaWarp + 1) * 32;
+constexpr int kLoadThreads = kLoadWarps * 32;
+constexpr int kTileSmem = 192 * 1024 + 1024;     // q~ (or o_lat), widened stages, copied codes; 1024 to align
+constexpr int kTileMaxStages = 4;
+constexpr int kCodeStages = 4;                   // stages of codes on their way
+constexpr int kTileSlotRing = 8;
+constexpr int kTileCols = 512;                   // tensor memory, 256 columns a group: S0 0..63, S1 64..127, O 128..255
+constexpr int kGroupCols = 256;
+constexpr int kColO = 128;
+constexpr float kLazy = 8.f;                     // growth of a row's maximum (log2) that rescales O
+constexpr int kTileShift = 6;
+
+struct __align__(16) TileShared {
+  float sk[kTileMaxStages][kTileKeys], sv[kTileMaxStages][kTileKeys];      // first: read in 16-byte pieces
+  uint64_t k_full[kTileMaxStages], k_empty[kTileMaxStages], v_full[kTileMaxStages], v_empty[kTileMaxStages];
+  uint64_t s_full[kGroups][2], p_full[kGroups][2], o_done[kGroups], q_full[kGroups], last;
+  uint32_t live[kTileMaxStages][2];              // keys with a slot, one bit each
+  int32_t E[kTileMaxStages];
+  int32_t slot[kTileSlotRing][kTileKeys];
+  uint32_t tmem;
+  volatile uint32_t abort;
+  int32_t b, tile;
+  int32_t kbeg, kend;
+  float scale[kTileRows];                        // power of two taken out of each q~ row
+};
+
+// ---- tcgen05 kind::f16 ------------------------------------------------------------------------------------------------
+// D = F32 (1 at bit 4), A = B = F16 (0), B's major-ness at bit 16 (1: N contiguous), N >> 3 at bit 17, M >> 4 at bit 24.
+__device__ __forceinline__ uint32_t idesc_f16(int n, bool b_n_major) {
+  return (1u << 4) | (b_n_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kGroupRows >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Descriptor of a tile whose rows are K indexes and whose N (or M) index is contiguous: rows of 128 bytes = 64 entries,
+// 128-byte swizzle, groups of 8 rows 1024 bytes apart (stride offset), 64-entry blocks `block_bytes` apart (leading offset).
+__device__ __forceinline__ uint64_t smem_desc_n_major_sw128(const void* tile, uint32_t block_bytes) {
+  const uint64_t addr = smem_u32(tile);
+  return ((addr & 0x3FFFFull) >> 4) | (static_cast<uint64_t>(block_bytes >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void named_barrier(int id, int count) { asm volatile("barrier.sync %0, %1;" ::"r"(id), "r"(count) : "memory"); }
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r)::"memory");
+  return r != 0u;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Wait for a phase, bounded by kMbarTimeoutNs; also gives up once another role has.  False: stop and leave.
+__device__ __forceinline__ bool tile_wait(TileShared& s, uint64_t* bar, uint32_t parity, int32_t* status_word) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t i = 0; i < kMbarMaxPolls; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (s.abort) return false;
+    if ((i & 63u) == 63u && global_timer_ns() - t0 > kMbarTimeoutNs) break;
+  }
+  s.abort = 1;
+  report_status(status_word, LSVD_ERR_TIMEOUT);
+  return false;
+}
+
+// 16-byte piece `chunk` (0..7) of row `row` in a swizzled [row][128 bytes] tile.
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+
+// 16 codes -> 16 fp16 values, two 16-byte pieces of a swizzled row.
+__device__ __forceinline__ void store_codes(uint8_t* tile, int row, int piece, uint4 w) {
+  uint4 a, b;
+  codes_to_half(w.x ^ 0x80808080u, a.x, a.y);
+  codes_to_half(w.y ^ 0x80808080u, a.z, a.w);
+  codes_to_half(w.z ^ 0x80808080u, b.x, b.y);
+  codes_to_half(w.w ^ 0x80808080u, b.z, b.w);
+  *reinterpret_cast<uint4*>(tile + swizzled(row, 2 * piece)) = a;
+  *reinterpret_cast<uint4*>(tile + swizzled(row, 2 * piece + 1)) = b;
+}
+
+// q~ = B_k q of the warp's 32 rows (mma m16n8k16, like the stream form's), as fp16 rows of the A operand relative to each
+// row's largest entry; the powers of two go to s.scale.  Ranks in blocks of 64: with two blocks the first is computed again
+// once the row's largest entry over both is known (its accumulators do not fit beside the second's).
+__device__ __forceinline__ void absorb_tile_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int row0, int rows,
+                                                 TileShared& s, uint8_t* q_tile) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int rk = H.nk * 16, first = warp * 32;      // rows of the block; q_tile is the group's
+  const __half* q[2][2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      q[m][e] = p.q + static_cast<int64_t>(r.start + row0 + min(first + 16 * m + 8 * e + g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+  float acc[2][8][4], top[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+  const int blocks = rk > 64 ? 2 : 1;
+#pragma unroll 1
+  for (int pass = 0; pass < (blocks == 2 ? 3 : 1); ++pass) {      // block 0, block 1, block 0 again
+    const int rank0 = pass == 1 ? 64 : 0;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
+#pragma unroll 1
+    for (int d0 = 0; d0 < p.head_dim; d0 += 16) {
+      const int d = d0 + 4 * t;
+      uint2 a[2][2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) a[m][e] = load_halves4(q[m][e] + d, p.head_dim - d, p.q_vec);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint2 b = make_uint2(0u, 0u);
+        const int rank = rank0 + 8 * j + g;
+        if (rank < rk) b = load_halves4(p.up_k + static_cast<int64_t>(H.k_col + rank) * p.up_k_row_stride + d, p.head_dim - d, p.up_k_vec);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) mma_f16_16x8x16(acc[m][j], a[m][0].x, a[m][1].x, a[m][0].y, a[m][1].y, b.x, b.y);
+      }
+    }
+    if (pass < 2) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top[m][e] = fmaxf(top[m][e], fmaxf(fabsf(acc[m][j][2 * e]), fabsf(acc[m][j][2 * e + 1])));
+          top[m][e] = fmaxf(top[m][e], __shfl_xor_sync(0xffffffffu, top[m][e], 1));
+          top[m][e] = fmaxf(top[m][e], __shfl_xor_sync(0xffffffffu, top[m][e], 2));
+        }
+    }
+    if (pass == 0 && blocks == 2) continue;
+    uint8_t* block = q_tile + (rank0 >> 6) * kGroupRows * 128;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int ex = exponent_of(top[m][e]) - 8, row = first + 16 * m + 8 * e + g;      // entries end up below 2^9
+        const float x = pow2i(-ex);
+        if (t == 0) s.scale[row] = pow2i(ex);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (rank0 + 8 * j < rk)
+            *reinterpret_cast<uint32_t*>(block + swizzled(row & (kGroupRows - 1), j) + 4 * t) = pack_half2(acc[m][j][2 * e] * x, acc[m][j][2 * e + 1] * x);
+      }
+  }
+}
+
+// o = B_v^T o_lat of the block's rows: the factor [r_v x head_dim] in the stages' place, o_lat (fp16, where q~ was) as A
+// (mma m16n8k16).  For the whole block, after its tensor memory is gone.
+__device__ __forceinline__ void chunk_tile_up(const ChunkParams& p, const TileShared& s, uint8_t* smem) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, h = blockIdx.x;
+  const ChunkHead H = p.head[h];
+  const int rv = H.nv * 16, q_bytes = ((max(H.nk, H.nv) + 3) >> 2) * kGroupRows * 128;
+  const ChunkRequest r = chunk_request(p, s.b, false);
+  const int row0 = s.tile * kTileRows, rows = min(kTileRows, r.n - row0);
+  __half* up = reinterpret_cast<__half*>(smem + kGroups * q_bytes);
+  for (int x = tid; x < rv * (p.head_dim >> 2); x += kTileThreads) {
+    const int rank = x / (p.head_dim >> 2), d = (x - rank * (p.head_dim >> 2)) * 4;
+    *reinterpret_cast<uint2*>(up + rank * p.head_dim + d) =
+        load_halves4(p.up_v + static_cast<int64_t>(H.v_col + rank) * p.up_v_row_stride + d, 4, p.up_v_vec);
+  }
+  __syncthreads();
+  if (warp >= kSoftmaxWarps || warp * 32 >= rows) return;
+#pragma unroll 1
+  for (int m = 0; m < 2; ++m) {
+    const int ra = warp * 32 + 16 * m + g, rb = ra + 8, la = ra & (kGroupRows - 1), lb = la + 8;
+    uint32_t a[8][4];
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < H.nv) {
+        const uint8_t* block = smem + (warp >> 2) * q_bytes + (q >> 2) * kGroupRows * 128;
+        const int c = 2 * (q & 3);
+        a[q][0] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c) + 4 * t);
+        a[q][1] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c) + 4 * t);
+        a[q][2] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c + 1) + 4 * t);
+        a[q][3] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c + 1) + 4 * t);
+      }
+    for (int d0 = 0; d0 < p.head_dim; d0 += 8) {
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < H.nv) {
+          const uint16_t* at = reinterpret_cast<const uint16_t*>(up) + (16 * q + 2 * t) * p.head_dim + d0 + g;
+          const uint32_t b0 = at[0] | (static_cast<uint32_t>(at[p.head_dim]) << 16);
+          const uint32_t b1 = at[8 * p.head_dim] | (static_cast<uint32_t>(at[9 * p.head_dim]) << 16);
+          mma_f16_16x8x16(y, a[q][0], a[q][1], a[q][2], a[q][3], b0, b1);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = e == 0 ? ra : rb;
+        if (row >= rows) continue;
+        __half* dst = p.out + static_cast<int64_t>(r.start + row0 + row) * p.out_stride_t + h * p.out_stride_h + d0 + 2 * t;
+        const uint32_t v = pack_half2(y[2 * e], y[2 * e + 1]);
+        if (p.out_vec2) {
+          *reinterpret_cast<uint32_t*>(dst) = v;
+        } else {
+          const __half2 hh = *reinterpret_cast<const __half2*>(&v);
+          dst[0] = __low2half(hh);
+          dst[1] = __high2half(hh);
+        }
+      }
+    }
+  }
+}
+
+// grid: (heads, row tiles of all requests (a bound), splits of the keys)
+template <bool kCap, bool kBias>
+__global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __grid_constant__ ChunkParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ TileShared s;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.x, split = blockIdx.z;
+  const ChunkHead H = p.head[h];
+  const int rk = H.nk * 16, rv = H.nv * 16;
+  const int kblocks = (H.nk + 3) >> 2, vblocks = (H.nv + 3) >> 2;            // 64-rank blocks
+  const int q_bytes = max(kblocks, vblocks) * kGroupRows * 128;              // of a group
+  const int k_bytes = kblocks * kTileKeys * 128, stage_bytes = k_bytes + vblocks * kTileKeys * 128;
+  const int code_bytes = kTileKeys * (rk + rv);
+  const int stages = kGroups * q_bytes + 4 * stage_bytes + kCodeStages * code_bytes <= kTileSmem - 1024 ? 4 : 2;
+  uint8_t* stage0 = smem + kGroups * q_bytes;
+  uint8_t* codes = stage0 + stages * stage_bytes;
+
+  grid_dependency_wait();
+  // which request and row tile: the tiles of the requests that this form takes, in batch order, a request's last tile first
+  // (it has the most keys to see)
+  if (warp == 0) {
+    int before = 0, found_b = -1, found_t = 0;
+    for (int b0 = 0; b0 < p.batch && found_b < 0; b0 += 32) {
+      int tiles = 0;
+      if (b0 + lane < p.batch) {
+        const ChunkRequest r = chunk_request(p, b0 + lane, h == 0 && blockIdx.y == 0 && split == 0);
+        if (r.n > p.tile_min) tiles = (r.n + kTileRows - 1) / kTileRows;
+      }
+      int inc = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      const int first = before + inc - tiles, mine = static_cast<int>(blockIdx.y) - first;
+      const uint32_t who = __ballot_sync(0xffffffffu, mine >= 0 && mine < tiles);
+      if (who != 0) {
+        const int src = __ffs(who) - 1;
+        found_b = b0 + src;
+        found_t = __shfl_sync(0xffffffffu, tiles - 1 - mine, src);
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) {
+      s.b = found_b;
+      s.tile = found_t;
+      s.kbeg = 0x7fffffff;
+      s.kend = 0;
+      s.abort = 0;
+      for (int i = 0; i < kTileMaxStages; ++i) {
+        mbar_init(&s.k_full[i], kLoadWarps);
+        mbar_init(&s.k_empty[i], 1);
+        mbar_init(&s.v_full[i], kLoadWarps);
+        mbar_init(&s.v_empty[i], 1);
+      }
+      for (int i = 0; i < kGroups; ++i) {
+        mbar_init(&s.s_full[i][0], 1);
+        mbar_init(&s.s_full[i][1], 1);
+        mbar_init(&s.o_done[i], 1);
+      }
+    }
+  }
+  __syncthreads();
+  if (s.b < 0) return;
+  const ChunkRequest r = chunk_request(p, s.b, false);
+  const int row0 = s.tile * kTileRows, rows = min(kTileRows, r.n - row0);
+  const int live_warps = (rows + 31) >> 5;                // softmax warps with rows, and groups with such warps
+  const int groups = (rows + kGroupRows - 1) / kGroupRows;
+  // the row of each softmax thread, and the block's keys
+  KeyRange keys;
+  keys.lo = keys.hi = 0;
+  if (tid < rows) keys = visible_keys(p, r, p.b_prefix_len != nullptr ? p.b_prefix_len[s.b] : 0, row0 + tid);
+  if (warp < kSoftmaxWarps) {
+    const int lo = __reduce_min_sync(0xffffffffu, keys.hi > keys.lo ? keys.lo : 0x7fffffff);
+    const int hi = __reduce_max_sync(0xffffffffu, keys.hi);
+    if (lane == 0 && hi > 0) {
+      atomicMin(&s.kbeg, lo);
+      atomicMax(&s.kend, hi);
+    }
+  }
+  if (tid == 0) {
+    for (int i = 0; i < groups; ++i) {
+      const int warps = min(4, live_warps - 4 * i);
+      mbar_init(&s.p_full[i][0], warps);
+      mbar_init(&s.p_full[i][1], warps);
+      mbar_init(&s.q_full[i], warps);
+    }
+    mbar_init(&s.last, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  if (warp == kMmaWarp) tmem_alloc(&s.tmem, kTileCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // Only now may the next kernel's blocks come in: one that takes tensor memory and then waits for this kernel must find
+  // every block of it already served.
+  grid_dependency_release();
+  const uint32_t tmem = s.tmem;
+  int kbeg = s.kbeg & ~(kTileKeys - 1), kend = s.kend;
+  if (p.tile_splits > 1) {
+    kbeg = static_cast<int>(max(static_cast<int64_t>(kbeg), static_cast<int64_t>(split) * p.tile_split_len));
+    kend = static_cast<int>(min(static_cast<int64_t>(kend), (static_cast<int64_t>(split) + 1) * p.tile_split_len));
+  }
+  const int ntiles = kend > kbeg ? (kend - kbeg + kTileKeys - 1) / kTileKeys : 0;
+
+  if (ntiles > 0 && warp == kMmaWarp) {
+    // ================= products: the whole warp keeps step, one elected lane issues =================
+    const uint32_t idesc_s = idesc_f16(kTileKeys, false), idesc_o = idesc_f16(rv, true);
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tile_wait(s, bar, parity, p.status_word)); };
+    // scores of tile j for both groups; a group's buffer still holds the weights of tile j - 2 until their product is done
+    auto scores = [&](int j) {
+      const int st = j & (stages - 1);
+      if (!wait(&s.k_full[st], (j / stages) & 1)) return false;
+#pragma unroll
+      for (int grp = 0; grp < kGroups; ++grp) {
+        if (grp >= groups) continue;
+        if (j >= 2 && !wait(&s.o_done[grp], j & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t qdesc = smem_desc_k_major_sw128(smem + grp * q_bytes), kdesc = smem_desc_k_major_sw128(stage0 + st * stage_bytes);
+          for (int q = 0; q < H.nk; ++q)        // 16 ranks a step: 32 bytes of a row; a 64-rank block is a tile of its own
+            umma_f16_ss(tmem + grp * kGroupCols + (j & 1) * kTileKeys, qdesc + ((q >> 2) * (kGroupRows * 128 >> 4) + (q & 3) * 2),
+                        kdesc + ((q >> 2) * (kTileKeys * 128 >> 4) + (q & 3) * 2), idesc_s, q > 0 ? 1u : 0u);
+          umma_commit(&s.s_full[grp][j & 1]);
+          if (grp + 1 == groups) umma_commit(&s.k_empty[st]);
+        }
+        __syncwarp();
+      }
+      return true;
+    };
+    bool go = true;
+    for (int grp = 0; grp < groups; ++grp) go = go && wait(&s.q_full[grp], 0);
+    go = go && scores(0);
+    if (ntiles > 1) go = go && scores(1);
+    for (int j = 0; go && j < ntiles; ++j) {
+      const int st = j & (stages - 1);
+      go = wait(&s.v_full[st], (j / stages) & 1);
+#pragma unroll
+      for (int grp = 0; grp < kGroups; ++grp) {
+        if (!go || grp >= groups) continue;
+        go = wait(&s.p_full[grp][j & 1], (j >> 1) & 1);
+        if (!go) continue;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vdesc = smem_desc_n_major_sw128(stage0 + st * stage_bytes + k_bytes, kTileKeys * 128);
+          const uint32_t base = tmem + grp * kGroupCols;
+#pragma unroll
+          for (int q = 0; q < kTileKeys / 16; ++q)    // 16 keys a step: two groups of eight rows; 8 columns of P
+            umma_f16_ts(base + kColO, base + (j & 1) * kTileKeys + 8 * q, vdesc + q * (2048 >> 4), idesc_o, (j | q) != 0 ? 1u : 0u);
+          umma_commit(&s.o_done[grp]);
+          if (grp + 1 == groups) umma_commit(&s.v_empty[st]);
+        }
+        __syncwarp();
+      }
+      if (go && j + 2 < ntiles) go = scores(j + 2);
+    }
+  } else if (ntiles > 0 && warp >= kSoftmaxWarps) {
+    // ================= gather and widen =================
+    const int lt = tid - kSoftmaxWarps * 32, lw = warp - kSoftmaxWarps;
+    const int32_t* r2t = p.req_to_token + static_cast<int64_t>(r.req) * p.req_to_token_stride;
+    const int8_t* kbase = p.cache_k + (p.head_major ? static_cast<int64_t>(H.k_col) * p.num_slots : H.k_col);
+    const int8_t* vbase = p.cache_v + (p.head_major ? static_cast<int64_t>(H.v_col) * p.num_slots : H.v_col);
+    const int64_t kstride = p.head_major ? rk : p.cache_k_row_stride, vstride = p.head_major ? rv : p.cache_v_row_stride;
+    const __half* sc = lw == 0 ? p.scale_v + (p.head_major ? static_cast<int64_t>(h) * p.num_slots : h)
+                               : p.scale_k + (p.head_major ? static_cast<int64_t>(h) * p.num_slots : h);
+    const int64_t sc_stride = p.head_major ? 1 : (lw == 0 ? p.scale_v_row_stride : p.scale_k_row_stride);
+    const uint32_t inv_k = 65536u / H.nk + 1, inv_v = 65536u / H.nv + 1;      // x / n for x < 576, n <= 8
+    auto fetch_slot = [&](int j) {
+      int slot = -1;
+      const int key = kbeg + j * kTileKeys + lt;
+      if (lt < kTileKeys && j < ntiles && key < kend) slot = r2t[key];
+      if (slot >= p.num_slots) {
+        report_status(p.status_word, LSVD_ERR_BOUNDS);
+        slot = -1;
+      }
+      return slot;
+    };
+    auto request = [&](int j) {
+      const int32_t* slots = s.slot[j & (kTileSlotRing - 1)];
+      uint8_t* kd = codes + (j & (kCodeStages - 1)) * code_bytes;
+      uint8_t* vd = kd + kTileKeys * rk;
+      for (int x = lt; x < kTileKeys * H.nk; x += kLoadThreads) {
+        const int row = (x * inv_k) >> 16, piece = x - row * H.nk, sl = slots[row];
+        copy16_or_zero(kd + x * 16, kbase + static_cast<int64_t>(max(sl, 0)) * kstride + piece * 16, sl >= 0);
+      }
+      for (int x = lt; x < kTileKeys * H.nv; x += kLoadThreads) {
+        const int row = (x * inv_v) >> 16, piece = x - row * H.nv, sl = slots[row];
+        copy16_or_zero(vd + x * 16, vbase + static_cast<int64_t>(max(sl, 0)) * vstride + piece * 16, sl >= 0);
+      }
+    };
+    float sc0 = 0.f, sc1 = 0.f;
+    int sl0 = -1, sl1 = -1, E = -200;
+    auto load_scales = [&](int j) {
+      if (lw > 1 || j >= ntiles) return;
+      sl0 = s.slot[j & (kTileSlotRing - 1)][lane];
+      sl1 = s.slot[j & (kTileSlotRing - 1)][lane + 32];
+      sc0 = sl0 >= 0 ? __half2float(sc[sl0 * sc_stride]) : 0.f;
+      sc1 = sl1 >= 0 ? __half2float(sc[sl1 * sc_stride]) : 0.f;
+    };
+    if (lt < kTileKeys)
+      for (int j = 0; j < kCodeStages; ++j) s.slot[j][lt] = fetch_slot(j);
+    int slot_ahead = fetch_slot(kCodeStages);
+    named_barrier(1, kLoadThreads);
+    for (int j = 0; j < kCodeStages - 1; ++j) {
+      if (j < ntiles) request(j);
+      copy_commit();
+    }
+    load_scales(0);
+    for (int j = 0; j < ntiles; ++j) {
+      const int st = j & (stages - 1);
+      copy_wait<kCodeStages - 2>();
+      // tile j's codes are here for every load warp, and all are done with the stage of tile j - 1
+      named_barrier(1, kLoadThreads);
+      if (lt < kTileKeys) s.slot[(j + kCodeStages) & (kTileSlotRing - 1)][lt] = slot_ahead;
+      slot_ahead = fetch_slot(j + kCodeStages + 1);
+      if (j + kCodeStages - 1 < ntiles) request(j + kCodeStages - 1);
+      copy_commit();
+      uint8_t* kd = stage0 + st * stage_bytes;
+      uint8_t* vd = kd + k_bytes;
+      const uint8_t* kc = codes + (j & (kCodeStages - 1)) * code_bytes;
+      const uint8_t* vc = kc + kTileKeys * rk;
+      // Every load warp attends every named barrier, whatever its waits returned, and all stop together.
+      bool ok = tile_wait(s, &s.k_empty[st], ((j / stages) & 1) ^ 1, p.status_word);
+      ok = ok && tile_wait(s, &s.v_empty[st], ((j / stages) & 1) ^ 1, p.status_word);
+      if (named_barrier_or(2, kLoadThreads, !ok)) break;
+      if (lw == 0) {
+        const float a0 = fabsf(sc0), a1 = fabsf(sc1);
+        int e = -200;
+        if (a0 > 0.f && a0 < INFINITY) e = exponent_of(a0);
+        if (a1 > 0.f && a1 < INFINITY) e = max(e, exponent_of(a1));
+        E = max(E, __reduce_max_sync(0xffffffffu, e));
+        const float x = pow2i(kTileShift - E);
+        s.sv[st][lane] = sc0 * x;
+        s.sv[st][lane + 32] = sc1 * x;
+        const uint32_t m0 = __ballot_sync(0xffffffffu, sl0 >= 0), m1 = __ballot_sync(0xffffffffu, sl1 >= 0);
+        if (lane == 0) {
+          s.E[st] = E;
+          s.live[st][0] = m0;
+          s.live[st][1] = m1;
+        }
+      } else if (lw == 1) {
+        s.sk[st][lane] = sc0;
+        s.sk[st][lane + 32] = sc1;
+      }
+      for (int x = lt; x < kTileKeys * H.nk; x += kLoadThreads) {
+        const int row = (x * inv_k) >> 16, piece = x - row * H.nk;
+        store_codes(kd + (piece >> 2) * kTileKeys * 128, row, piece & 3, *reinterpret_cast<const uint4*>(kc + x * 16));
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.k_full[st]);
+      load_scales(j + 1);
+      for (int x = lt; x < kTileKeys * H.nv; x += kLoadThreads) {
+        const int row = (x * inv_v) >> 16, piece = x - row * H.nv;
+        store_codes(vd + (piece >> 2) * kTileKeys * 128, row, piece & 3, *reinterpret_cast<const uint4*>(vc + x * 16));
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.v_full[st]);
+    }
+    copy_wait<0>();
+  } else if (warp < live_warps) {
+    // ================= softmax: thread = row =================
+    const int grp = warp >> 2;
+    uint8_t* q_tile = smem + grp * q_bytes;
+    const uint32_t lane_addr = tmem + grp * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int token = r.start + row0 + tid;
+    const int pos = r.len - r.n + row0 + tid;
+    float f = 0.f, m = -INFINITY, l = 0.f;
+    int E = -200;
+    bool go = true;
+    if (ntiles > 0) {
+      absorb_tile_rows(p, H, h, r, row0, rows, s, q_tile);
+      __syncwarp();
+      f = s.scale[tid];
+      f = fmaxf(f * p.score_scale * (kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e), 1e-37f);
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.q_full[grp]);
+    }
+    const float cap_log2e = p.softcap * kChunkLog2e;
+    const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
+    // keys that every row of the warp sees
+    const int inner_lo = __reduce_max_sync(0xffffffffu, tid < rows ? keys.lo : 0);
+    const int inner_hi = __reduce_min_sync(0xffffffffu, tid < rows ? keys.hi : 0x7fffffff);
+    const int outer_lo = __reduce_min_sync(0xffffffffu, keys.hi > keys.lo ? keys.lo : 0x7fffffff);
+    const int outer_hi = __reduce_max_sync(0xffffffffu, keys.hi);
+
+    for (int j = 0; go && j < ntiles; ++j) {
+      const int st = j & (stages - 1), k0 = kbeg + j * kTileKeys;
+      const uint32_t s_addr = lane_addr + (j & 1) * kTileKeys;
+      go = tile_wait(s, &s.k_full[st], (j / stages) & 1, p.status_word) && tile_wait(s, &s.v_full[st], (j / stages) & 1, p.status_word) &&
+           tile_wait(s, &s.s_full[grp][j & 1], (j >> 1) & 1, p.status_word);
+      if (!__all_sync(0xffffffffu, go)) {
+        go = false;
+        break;
+      }
+      tc_fence_after();
+      const int e_new = s.E[st];
+      const bool nothing = k0 >= outer_hi || k0 + kTileKeys <= outer_lo;      // of this warp's rows
+      const uint32_t live0 = s.live[st][0], live1 = s.live[st][1];
+      const bool masked = k0 < inner_lo || k0 + kTileKeys > inner_hi || (live0 & live1) != 0xffffffffu;
+      float2 x[kTileKeys / 2];
+      float top = -INFINITY;
+      if (!nothing) {
+        // (half by half: the scales of the second half are not fetched before the first half's scores are in)
+        const float4* sk = reinterpret_cast<const float4*>(s.sk[st]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t raw[32];
+          __syncwarp();
+          tmem_ld32(s_addr + 32 * half, raw);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 c = sk[8 * half + i];
+            x[16 * half + 2 * i] = mul2(make_float2(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), make_float2(c.x, c.y));
+            x[16 * half + 2 * i + 1] = mul2(make_float2(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), make_float2(c.z, c.w));
+          }
+        }
+        if (kCap || kBias) {
+          const float away = static_cast<float>(pos - k0);
+#pragma unroll
+          for (int i = 0; i < kTileKeys / 2; ++i) {
+            float a = x[i].x * f, b = x[i].y * f;
+            if (kCap) {
+              a = capped_log2(a, cap_log2e);
+              b = capped_log2(b, cap_log2e);
+            }
+            if (kBias) {
+              a = fmaf(-slope, fabsf(away - static_cast<float>(2 * i)), a);
+              b = fmaf(-slope, fabsf(away - static_cast<float>(2 * i + 1)), b);
+            }
+            x[i] = make_float2(a, b);
+          }
+        }
+        if (masked) {
+          const int a = min(max(keys.lo - k0, 0), 64), b = min(max(keys.hi - k0, 0), 64);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {            // bits of the keys that the row sees, 32 at a time
+            const int from = min(max(a - 32 * w, 0), 32), upto = min(max(b - 32 * w, 0), 32);
+            const uint32_t mask = (w == 0 ? live0 : live1) & (upto >= 32 ? ~0u : (1u << upto) - 1u) & (from >= 32 ? 0u : ~0u << from);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (!((mask >> (2 * i)) & 1u)) x[16 * w + i].x = -INFINITY;
+              if (!((mask >> (2 * i + 1)) & 1u)) x[16 * w + i].y = -INFINITY;
+            }
+          }
+        }
+        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kTileKeys / 2; i += 2) {
+          t0 = max3(t0, x[i].x, x[i].y);
+          t1 = max3(t1, x[i + 1].x, x[i + 1].y);
+        }
+        top = fmaxf(t0, t1);
+        if (!kCap && !kBias) top *= f;
+      }
+      // a new reference: the first maximum of a row, one that has grown by more than 2^8, or a larger V scale
+      const bool first = m == -INFINITY;
+      const bool grown = first ? top > -INFINITY : top > m + kLazy;
+      if (__any_sync(0xffffffffu, grown) || e_new != E) {
+        const float m_new = grown ? top : m;
+        const float c = first ? 0.f : ex2(m - m_new);
+        l *= c;
+        if (j > 0 && __any_sync(0xffffffffu, (grown && !first) || e_new != E)) {
+          go = tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
+          if (!__all_sync(0xffffffffu, go)) {
+            go = false;
+            break;
+          }
+          tc_fence_after();
+          const float by = (first ? 1.f : c) * pow2i(max(E - e_new, -126));
+          __syncwarp();
+#pragma unroll 1
+          for (int col = 0; col < rv; col += 16) {
+            uint32_t v[16];
+            tmem_ld16(lane_addr + kColO + col, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
+            tmem_st16(lane_addr + kColO + col, v);
+          }
+        }
+        m = m_new;
+        E = e_new;
+      }
+      __syncwarp();
+      if (nothing) {
+        uint32_t z[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i] = 0u;
+        tmem_st16(s_addr, z);
+        tmem_st16(s_addr + 16, z);
+      } else {
+        const float base = m == -INFINITY ? 0.f : m;
+        const float2 nb = make_float2(-base, -base), ff = make_float2(f, f);
+        float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+        const float4* sv = reinterpret_cast<const float4*>(s.sv[st]);
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {         // (16-column stores cost spills)
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 8 * part + 2 * i;
+            const float2 y0 = (kCap || kBias) ? add2(x[at], nb) : fma2(x[at], ff, nb);
+            const float2 y1 = (kCap || kBias) ? add2(x[at + 1], nb) : fma2(x[at + 1], ff, nb);
+            const float2 p0 = make_float2(ex2(y0.x), ex2(y0.y)), p1 = make_float2(ex2(y1.x), ex2(y1.y));
+            sum0 = add2(sum0, p0);
+            sum1 = add2(sum1, p1);
+            const float4 c = sv[4 * part + i];
+            float2 w0 = mul2(p0, make_float2(c.x, c.y)), w1 = mul2(p1, make_float2(c.z, c.w));
+            if (masked) {             // a masked key's weight is zero whatever its scale holds
+              if (p0.x == 0.f) w0.x = 0.f;
+              if (p0.y == 0.f) w0.y = 0.f;
+              if (p1.x == 0.f) w1.x = 0.f;
+              if (p1.y == 0.f) w1.y = 0.f;
+            }
+            const __half2 h0 = __floats2half2_rn(w0.x, w0.y), h1 = __floats2half2_rn(w1.x, w1.y);
+            w[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
+            w[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+          }
+          __syncwarp();
+          tmem_st8(s_addr + 8 * part, w);
+        }
+        sum0 = add2(sum0, sum1);
+        l += sum0.x + sum0.y;
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.p_full[grp][j & 1]);
+    }
+
+    // ---- results -------------------------------------------------------------------------------------------------------
+    // (all that is known here is that the product of tile ntiles - 3 is done: a phase is waited for by its parity, one by one)
+    if (go && ntiles > 1) go = tile_wait(s, &s.o_done[grp], ntiles & 1, p.status_word);
+    if (go && ntiles > 0) go = tile_wait(s, &s.o_done[grp], (ntiles - 1) & 1, p.status_word);
+    go = __all_sync(0xffffffffu, go);
+    tc_fence_after();
+    if (go) {
+      const float back = ntiles > 0 ? (E > -200 ? pow2i(E - kTileShift) : 1.f) : 0.f;
+      const float by = p.tile_splits > 1 ? back : (l == 0.f ? 0.f : back / l);
+      const bool to_up = p.out != nullptr && p.tile_splits == 1;
+      const int64_t part = static_cast<int64_t>(split) * p.num_tokens + token;
+      if (p.tile_splits > 1 && tid < rows) p.tile_ml[part * p.num_heads + h] = make_float2(m, l);
+#pragma unroll 1
+      for (int c = 0; c < rv; c += 16) {
+        uint32_t v[16];
+        float y[16];
+        __syncwarp();
+        if (ntiles > 0) tmem_ld16(lane_addr + kColO + c, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = (ntiles > 0 && by != 0.f) ? __uint_as_float(v[i]) * by : 0.f;
+        if (p.tile_splits > 1) {
+          if (tid < rows && ntiles > 0) {
+            float4* dst = reinterpret_cast<float4*>(p.tile_o + part * p.sum_rv + H.v_col + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          }
+          continue;
+        }
+        __align__(16) __half2 hh[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hh[i] = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
+        const uint4 lo = *reinterpret_cast<const uint4*>(&hh[0]), hi = *reinterpret_cast<const uint4*>(&hh[4]);
+        if (p.out_latent != nullptr && tid < rows) {
+          __half* dst = p.out_latent + token * p.out_latent_stride_t + H.v_col + c;
+          store_halves8(dst, lo, p.out_lat_vec16);
+          store_halves8(dst + 8, hi, p.out_lat_vec16);
+        }
+        if (to_up && ntiles > 0) {
+          uint8_t* block = q_tile + (c >> 6) * kGroupRows * 128;
+          const int piece = (c & 63) >> 3, row = tid & (kGroupRows - 1);
+          *reinterpret_cast<uint4*>(block + swizzled(row, piece)) = lo;
+          *reinterpret_cast<uint4*>(block + swizzled(row, piece + 1)) = hi;
+        }
+      }
+      if (to_up && ntiles == 0 && tid < rows)
+        for (int d = 0; d < p.head_dim; ++d) p.out[token * p.out_stride_t + h * p.out_stride_h + d] = __float2half_rn(0.f);
+    } else {
+      s.abort = 1;
+    }
+  }
+
+  // Every role is through with its stages here (one that gave up has set the abort flag).  Block barriers and
+  // tensor memory instructions take whole warps.
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) {
+    if (s.abort) {
+      // products may be in flight: an arrival behind all of them, waited for (bounded), before their memory goes
+      if (elect_one()) umma_commit(&s.last);
+      __syncwarp();
+      mbar_wait_bounded(&s.last, 0);
+      __syncwarp();
+    }
+    tmem_dealloc(tmem, kTileCols);
+  }
+  // (what follows is worked out anew: held over the loops above, it would not fit the registers)
+  if (s.kend <= s.kbeg || p.out == nullptr || p.tile_splits > 1 || s.abort) return;
+  chunk_tile_up(p, s, smem);
+}
+
+cudaError_t launch_chunk_tile(const ChunkParams& p, int tiles, cudaStream_t st) {
+  const bool cap = p.softcap > 0.f, bias = p.alibi_slopes != nullptr;
+  void (*kern)(ChunkParams) = cap ? (bias ? chunk_tile_kernel<true, true> : chunk_tile_kernel<true, false>)
+                                  : (bias ? chunk_tile_kernel<false, true> : chunk_tile_kernel<false, false>);
+  const cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), kTileSmem);
+  if (e != cudaSuccess) return e;
+  return launch_chained(kern, dim3(p.num_heads, tiles, p.tile_splits), dim3(kTileThreads), kTileSmem, st, 1, true, p);
+}
+
+}  // namespace lsvd
