@@ -155,14 +155,12 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       copy16_or_zero(vd + tok * rv + v_piece_at(tok, piece, H.nv) * 16, vbase + static_cast<int64_t>(max(sl, 0)) * vstride + piece * 16, sl >= 0);
     }
   };
-  auto load_scales = [&](int i, float& a, float& c) {
-    a = c = 0.f;
+  // (kept as loaded until the tile is in hand: a conversion here would wait for the load)
+  auto load_scales = [&](int i, __half& a, __half& c) {
     if (i >= mine) return;
-    const int sl = s.slot[warp][i & (stages - 1)][lane];
-    if (sl >= 0) {
-      a = __half2float(ksc[sl * kss]);
-      c = __half2float(vsc[sl * vss]);
-    }
+    const int sl = max(s.slot[warp][i & (stages - 1)][lane], 0);
+    a = ksc[sl * kss];
+    c = vsc[sl * vss];
   };
 
   // the first stages are on their way while the query rows are absorbed
@@ -173,7 +171,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     if (i < mine) request(i, slot);
     copy_commit();
   }
-  float sk_next, sv_next;
+  __half sk_next = __ushort_as_half(0), sv_next = sk_next;
   load_scales(0, sk_next, sv_next);
 
   absorb_rows(p, H, h, r, rows, ring_mem);
@@ -247,9 +245,9 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       if (i + stages - 1 < mine) request(i + stages - 1, slot);
       copy_commit();
     }
-    const float sk = sk_next, sv = sv_next;
     const int st = i & (stages - 1);
     const int my_slot = s.slot[warp][st][lane];
+    const float sk = my_slot >= 0 ? __half2float(sk_next) : 0.f, sv = my_slot >= 0 ? __half2float(sv_next) : 0.f;
     const uint32_t valid = __ballot_sync(0xffffffffu, my_slot >= 0);
     load_scales(i + 1, sk_next, sv_next);
     // V scales relative to the largest one: a larger one than before moves the accumulators' exponent

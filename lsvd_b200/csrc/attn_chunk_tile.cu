@@ -426,41 +426,71 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     const __half* sc = lw == 0 ? p.scale_v + (p.head_major ? static_cast<int64_t>(h) * p.num_slots : h)
                                : p.scale_k + (p.head_major ? static_cast<int64_t>(h) * p.num_slots : h);
     const int64_t sc_stride = p.head_major ? 1 : (lw == 0 ? p.scale_v_row_stride : p.scale_k_row_stride);
-    const uint32_t inv_k = 65536u / H.nk + 1, inv_v = 65536u / H.nv + 1;      // x / n for x < 576, n <= 8
+    // A thread's pieces of a tile: 16-byte piece kp of rows k_first, k_first + k_step, ... (threads beyond the last whole row: none)
+    const int k_step = kLoadThreads / H.nk, v_step = kLoadThreads / H.nv;
+    const int k_first = lt / H.nk < k_step ? lt / H.nk : kTileKeys, v_first = lt / H.nv < v_step ? lt / H.nv : kTileKeys;
+    const int kp = lt % H.nk, vp = lt % H.nv;
+    const int8_t* ksrc = kbase + kp * 16;
+    const int8_t* vsrc = vbase + vp * 16;
+    // What is loaded ahead is looked at one tile later, not where it is requested: a comparison or a conversion right behind
+    // the load waits for it (1100 of 3700 cycles per tile).
     auto fetch_slot = [&](int j) {
-      int slot = -1;
       const int key = kbeg + j * kTileKeys + lt;
-      if (lt < kTileKeys && j < ntiles && key < kend) slot = r2t[key];
+      return lt < kTileKeys && j < ntiles && key < kend ? r2t[key] : -1;
+    };
+    auto keep_slot = [&](int j, int slot) {
       if (slot >= p.num_slots) {
         report_status(p.status_word, LSVD_ERR_BOUNDS);
         slot = -1;
       }
-      return slot;
+      if (lt < kTileKeys) s.slot[j & (kTileSlotRing - 1)][lt] = slot;
+    };
+    // three rows at a time: their slots, then their copies
+    auto request_rows = [&](const int32_t* slots, uint8_t* dst, const int8_t* src, int64_t stride, int first, int step, int row_bytes) {
+      for (int r0 = first; r0 < kTileKeys; r0 += 3 * step) {
+        int sl[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) sl[i] = r0 + i * step < kTileKeys ? slots[r0 + i * step] : -1;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (r0 + i * step < kTileKeys)
+            copy16_or_zero(dst + (r0 + i * step) * row_bytes, src + static_cast<int64_t>(max(sl[i], 0)) * stride, sl[i] >= 0);
+      }
     };
     auto request = [&](int j) {
       const int32_t* slots = s.slot[j & (kTileSlotRing - 1)];
       uint8_t* kd = codes + (j & (kCodeStages - 1)) * code_bytes;
-      uint8_t* vd = kd + kTileKeys * rk;
-      for (int x = lt; x < kTileKeys * H.nk; x += kLoadThreads) {
-        const int row = (x * inv_k) >> 16, piece = x - row * H.nk, sl = slots[row];
-        copy16_or_zero(kd + x * 16, kbase + static_cast<int64_t>(max(sl, 0)) * kstride + piece * 16, sl >= 0);
-      }
-      for (int x = lt; x < kTileKeys * H.nv; x += kLoadThreads) {
-        const int row = (x * inv_v) >> 16, piece = x - row * H.nv, sl = slots[row];
-        copy16_or_zero(vd + x * 16, vbase + static_cast<int64_t>(max(sl, 0)) * vstride + piece * 16, sl >= 0);
+      request_rows(slots, kd + kp * 16, ksrc, kstride, k_first, k_step, rk);
+      request_rows(slots, kd + kTileKeys * rk + vp * 16, vsrc, vstride, v_first, v_step, rv);
+    };
+    // and widened: three rows of codes in registers, then stored as fp16
+    auto widen_rows = [&](uint8_t* tile, const uint8_t* src, int piece, int first, int step, int row_bytes) {
+      for (int r0 = first; r0 < kTileKeys; r0 += 3 * step) {
+        uint4 w[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (r0 + i * step < kTileKeys) w[i] = *reinterpret_cast<const uint4*>(src + (r0 + i * step) * row_bytes);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (r0 + i * step < kTileKeys) store_codes(tile, r0 + i * step, piece, w[i]);
       }
     };
-    float sc0 = 0.f, sc1 = 0.f;
+    __half raw0 = __ushort_as_half(0), raw1 = raw0;
     int sl0 = -1, sl1 = -1, E = -200;
     auto load_scales = [&](int j) {
       if (lw > 1 || j >= ntiles) return;
       sl0 = s.slot[j & (kTileSlotRing - 1)][lane];
       sl1 = s.slot[j & (kTileSlotRing - 1)][lane + 32];
-      sc0 = sl0 >= 0 ? __half2float(sc[sl0 * sc_stride]) : 0.f;
-      sc1 = sl1 >= 0 ? __half2float(sc[sl1 * sc_stride]) : 0.f;
+      raw0 = sc[max(sl0, 0) * sc_stride];
+      raw1 = sc[max(sl1, 0) * sc_stride];
     };
-    if (lt < kTileKeys)
-      for (int j = 0; j < kCodeStages; ++j) s.slot[j][lt] = fetch_slot(j);
+    {
+      int first[kCodeStages];
+#pragma unroll
+      for (int j = 0; j < kCodeStages; ++j) first[j] = fetch_slot(j);
+#pragma unroll
+      for (int j = 0; j < kCodeStages; ++j) keep_slot(j, first[j]);
+    }
     int slot_ahead = fetch_slot(kCodeStages);
     named_barrier(1, kLoadThreads);
     for (int j = 0; j < kCodeStages - 1; ++j) {
@@ -468,23 +498,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       copy_commit();
     }
     load_scales(0);
+    bool ok = true;
     for (int j = 0; j < ntiles; ++j) {
       const int st = j & (stages - 1);
       copy_wait<kCodeStages - 2>();
-      // tile j's codes are here for every load warp, and all are done with the stage of tile j - 1
-      named_barrier(1, kLoadThreads);
-      if (lt < kTileKeys) s.slot[(j + kCodeStages) & (kTileSlotRing - 1)][lt] = slot_ahead;
+      // tile j's codes are here for every load warp, and all are done with the stage of tile j - 1.  Every load warp comes
+      // here, whatever its waits returned, and all stop together.
+      if (named_barrier_or(1, kLoadThreads, !ok)) break;
+      keep_slot(j + kCodeStages, slot_ahead);
       slot_ahead = fetch_slot(j + kCodeStages + 1);
       if (j + kCodeStages - 1 < ntiles) request(j + kCodeStages - 1);
       copy_commit();
       uint8_t* kd = stage0 + st * stage_bytes;
-      uint8_t* vd = kd + k_bytes;
       const uint8_t* kc = codes + (j & (kCodeStages - 1)) * code_bytes;
-      const uint8_t* vc = kc + kTileKeys * rk;
-      // Every load warp attends every named barrier, whatever its waits returned, and all stop together.
-      bool ok = tile_wait(s, &s.k_empty[st], ((j / stages) & 1) ^ 1, p.status_word);
+      ok = tile_wait(s, &s.k_empty[st], ((j / stages) & 1) ^ 1, p.status_word);
       ok = ok && tile_wait(s, &s.v_empty[st], ((j / stages) & 1) ^ 1, p.status_word);
-      if (named_barrier_or(2, kLoadThreads, !ok)) break;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) continue;
+      // the scales go first: the softmax reads them once K is there
+      const float sc0 = sl0 >= 0 ? __half2float(raw0) : 0.f, sc1 = sl1 >= 0 ? __half2float(raw1) : 0.f;
       if (lw == 0) {
         const float a0 = fabsf(sc0), a1 = fabsf(sc1);
         int e = -200;
@@ -504,18 +536,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
         s.sk[st][lane] = sc0;
         s.sk[st][lane + 32] = sc1;
       }
-      for (int x = lt; x < kTileKeys * H.nk; x += kLoadThreads) {
-        const int row = (x * inv_k) >> 16, piece = x - row * H.nk;
-        store_codes(kd + (piece >> 2) * kTileKeys * 128, row, piece & 3, *reinterpret_cast<const uint4*>(kc + x * 16));
-      }
+      load_scales(j + 1);
+      widen_rows(kd + (kp >> 2) * kTileKeys * 128, kc + kp * 16, kp & 3, k_first, k_step, rk);
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.k_full[st]);
-      load_scales(j + 1);
-      for (int x = lt; x < kTileKeys * H.nv; x += kLoadThreads) {
-        const int row = (x * inv_v) >> 16, piece = x - row * H.nv;
-        store_codes(vd + (piece >> 2) * kTileKeys * 128, row, piece & 3, *reinterpret_cast<const uint4*>(vc + x * 16));
-      }
+      widen_rows(kd + k_bytes + (vp >> 2) * kTileKeys * 128, kc + kTileKeys * rk + vp * 16, vp & 3, v_first, v_step, rv);
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.v_full[st]);
@@ -551,8 +577,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     for (int j = 0; go && j < ntiles; ++j) {
       const int st = j & (stages - 1), k0 = kbeg + j * kTileKeys;
       const uint32_t s_addr = lane_addr + (j & 1) * kTileKeys;
-      go = tile_wait(s, &s.k_full[st], (j / stages) & 1, p.status_word) && tile_wait(s, &s.v_full[st], (j / stages) & 1, p.status_word) &&
-           tile_wait(s, &s.s_full[grp][j & 1], (j >> 1) & 1, p.status_word);
+      go = tile_wait(s, &s.k_full[st], (j / stages) & 1, p.status_word) && tile_wait(s, &s.s_full[grp][j & 1], (j >> 1) & 1, p.status_word);
       if (!__all_sync(0xffffffffu, go)) {
         go = false;
         break;
@@ -653,21 +678,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
         tmem_st16(s_addr, z);
         tmem_st16(s_addr + 16, z);
       } else {
+        // exponentials in place (the unit that bounds the kernel works without a pause), then the weights
         const float base = m == -INFINITY ? 0.f : m;
         const float2 nb = make_float2(-base, -base), ff = make_float2(f, f);
-        float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+        float2 sum[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kTileKeys / 2; ++i) {
+          const float2 y = (kCap || kBias) ? add2(x[i], nb) : fma2(x[i], ff, nb);
+          x[i] = make_float2(ex2(y.x), ex2(y.y));
+          sum[i & 3] = add2(sum[i & 3], x[i]);
+        }
         const float4* sv = reinterpret_cast<const float4*>(s.sv[st]);
 #pragma unroll
         for (int part = 0; part < 4; ++part) {         // (16-column stores cost spills)
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int at = 8 * part + 2 * i;
-            const float2 y0 = (kCap || kBias) ? add2(x[at], nb) : fma2(x[at], ff, nb);
-            const float2 y1 = (kCap || kBias) ? add2(x[at + 1], nb) : fma2(x[at + 1], ff, nb);
-            const float2 p0 = make_float2(ex2(y0.x), ex2(y0.y)), p1 = make_float2(ex2(y1.x), ex2(y1.y));
-            sum0 = add2(sum0, p0);
-            sum1 = add2(sum1, p1);
+            const float2 p0 = x[8 * part + 2 * i], p1 = x[8 * part + 2 * i + 1];
             const float4 c = sv[4 * part + i];
             float2 w0 = mul2(p0, make_float2(c.x, c.y)), w1 = mul2(p1, make_float2(c.z, c.w));
             if (masked) {             // a masked key's weight is zero whatever its scale holds
@@ -676,15 +705,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
               if (p1.x == 0.f) w1.x = 0.f;
               if (p1.y == 0.f) w1.y = 0.f;
             }
-            const __half2 h0 = __floats2half2_rn(w0.x, w0.y), h1 = __floats2half2_rn(w1.x, w1.y);
-            w[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
-            w[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+            w[2 * i] = pack_half2(w0.x, w0.y);
+            w[2 * i + 1] = pack_half2(w1.x, w1.y);
           }
           __syncwarp();
           tmem_st8(s_addr + 8 * part, w);
         }
-        sum0 = add2(sum0, sum1);
-        l += sum0.x + sum0.y;
+        sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+        l += sum[0].x + sum[0].y;
       }
       tmem_wait_st();
       tc_fence_before();
