@@ -614,6 +614,8 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
       ((a->cache_k_row_stride % 16) != 0 || (a->cache_v_row_stride % 16) != 0 || a->cache_k_row_stride < sum_rk ||
        a->cache_v_row_stride < sum_rv || a->scale_k_row_stride < a->num_heads || a->scale_v_row_stride < a->num_heads))
     return LSVD_ERR_INVALID_ARG;
+  if (a->cache_layout == LSVD_CACHE_SLOT_MAJOR && (a->cache_k_row_stride > 0x7fffffffLL || a->cache_v_row_stride > 0x7fffffffLL))
+    return LSVD_ERR_UNSUPPORTED;
   const void* halves[] = {a->q, a->up_k, a->up_v, a->scale_k, a->scale_v, a->out, a->out_latent};
   for (const void* x : halves)
     if (!aligned(x, 2)) return LSVD_ERR_INVALID_ARG;
