@@ -28,8 +28,7 @@ constexpr int kGroups = 2;
 constexpr int kTileRows = kChunkTileRows;
 static_assert(kTileRows == kGroups * kGroupRows, "two products' rows");
 constexpr int kTileKeys = 64;
-constexpr int kHalves = 2;                       // threads that share a row: each takes half of a tile's keys
-constexpr int kSoftmaxWarps = 4 * kGroups * kHalves, kLoadWarps = 3;
+constexpr int kSoftmaxWarps = 4 * kGroups, kLoadWarps = 3;
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
 constexpr int kTileThreads = (kMmaWarp + 1) * 32;
 constexpr int kLoadThreads = kLoadWarps * 32;
@@ -45,7 +44,7 @@ constexpr int kTileShift = 6;
 
 struct __align__(16) TileShared {
   float sk[kTileMaxStages][kTileKeys], sv[kTileMaxStages][kTileKeys];      // first: read in 16-byte pieces
-  uint64_t k_full[kTileMaxStages], k_empty[kTileMaxStages], v_full[kTileMaxStages], v_empty[kTileMaxStages];
+  uint64_t full[kTileMaxStages], empty[kTileMaxStages];
   uint64_t s_full[kGroups][2], p_full[kGroups][2], o_done[kGroups], q_full[kGroups], last;
   uint32_t live[kTileMaxStages][2];              // keys with a slot, one bit each
   int32_t E[kTileMaxStages];
@@ -54,10 +53,7 @@ struct __align__(16) TileShared {
   volatile uint32_t abort;
   int32_t b, tile;
   int32_t kbeg, kend;
-  int32_t first, rows;                           // the block's first row, and how many
   float scale[kTileRows];                        // power of two taken out of each q~ row
-  int32_t lo[kTileRows], hi[kTileRows];          // keys that each row sees
-  float both[kHalves][kTileRows];                // what the two threads of a row tell one another
 };
 
 // ---- tcgen05 kind::f16 ------------------------------------------------------------------------------------------------
@@ -109,24 +105,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// Wait for a phase, bounded by kMbarTimeoutNs; also gives up once another role has.  False: stop and leave.  The thread is
-// suspended for up to a millisecond a poll: a dozen warps that poll at full speed take the load warps' issue slots.
-__device__ __forceinline__ bool tile_poll(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u) : "memory");
-  return ok != 0;
-}
+// Wait for a phase, bounded by kMbarTimeoutNs; also gives up once another role has.  False: stop and leave.
 __device__ __forceinline__ bool tile_wait(TileShared& s, uint64_t* bar, uint32_t parity, int32_t* status_word) {
-  if (tile_poll(bar, parity)) return true;
+  if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
   for (uint32_t i = 0; i < kMbarMaxPolls; ++i) {
-    if (tile_poll(bar, parity)) return true;
-    if (s.abort || global_timer_ns() - t0 > kMbarTimeoutNs) break;
+    if (mbar_try_wait(bar, parity)) return true;
+    if (s.abort) return false;
+    if ((i & 63u) == 63u && global_timer_ns() - t0 > kMbarTimeoutNs) break;
   }
-  if (!s.abort) report_status(status_word, LSVD_ERR_TIMEOUT);
   s.abort = 1;
+  report_status(status_word, LSVD_ERR_TIMEOUT);
   return false;
 }
 
@@ -144,119 +133,70 @@ __device__ __forceinline__ void store_codes(uint8_t* tile, int row, int piece, u
   *reinterpret_cast<uint4*>(tile + swizzled(row, 2 * piece + 1)) = b;
 }
 
-// A tile's rows of N 16-byte pieces: thread lt of the load warps has piece lt % N of rows lt / N, + kStep, ...  N is a
-// compile-time number (1 to 8) so that every offset is: with runtime steps the load warps spent 3000 instructions a tile.
-template <int N>
-struct TileRows {
-  static constexpr int kStep = kLoadThreads / N < kTileKeys ? kLoadThreads / N : kTileKeys;
-  static constexpr int kPasses = (kTileKeys + kStep - 1) / kStep;
-};
-template <int N>
-__device__ __forceinline__ void copy_rows(int lt, const int32_t* slots, uint8_t* dst, const int8_t* src, uint32_t stride) {
-  using R = TileRows<N>;
-  const int row = lt / N, piece = lt % N;
-  if (row >= R::kStep) return;
-#pragma unroll
-  for (int i = 0; i < R::kPasses; ++i)
-    if (row + i * R::kStep < kTileKeys) {
-      const int slot = slots[row + i * R::kStep];
-      copy16_or_zero(dst + lt * 16 + i * (R::kStep * N * 16), src + static_cast<uint64_t>(static_cast<uint32_t>(max(slot, 0))) * stride + piece * 16,
-                     slot >= 0);
-    }
-}
-template <int N>
-__device__ __forceinline__ void widen_rows(int lt, const uint8_t* src, uint8_t* tile) {
-  using R = TileRows<N>;
-  const int row = lt / N, piece = lt % N;
-  if (row >= R::kStep) return;
-  tile += (piece >> 2) * kTileKeys * 128;
-#pragma unroll
-  for (int i0 = 0; i0 < R::kPasses; i0 += 2) {
-    uint4 w[2];
-#pragma unroll
-    for (int i = i0; i < i0 + 2 && i < R::kPasses; ++i)
-      if (row + i * R::kStep < kTileKeys) w[i - i0] = *reinterpret_cast<const uint4*>(src + lt * 16 + i * (R::kStep * N * 16));
-#pragma unroll
-    for (int i = i0; i < i0 + 2 && i < R::kPasses; ++i)
-      if (row + i * R::kStep < kTileKeys) store_codes(tile, row + i * R::kStep, piece & 3, w[i - i0]);
-  }
-}
-__device__ __forceinline__ void copy_rows(int n, int lt, const int32_t* slots, uint8_t* dst, const int8_t* src, uint32_t stride) {
-  asm volatile("" : "+r"(lt));        // nothing of the eight forms is to be worked out ahead of the loop and kept (spills)
-  switch (n) {
-    case 1: return copy_rows<1>(lt, slots, dst, src, stride);
-    case 2: return copy_rows<2>(lt, slots, dst, src, stride);
-    case 3: return copy_rows<3>(lt, slots, dst, src, stride);
-    case 4: return copy_rows<4>(lt, slots, dst, src, stride);
-    case 5: return copy_rows<5>(lt, slots, dst, src, stride);
-    case 6: return copy_rows<6>(lt, slots, dst, src, stride);
-    case 7: return copy_rows<7>(lt, slots, dst, src, stride);
-    default: return copy_rows<8>(lt, slots, dst, src, stride);
-  }
-}
-__device__ __forceinline__ void widen_rows(int n, int lt, const uint8_t* src, uint8_t* tile) {
-  asm volatile("" : "+r"(lt));
-  switch (n) {
-    case 1: return widen_rows<1>(lt, src, tile);
-    case 2: return widen_rows<2>(lt, src, tile);
-    case 3: return widen_rows<3>(lt, src, tile);
-    case 4: return widen_rows<4>(lt, src, tile);
-    case 5: return widen_rows<5>(lt, src, tile);
-    case 6: return widen_rows<6>(lt, src, tile);
-    case 7: return widen_rows<7>(lt, src, tile);
-    default: return widen_rows<8>(lt, src, tile);
-  }
-}
-
-// q~ = B_k q of the warp's 16 rows (mma m16n8k16, like the stream form's), as fp16 rows of the A operand relative to each
+// q~ = B_k q of the warp's 32 rows (mma m16n8k16, like the stream form's), as fp16 rows of the A operand relative to each
 // row's largest entry; the powers of two go to s.scale.  Ranks in blocks of 64: with two blocks the first is computed again
 // once the row's largest entry over both is known (its accumulators do not fit beside the second's).
 __device__ __forceinline__ void absorb_tile_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int row0, int rows,
                                                  TileShared& s, uint8_t* q_tile) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int rk = H.nk * 16, first = warp * 16;      // rows of the block; q_tile is the group's
-  const __half* qa = p.q + static_cast<int64_t>(r.start + row0 + min(first + g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
-  const __half* qb = p.q + static_cast<int64_t>(r.start + row0 + min(first + 8 + g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
-  float acc[8][4], top[2] = {0.f, 0.f};
+  const int rk = H.nk * 16, first = warp * 32;      // rows of the block; q_tile is the group's
+  const __half* q[2][2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      q[m][e] = p.q + static_cast<int64_t>(r.start + row0 + min(first + 16 * m + 8 * e + g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+  float acc[2][8][4], top[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
   const int blocks = rk > 64 ? 2 : 1;
 #pragma unroll 1
   for (int pass = 0; pass < (blocks == 2 ? 3 : 1); ++pass) {      // block 0, block 1, block 0 again
     const int rank0 = pass == 1 ? 64 : 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
 #pragma unroll 1
     for (int d0 = 0; d0 < p.head_dim; d0 += 16) {
       const int d = d0 + 4 * t;
-      const uint2 a0 = load_halves4(qa + d, p.head_dim - d, p.q_vec), a1 = load_halves4(qb + d, p.head_dim - d, p.q_vec);
+      uint2 a[2][2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) a[m][e] = load_halves4(q[m][e] + d, p.head_dim - d, p.q_vec);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         uint2 b = make_uint2(0u, 0u);
         const int rank = rank0 + 8 * j + g;
         if (rank < rk) b = load_halves4(p.up_k + static_cast<int64_t>(H.k_col + rank) * p.up_k_row_stride + d, p.head_dim - d, p.up_k_vec);
-        mma_f16_16x8x16(acc[j], a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) mma_f16_16x8x16(acc[m][j], a[m][0].x, a[m][1].x, a[m][0].y, a[m][1].y, b.x, b.y);
       }
     }
     if (pass < 2) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top[e] = fmaxf(top[e], fmaxf(fabsf(acc[j][2 * e]), fabsf(acc[j][2 * e + 1])));
-        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-      }
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top[m][e] = fmaxf(top[m][e], fmaxf(fabsf(acc[m][j][2 * e]), fabsf(acc[m][j][2 * e + 1])));
+          top[m][e] = fmaxf(top[m][e], __shfl_xor_sync(0xffffffffu, top[m][e], 1));
+          top[m][e] = fmaxf(top[m][e], __shfl_xor_sync(0xffffffffu, top[m][e], 2));
+        }
     }
     if (pass == 0 && blocks == 2) continue;
     uint8_t* block = q_tile + (rank0 >> 6) * kGroupRows * 128;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int ex = exponent_of(top[e]) - 8, row = first + 8 * e + g;      // entries end up below 2^9
-      const float x = pow2i(-ex);
-      if (t == 0) s.scale[row] = pow2i(ex);
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (rank0 + 8 * j < rk)
-          *reinterpret_cast<uint32_t*>(block + swizzled(row & (kGroupRows - 1), j) + 4 * t) = pack_half2(acc[j][2 * e] * x, acc[j][2 * e + 1] * x);
-    }
+      for (int e = 0; e < 2; ++e) {
+        const int ex = exponent_of(top[m][e]) - 8, row = first + 16 * m + 8 * e + g;      // entries end up below 2^9
+        const float x = pow2i(-ex);
+        if (t == 0) s.scale[row] = pow2i(ex);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (rank0 + 8 * j < rk)
+            *reinterpret_cast<uint32_t*>(block + swizzled(row & (kGroupRows - 1), j) + 4 * t) = pack_half2(acc[m][j][2 * e] * x, acc[m][j][2 * e + 1] * x);
+      }
   }
 }
 
@@ -275,24 +215,31 @@ __device__ __forceinline__ void chunk_tile_up(const ChunkParams& p, const TileSh
         load_halves4(p.up_v + static_cast<int64_t>(H.v_col + rank) * p.up_v_row_stride + d, 4, p.up_v_vec);
   }
   __syncthreads();
-  if (warp * 16 >= rows) return;
-  {
-    const int ra = warp * 16 + g, rb = ra + 8, la = ra & (kGroupRows - 1), lb = la + 8;
+  if (warp >= kSoftmaxWarps || warp * 32 >= rows) return;
 #pragma unroll 1
+  for (int m = 0; m < 2; ++m) {
+    const int ra = warp * 32 + 16 * m + g, rb = ra + 8, la = ra & (kGroupRows - 1), lb = la + 8;
+    uint32_t a[8][4];
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < H.nv) {
+        const uint8_t* block = smem + (warp >> 2) * q_bytes + (q >> 2) * kGroupRows * 128;
+        const int c = 2 * (q & 3);
+        a[q][0] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c) + 4 * t);
+        a[q][1] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c) + 4 * t);
+        a[q][2] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c + 1) + 4 * t);
+        a[q][3] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c + 1) + 4 * t);
+      }
     for (int d0 = 0; d0 < p.head_dim; d0 += 8) {
       float y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-      for (int q = 0; q < H.nv; ++q) {
-        const uint8_t* block = smem + (warp >> 3) * q_bytes + (q >> 2) * kGroupRows * 128;
-        const int c = 2 * (q & 3);
-        const uint16_t* at = reinterpret_cast<const uint16_t*>(up) + (16 * q + 2 * t) * p.head_dim + d0 + g;
-        const uint32_t b0 = at[0] | (static_cast<uint32_t>(at[p.head_dim]) << 16);
-        const uint32_t b1 = at[8 * p.head_dim] | (static_cast<uint32_t>(at[9 * p.head_dim]) << 16);
-        mma_f16_16x8x16(y, *reinterpret_cast<const uint32_t*>(block + swizzled(la, c) + 4 * t),
-                        *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c) + 4 * t),
-                        *reinterpret_cast<const uint32_t*>(block + swizzled(la, c + 1) + 4 * t),
-                        *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c + 1) + 4 * t), b0, b1);
-      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < H.nv) {
+          const uint16_t* at = reinterpret_cast<const uint16_t*>(up) + (16 * q + 2 * t) * p.head_dim + d0 + g;
+          const uint32_t b0 = at[0] | (static_cast<uint32_t>(at[p.head_dim]) << 16);
+          const uint32_t b1 = at[8 * p.head_dim] | (static_cast<uint32_t>(at[9 * p.head_dim]) << 16);
+          mma_f16_16x8x16(y, a[q][0], a[q][1], a[q][2], a[q][3], b0, b1);
+        }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = e == 0 ? ra : rb;
@@ -363,10 +310,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       s.kend = 0;
       s.abort = 0;
       for (int i = 0; i < kTileMaxStages; ++i) {
-        mbar_init(&s.k_full[i], kLoadWarps);
-        mbar_init(&s.k_empty[i], 1);
-        mbar_init(&s.v_full[i], kLoadWarps);
-        mbar_init(&s.v_empty[i], 1);
+        mbar_init(&s.full[i], kLoadWarps);
+        mbar_init(&s.empty[i], 1);
       }
       for (int i = 0; i < kGroups; ++i) {
         mbar_init(&s.s_full[i][0], 1);
@@ -379,19 +324,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
   if (s.b < 0) return;
   const ChunkRequest r = chunk_request(p, s.b, false);
   const int row0 = s.tile * kTileRows, rows = min(kTileRows, r.n - row0);
+  const int live_warps = (rows + 31) >> 5;                // softmax warps with rows, and groups with such warps
   const int groups = (rows + kGroupRows - 1) / kGroupRows;
-  // The row of each softmax thread, and the block's keys.  Warp w of a group has the tensor memory lanes 32 (w % 4) .., that is
-  // the group's rows of that number, and the keys of half w / 4 of a tile.
-  const int grp = warp >> 3, half = (warp >> 2) & 1, row = grp * kGroupRows + (warp & 3) * 32 + lane;
-  const bool live = warp < kSoftmaxWarps && row - lane < rows;
+  // the row of each softmax thread, and the block's keys
   KeyRange keys;
   keys.lo = keys.hi = 0;
-  if (live && row < rows) keys = visible_keys(p, r, p.b_prefix_len != nullptr ? p.b_prefix_len[s.b] : 0, row0 + row);
+  if (tid < rows) keys = visible_keys(p, r, p.b_prefix_len != nullptr ? p.b_prefix_len[s.b] : 0, row0 + tid);
   if (warp < kSoftmaxWarps) {
-    if (half == 0) {
-      s.lo[row] = keys.lo;
-      s.hi[row] = keys.hi;
-    }
     const int lo = __reduce_min_sync(0xffffffffu, keys.hi > keys.lo ? keys.lo : 0x7fffffff);
     const int hi = __reduce_max_sync(0xffffffffu, keys.hi);
     if (lane == 0 && hi > 0) {
@@ -400,13 +339,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     }
   }
   if (tid == 0) {
-    s.first = r.start + row0;
-    s.rows = rows;
     for (int i = 0; i < groups; ++i) {
-      const int mine = min(kGroupRows, rows - i * kGroupRows);
-      mbar_init(&s.p_full[i][0], kHalves * ((mine + 31) / 32));
-      mbar_init(&s.p_full[i][1], kHalves * ((mine + 31) / 32));
-      mbar_init(&s.q_full[i], (mine + 15) / 16);
+      const int warps = min(4, live_warps - 4 * i);
+      mbar_init(&s.p_full[i][0], warps);
+      mbar_init(&s.p_full[i][1], warps);
+      mbar_init(&s.q_full[i], warps);
     }
     mbar_init(&s.last, 1);
     fence_mbar_init();
@@ -434,7 +371,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     // scores of tile j for both groups; a group's buffer still holds the weights of tile j - 2 until their product is done
     auto scores = [&](int j) {
       const int st = j & (stages - 1);
-      if (!wait(&s.k_full[st], (j / stages) & 1)) return false;
+      if (!wait(&s.full[st], (j / stages) & 1)) return false;
 #pragma unroll
       for (int grp = 0; grp < kGroups; ++grp) {
         if (grp >= groups) continue;
@@ -446,7 +383,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
             umma_f16_ss(tmem + grp * kGroupCols + (j & 1) * kTileKeys, qdesc + ((q >> 2) * (kGroupRows * 128 >> 4) + (q & 3) * 2),
                         kdesc + ((q >> 2) * (kTileKeys * 128 >> 4) + (q & 3) * 2), idesc_s, q > 0 ? 1u : 0u);
           umma_commit(&s.s_full[grp][j & 1]);
-          if (grp + 1 == groups) umma_commit(&s.k_empty[st]);
         }
         __syncwarp();
       }
@@ -458,7 +394,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     if (ntiles > 1) go = go && scores(1);
     for (int j = 0; go && j < ntiles; ++j) {
       const int st = j & (stages - 1);
-      go = wait(&s.v_full[st], (j / stages) & 1);
 #pragma unroll
       for (int grp = 0; grp < kGroups; ++grp) {
         if (!go || grp >= groups) continue;
@@ -472,7 +407,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
           for (int q = 0; q < kTileKeys / 16; ++q)    // 16 keys a step: two groups of eight rows; 8 columns of P
             umma_f16_ts(base + kColO, base + (j & 1) * kTileKeys + 8 * q, vdesc + q * (2048 >> 4), idesc_o, (j | q) != 0 ? 1u : 0u);
           umma_commit(&s.o_done[grp]);
-          if (grp + 1 == groups) umma_commit(&s.v_empty[st]);
+          if (grp + 1 == groups) umma_commit(&s.empty[st]);
         }
         __syncwarp();
       }
@@ -502,11 +437,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       }
       if (lt < kTileKeys) s.slot[j & (kTileSlotRing - 1)][lt] = slot;
     };
+    // A thread's pieces of a tile: 16-byte piece `piece` of rows row0, row0 + step, ... (threads beyond the last whole row: none).
+    // The passes are loops on purpose, and K and V share them: unrolled, the roles' code does not fit the instruction cache.
+    const int k_step = kLoadThreads / H.nk, v_step = kLoadThreads / H.nv;
+    const int k_row = lt / H.nk < k_step ? lt / H.nk : kTileKeys, v_row = lt / H.nv < v_step ? lt / H.nv : kTileKeys;
+    const int k_piece = lt % H.nk, v_piece = lt % H.nv;
     auto request = [&](int j) {
       const int32_t* slots = s.slot[j & (kTileSlotRing - 1)];
-      uint8_t* kd = codes + (j & (kCodeStages - 1)) * code_bytes;
-      copy_rows(H.nk, lt, slots, kd, kbase, kstride);
-      copy_rows(H.nv, lt, slots, kd + kTileKeys * rk, vbase, vstride);
+      uint8_t* dst = codes + (j & (kCodeStages - 1)) * code_bytes;
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        const int step = part ? v_step : k_step, bytes = part ? rv : rk;
+        const uint32_t stride = part ? vstride : kstride;
+        const int8_t* src = (part ? vbase + v_piece * 16 : kbase + k_piece * 16);
+        uint8_t* to = dst + lt * 16;
+#pragma unroll 1
+        for (int row = part ? v_row : k_row; row < kTileKeys; row += step, to += step * bytes) {
+          const int slot = slots[row];
+          copy16_or_zero(to, src + static_cast<uint64_t>(static_cast<uint32_t>(max(slot, 0))) * stride, slot >= 0);
+        }
+        dst += kTileKeys * rk;
+      }
+    };
+    auto widen = [&](const uint8_t* src, uint8_t* dst) {
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        const int step = part ? v_step : k_step, piece = part ? v_piece : k_piece, bytes = part ? rv : rk;
+        const uint8_t* from = src + lt * 16;
+        uint8_t* tile = dst + (piece >> 2) * kTileKeys * 128;
+#pragma unroll 1
+        for (int row = part ? v_row : k_row; row < kTileKeys; row += step, from += step * bytes)
+          store_codes(tile, row, piece & 3, *reinterpret_cast<const uint4*>(from));
+        src += kTileKeys * rk;
+        dst += k_bytes;
+      }
     };
     __half raw0 = __ushort_as_half(0), raw1 = raw0;
     int sl0 = -1, sl1 = -1, E = -200;
@@ -544,9 +508,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       copy_commit();
       uint8_t* kd = stage0 + st * stage_bytes;
       const uint8_t* kc = codes + (j & (kCodeStages - 1)) * code_bytes;
-      ok = tile_wait(s, &s.k_empty[st], ((j / stages) & 1) ^ 1, p.status_word);
-      ok = ok && tile_wait(s, &s.v_empty[st], ((j / stages) & 1) ^ 1, p.status_word);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = __all_sync(0xffffffffu, tile_wait(s, &s.empty[st], ((j / stages) & 1) ^ 1, p.status_word));
       if (!ok) continue;
       // the scales go first: the softmax reads them once K is there
       const float sc0 = sl0 >= 0 ? __half2float(raw0) : 0.f, sc1 = sl1 >= 0 ? __half2float(raw1) : 0.f;
@@ -570,165 +532,182 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
         s.sk[st][lane + 32] = sc1;
       }
       load_scales(j + 1);
-      widen_rows(H.nk, lt, kc, kd);
+      widen(kc, kd);
       fence_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.k_full[st]);
-      widen_rows(H.nv, lt, kc + kTileKeys * rk, kd + k_bytes);
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.v_full[st]);
+      if (lane == 0) mbar_arrive(&s.full[st]);
     }
     copy_wait<0>();
-  } else if (warp < kSoftmaxWarps) {
-    // ================= softmax: two threads a row =================
-    if (ntiles > 0 && warp * 16 < rows) {
-      absorb_tile_rows(p, H, h, r, row0, rows, s, smem + grp * q_bytes);
+  } else if (warp < live_warps) {
+    // ================= softmax: thread = row =================
+    const int grp = warp >> 2;
+    uint8_t* q_tile = smem + grp * q_bytes;
+    const uint32_t lane_addr = tmem + grp * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int token = r.start + row0 + tid;
+    const int pos = r.len - r.n + row0 + tid;
+    float f = 0.f, m = -INFINITY, l = 0.f;
+    int E = -200;
+    bool go = true;
+    if (ntiles > 0) {
+      absorb_tile_rows(p, H, h, r, row0, rows, s, q_tile);
+      __syncwarp();
+      f = s.scale[tid];
+      f = fmaxf(f * p.score_scale * (kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e), 1e-37f);
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.q_full[grp]);
     }
-    const uint32_t lane_addr = tmem + grp * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const int pos = kBias ? r.len - r.n + row0 + row : 0, partner = 2 + grp * 4 + (warp & 3);      // named barrier of the rows' two warps
-    float f = 0.f, m = -INFINITY, l = 0.f;
-    int E = -200;
-    bool go = live;
-    if (go && ntiles > 0) {
-      go = __all_sync(0xffffffffu, tile_wait(s, &s.q_full[grp], 0, p.status_word));
-      f = fmaxf(s.scale[row] * p.score_scale * (kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e), 1e-37f);
-    }
     const float cap_log2e = p.softcap * kChunkLog2e;
     const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
-    // A wait that gave up: both warps of the rows learn of it at their next common barrier (or have no further one).
-    for (int j = 0; live && j < ntiles; ++j) {
+    // keys that every row of the warp sees
+    const int inner_lo = __reduce_max_sync(0xffffffffu, tid < rows ? keys.lo : 0);
+    const int inner_hi = __reduce_min_sync(0xffffffffu, tid < rows ? keys.hi : 0x7fffffff);
+    const int outer_lo = __reduce_min_sync(0xffffffffu, keys.hi > keys.lo ? keys.lo : 0x7fffffff);
+    const int outer_hi = __reduce_max_sync(0xffffffffu, keys.hi);
+
+    for (int j = 0; go && j < ntiles; ++j) {
       const int st = j & (stages - 1), k0 = kbeg + j * kTileKeys;
       const uint32_t s_addr = lane_addr + (j & 1) * kTileKeys;
-      go = go && tile_wait(s, &s.k_full[st], (j / stages) & 1, p.status_word) && tile_wait(s, &s.s_full[grp][j & 1], (j >> 1) & 1, p.status_word);
-      go = __all_sync(0xffffffffu, go);
+      go = tile_wait(s, &s.full[st], (j / stages) & 1, p.status_word) && tile_wait(s, &s.s_full[grp][j & 1], (j >> 1) & 1, p.status_word);
+      if (!__all_sync(0xffffffffu, go)) {
+        go = false;
+        break;
+      }
       tc_fence_after();
       const int e_new = s.E[st];
-      const int lo = s.lo[row], hi = s.hi[row];
-      const bool nothing = __all_sync(0xffffffffu, hi <= k0 || lo >= k0 + kTileKeys);      // (both warps of the rows find the same)
-      const int kh = k0 + 32 * half;                                          // this thread's first key
-      uint32_t mask = s.live[st][half];                                       // keys that the row sees
-      {
-        const int a = min(max(lo - kh, 0), 32), b = min(max(hi - kh, 0), 32);
-        mask &= (b >= 32 ? ~0u : (1u << b) - 1u) & (a >= 32 ? 0u : ~0u << a);
-      }
-      const bool masked = __any_sync(0xffffffffu, mask != ~0u && row < s.rows);
-      // O (this thread's columns) and the sum for a new reference (factor c) or a larger V scale; the product of tile j - 1 is
-      // waited for
-      auto rescale = [&](float c, int e) {
-        l *= c;
-        if (j == 0) return;
-        go = go && tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
-        go = __all_sync(0xffffffffu, go);
-        if (!go) return;
-        tc_fence_after();
-        const float by = c * pow2i(max(E - e, -126));
-        __syncwarp();
-#pragma unroll 1
-        for (int col = 16 * half; col < rv; col += 32) {
-          uint32_t v[16];
-          tmem_ld16(lane_addr + kColO + col, v);
+      const bool nothing = k0 >= outer_hi || k0 + kTileKeys <= outer_lo;      // of this warp's rows
+      const uint32_t live0 = s.live[st][0], live1 = s.live[st][1];
+      const bool masked = k0 < inner_lo || k0 + kTileKeys > inner_hi || (live0 & live1) != 0xffffffffu;
+      float2 x[kTileKeys / 2];
+      float top = -INFINITY;
+      if (!nothing) {
+        // (half by half: the scales of the second half are not fetched before the first half's scores are in)
+        const float4* sk = reinterpret_cast<const float4*>(s.sk[st]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
-          tmem_st16(lane_addr + kColO + col, v);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t raw[32];
+          __syncwarp();
+          tmem_ld32(s_addr + 32 * half, raw);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 c = sk[8 * half + i];
+            x[16 * half + 2 * i] = mul2(make_float2(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), make_float2(c.x, c.y));
+            x[16 * half + 2 * i + 1] = mul2(make_float2(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), make_float2(c.z, c.w));
+          }
         }
-        tmem_wait_st();              // it may be read again in this tile
-      };
-      if (e_new != E) {
-        rescale(1.f, e_new);
-        E = e_new;
-      }
-      uint32_t w[2][8];
-      float2 sum = make_float2(0.f, 0.f);
-      if (nothing) {
+        if (kCap || kBias) {
+          const float away = static_cast<float>(pos - k0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = 0u;
-      } else {
-        const float4* sk = reinterpret_cast<const float4*>(s.sk[st] + 32 * half);
-        const float4* sv = reinterpret_cast<const float4*>(s.sv[st] + 32 * half);
-        const float away = static_cast<float>(pos - kh);
-        // One pass: the weights against the row's reference so far, and how far the scores rise above it.  Where some row's rise
-        // is more than 2^8 (the first tile, hardly any after it) the reference moves and the tile is worked through again.
-#pragma unroll 1
-        for (int pass = 0;; ++pass) {
-          asm volatile("" : "+r"(mask));       // its tests are not to be kept across the passes (spills)
-          const float base = m == -INFINITY ? 0.f : m;
-          const float2 nb = make_float2(-base, -base), ff = make_float2(f, f);
-          float t0 = -INFINITY, t1 = -INFINITY;
-          sum = make_float2(0.f, 0.f);
+          for (int i = 0; i < kTileKeys / 2; ++i) {
+            float a = x[i].x * f, b = x[i].y * f;
+            if (kCap) {
+              a = capped_log2(a, cap_log2e);
+              b = capped_log2(b, cap_log2e);
+            }
+            if (kBias) {
+              a = fmaf(-slope, fabsf(away - static_cast<float>(2 * i)), a);
+              b = fmaf(-slope, fabsf(away - static_cast<float>(2 * i + 1)), b);
+            }
+            x[i] = make_float2(a, b);
+          }
+        }
+        if (masked) {
+          const int a = min(max(keys.lo - k0, 0), 64), b = min(max(keys.hi - k0, 0), 64);
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            uint32_t raw[16];
-            __syncwarp();
-            tmem_ld16(s_addr + 32 * half + 16 * part, raw);
+          for (int w = 0; w < 2; ++w) {            // bits of the keys that the row sees, 32 at a time
+            const int from = min(max(a - 32 * w, 0), 32), upto = min(max(b - 32 * w, 0), 32);
+            const uint32_t mask = (w == 0 ? live0 : live1) & (upto >= 32 ? ~0u : (1u << upto) - 1u) & (from >= 32 ? 0u : ~0u << from);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float4 ck = sk[4 * part + i], cv = sv[4 * part + i];
-              float2 y[2] = {mul2(make_float2(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), make_float2(ck.x, ck.y)),
-                             mul2(make_float2(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), make_float2(ck.z, ck.w))};
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int key = 16 * part + 4 * i + 2 * e;
-                if (kCap || kBias) {
-                  float u = y[e].x * f, v = y[e].y * f;
-                  if (kCap) {
-                    u = capped_log2(u, cap_log2e);
-                    v = capped_log2(v, cap_log2e);
-                  }
-                  if (kBias) {
-                    u = fmaf(-slope, fabsf(away - static_cast<float>(key)), u);
-                    v = fmaf(-slope, fabsf(away - static_cast<float>(key + 1)), v);
-                  }
-                  y[e] = add2(make_float2(u, v), nb);
-                } else {
-                  y[e] = fma2(y[e], ff, nb);
-                }
-                if (masked) {
-                  if (!((mask >> key) & 1u)) y[e].x = -INFINITY;
-                  if (!((mask >> (key + 1)) & 1u)) y[e].y = -INFINITY;
-                }
-              }
-              t0 = max3(t0, y[0].x, y[0].y);
-              t1 = max3(t1, y[1].x, y[1].y);
-              const float2 p0 = make_float2(ex2(y[0].x), ex2(y[0].y)), p1 = make_float2(ex2(y[1].x), ex2(y[1].y));
-              sum = add2(sum, add2(p0, p1));
-              float2 w0 = mul2(p0, make_float2(cv.x, cv.y)), w1 = mul2(p1, make_float2(cv.z, cv.w));
-              if (masked) {             // a masked key's weight is zero whatever its scale holds
-                if (p0.x == 0.f) w0.x = 0.f;
-                if (p0.y == 0.f) w0.y = 0.f;
-                if (p1.x == 0.f) w1.x = 0.f;
-                if (p1.y == 0.f) w1.y = 0.f;
-              }
-              w[part][2 * i] = pack_half2(w0.x, w0.y);
-              w[part][2 * i + 1] = pack_half2(w1.x, w1.y);
+            for (int i = 0; i < 16; ++i) {
+              if (!((mask >> (2 * i)) & 1u)) x[16 * w + i].x = -INFINITY;
+              if (!((mask >> (2 * i + 1)) & 1u)) x[16 * w + i].y = -INFINITY;
             }
           }
-          float rise = fmaxf(t0, t1);
-          const bool first = m == -INFINITY;
-          // The barrier also lets no weight be stored over scores that the other warp has not read.
-          const bool again = named_barrier_or(partner, 64, pass == 0 && (first ? rise > -INFINITY : rise > kLazy));
-          if (!again) break;
-          s.both[half][row] = rise;
-          named_barrier(partner, 64);
-          rise = fmaxf(rise, s.both[half ^ 1][row]);
-          named_barrier(partner, 64);
-          const bool moves = first ? rise > -INFINITY : rise > kLazy;
-          // (a first reference finds O and the sum at zero: times 1 keeps a NaN of a row that has one)
-          rescale(moves && !first ? ex2(-rise) : 1.f, E);
-          if (moves) m = base + rise;
         }
-      }
-      l += sum.x + sum.y;
-      __syncwarp();
-      if (go) {
+        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-        for (int part = 0; part < 2; ++part) tmem_st8(s_addr + 16 * half + 8 * part, w[part]);
+        for (int i = 0; i < kTileKeys / 2; i += 2) {
+          t0 = max3(t0, x[i].x, x[i].y);
+          t1 = max3(t1, x[i + 1].x, x[i + 1].y);
+        }
+        top = fmaxf(t0, t1);
+        if (!kCap && !kBias) top *= f;
+      }
+      // a new reference: the first maximum of a row, one that has grown by more than 2^8, or a larger V scale
+      const bool first = m == -INFINITY;
+      const bool grown = first ? top > -INFINITY : top > m + kLazy;
+      if (__any_sync(0xffffffffu, grown) || e_new != E) {
+        const float m_new = grown ? top : m;
+        const float c = first ? 0.f : ex2(m - m_new);
+        l *= c;
+        if (j > 0 && __any_sync(0xffffffffu, (grown && !first) || e_new != E)) {
+          go = tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
+          if (!__all_sync(0xffffffffu, go)) {
+            go = false;
+            break;
+          }
+          tc_fence_after();
+          const float by = (first ? 1.f : c) * pow2i(max(E - e_new, -126));
+          __syncwarp();
+#pragma unroll 1
+          for (int col = 0; col < rv; col += 16) {
+            uint32_t v[16];
+            tmem_ld16(lane_addr + kColO + col, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
+            tmem_st16(lane_addr + kColO + col, v);
+          }
+        }
+        m = m_new;
+        E = e_new;
+      }
+      __syncwarp();
+      if (nothing) {
+        uint32_t z[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i] = 0u;
+        tmem_st16(s_addr, z);
+        tmem_st16(s_addr + 16, z);
+      } else {
+        // exponentials in place (the unit that bounds the kernel works without a pause), then the weights
+        const float base = m == -INFINITY ? 0.f : m;
+        const float2 nb = make_float2(-base, -base), ff = make_float2(f, f);
+        float2 sum[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kTileKeys / 2; ++i) {
+          const float2 y = (kCap || kBias) ? add2(x[i], nb) : fma2(x[i], ff, nb);
+          x[i] = make_float2(ex2(y.x), ex2(y.y));
+          sum[i & 3] = add2(sum[i & 3], x[i]);
+        }
+        const float4* sv = reinterpret_cast<const float4*>(s.sv[st]);
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {         // (16-column stores cost spills)
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 p0 = x[8 * part + 2 * i], p1 = x[8 * part + 2 * i + 1];
+            const float4 c = sv[4 * part + i];
+            float2 w0 = mul2(p0, make_float2(c.x, c.y)), w1 = mul2(p1, make_float2(c.z, c.w));
+            if (masked) {             // a masked key's weight is zero whatever its scale holds
+              if (p0.x == 0.f) w0.x = 0.f;
+              if (p0.y == 0.f) w0.y = 0.f;
+              if (p1.x == 0.f) w1.x = 0.f;
+              if (p1.y == 0.f) w1.y = 0.f;
+            }
+            w[2 * i] = pack_half2(w0.x, w0.y);
+            w[2 * i + 1] = pack_half2(w1.x, w1.y);
+          }
+          __syncwarp();
+          tmem_st8(s_addr + 8 * part, w);
+        }
+        sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+        l += sum[0].x + sum[0].y;
       }
       tmem_wait_st();
       tc_fence_before();
+      __syncwarp();
       // Phases are told apart by parity alone: before the last product is let go, the one in front of it is seen to have ended.
       if (j > 0 && j + 1 == ntiles) go = go && tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
       go = __all_sync(0xffffffffu, go);
@@ -736,23 +715,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     }
 
     // ---- results -------------------------------------------------------------------------------------------------------
+    // (all that is known here is that the product of tile ntiles - 3 is done: a phase is waited for by its parity, one by one)
     if (go && ntiles > 0) go = tile_wait(s, &s.o_done[grp], (ntiles - 1) & 1, p.status_word);
     go = __all_sync(0xffffffffu, go);
     tc_fence_after();
-    if (live) {
-      s.both[half][row] = l;
-      named_barrier(partner, 64);
-      l += s.both[half ^ 1][row];
-    }
     if (go) {
-      const int token = s.first + row;
       const float back = ntiles > 0 ? (E > -200 ? pow2i(E - kTileShift) : 1.f) : 0.f;
       const float by = p.tile_splits > 1 ? back : (l == 0.f ? 0.f : back / l);
       const bool to_up = p.out != nullptr && p.tile_splits == 1;
       const int64_t part = static_cast<int64_t>(split) * p.num_tokens + token;
-      if (p.tile_splits > 1 && row < s.rows && half == 0) p.tile_ml[part * p.num_heads + h] = make_float2(m, l);
+      if (p.tile_splits > 1 && tid < rows) p.tile_ml[part * p.num_heads + h] = make_float2(m, l);
 #pragma unroll 1
-      for (int c = 16 * half; c < rv; c += 32) {
+      for (int c = 0; c < rv; c += 16) {
         uint32_t v[16];
         float y[16];
         __syncwarp();
@@ -760,30 +734,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
 #pragma unroll
         for (int i = 0; i < 16; ++i) y[i] = (ntiles > 0 && by != 0.f) ? __uint_as_float(v[i]) * by : 0.f;
         if (p.tile_splits > 1) {
-          if (row < s.rows && ntiles > 0) {
+          if (tid < rows && ntiles > 0) {
             float4* dst = reinterpret_cast<float4*>(p.tile_o + part * p.sum_rv + H.v_col + c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
           }
           continue;
         }
-        const uint4 lo = make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]), pack_half2(y[4], y[5]), pack_half2(y[6], y[7]));
-        const uint4 hi = make_uint4(pack_half2(y[8], y[9]), pack_half2(y[10], y[11]), pack_half2(y[12], y[13]), pack_half2(y[14], y[15]));
-        if (p.out_latent != nullptr && row < s.rows) {
+        __align__(16) __half2 hh[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hh[i] = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
+        const uint4 lo = *reinterpret_cast<const uint4*>(&hh[0]), hi = *reinterpret_cast<const uint4*>(&hh[4]);
+        if (p.out_latent != nullptr && tid < rows) {
           __half* dst = p.out_latent + token * p.out_latent_stride_t + H.v_col + c;
           store_halves8(dst, lo, p.out_lat_vec16);
           store_halves8(dst + 8, hi, p.out_lat_vec16);
         }
         if (to_up && ntiles > 0) {
-          uint8_t* block = smem + grp * q_bytes + (c >> 6) * kGroupRows * 128;
-          const int piece = (c & 63) >> 3;
-          *reinterpret_cast<uint4*>(block + swizzled(row & (kGroupRows - 1), piece)) = lo;
-          *reinterpret_cast<uint4*>(block + swizzled(row & (kGroupRows - 1), piece + 1)) = hi;
+          uint8_t* block = q_tile + (c >> 6) * kGroupRows * 128;
+          const int piece = (c & 63) >> 3, row = tid & (kGroupRows - 1);
+          *reinterpret_cast<uint4*>(block + swizzled(row, piece)) = lo;
+          *reinterpret_cast<uint4*>(block + swizzled(row, piece + 1)) = hi;
         }
       }
-      if (to_up && ntiles == 0 && half == 0 && row < s.rows)
+      if (to_up && ntiles == 0 && tid < rows)
         for (int d = 0; d < p.head_dim; ++d) p.out[token * p.out_stride_t + h * p.out_stride_h + d] = __float2half_rn(0.f);
-    } else if (live) {
+    } else {
       s.abort = 1;
     }
   }
