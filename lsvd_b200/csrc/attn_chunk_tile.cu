@@ -99,6 +99,11 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r)::"memory");
   return r != 0u;
 }
+// Four 8 x 8 tiles of halves, transposed: lane i gives the address of row i & 7 of tile i >> 3.
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const uint8_t* row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(row)) : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -133,70 +138,77 @@ __device__ __forceinline__ void store_codes(uint8_t* tile, int row, int piece, u
   *reinterpret_cast<uint4*>(tile + swizzled(row, 2 * piece + 1)) = b;
 }
 
-// q~ = B_k q of the warp's 32 rows (mma m16n8k16, like the stream form's), as fp16 rows of the A operand relative to each
-// row's largest entry; the powers of two go to s.scale.  Ranks in blocks of 64: with two blocks the first is computed again
-// once the row's largest entry over both is known (its accumulators do not fit beside the second's).
+// q~ = B_k q of the block's rows (mma m16n8k16, like the stream form's; a warp has 32), as fp16 rows of the A operand relative to
+// each row's largest entry; the powers of two go to s.scale.  The factor is first brought to `up`, 64 ranks at a time, by the
+// `warps` warps that come here (read from global memory by every warp, 8 bytes a lane, the block's prologue took 34000 cycles).
+// With more than 64 ranks the first block is computed again once the row's largest entry over both is known.
 __device__ __forceinline__ void absorb_tile_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int row0, int rows,
-                                                 TileShared& s, uint8_t* q_tile) {
+                                                 int warps, TileShared& s, uint8_t* q_tile, uint8_t* up) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int rk = H.nk * 16, first = warp * 32;      // rows of the block; q_tile is the group's
-  const __half* q[2][2];
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      q[m][e] = p.q + static_cast<int64_t>(r.start + row0 + min(first + 16 * m + 8 * e + g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
-  float acc[2][8][4], top[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-  const int blocks = rk > 64 ? 2 : 1;
+  const int rk = H.nk * 16, blocks = rk > 64 ? 2 : 1;
+  const int steps = (p.head_dim + 15) >> 4, stride = ((p.head_dim * 2 + 127) & ~127) + 32;      // (rows of lanes g on other banks)
+  float top[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll 1
   for (int pass = 0; pass < (blocks == 2 ? 3 : 1); ++pass) {      // block 0, block 1, block 0 again
     const int rank0 = pass == 1 ? 64 : 0;
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
-#pragma unroll 1
-    for (int d0 = 0; d0 < p.head_dim; d0 += 16) {
-      const int d = d0 + 4 * t;
-      uint2 a[2][2];
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) a[m][e] = load_halves4(q[m][e] + d, p.head_dim - d, p.q_vec);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint2 b = make_uint2(0u, 0u);
-        const int rank = rank0 + 8 * j + g;
-        if (rank < rk) b = load_halves4(p.up_k + static_cast<int64_t>(H.k_col + rank) * p.up_k_row_stride + d, p.head_dim - d, p.up_k_vec);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) mma_f16_16x8x16(acc[m][j], a[m][0].x, a[m][1].x, a[m][0].y, a[m][1].y, b.x, b.y);
-      }
+    if (pass > 0) named_barrier(2, warps * 32);
+#pragma unroll 4
+    for (int x = threadIdx.x; x < 64 * 4 * steps; x += warps * 32) {
+      const int rank = x / (4 * steps), d = (x - rank * (4 * steps)) * 4;
+      uint2 v = make_uint2(0u, 0u);
+      if (rank0 + rank < rk) v = load_halves4(p.up_k + static_cast<int64_t>(H.k_col + rank0 + rank) * p.up_k_row_stride + d, p.head_dim - d, p.up_k_vec);
+      *reinterpret_cast<uint2*>(up + rank * stride + d * 2) = v;
     }
-    if (pass < 2) {
+    named_barrier(2, warps * 32);
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m) {
+      const int first = warp * 32 + 16 * m;
+      const __half* qa = p.q + static_cast<int64_t>(r.start + row0 + min(first + g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+      const __half* qb = p.q + static_cast<int64_t>(r.start + row0 + min(first + 8 + g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+      float acc[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll 1
+      for (int s0 = 0; s0 < steps; s0 += 8) {
+        uint2 a[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int d = (s0 + i) * 16 + 4 * t;
+          a[i] = load_halves4(qa + d, p.head_dim - d, p.q_vec);
+          b[i] = load_halves4(qb + d, p.head_dim - d, p.q_vec);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (s0 + i >= steps) continue;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint2 u = *reinterpret_cast<const uint2*>(up + (8 * j + g) * stride + (s0 + i) * 32 + 8 * t);
+            mma_f16_16x8x16(acc[j], a[i].x, b[i].x, a[i].y, b[i].y, u.x, u.y);
+          }
+        }
+      }
+      if (pass < 2) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) top[m][e] = fmaxf(top[m][e], fmaxf(fabsf(acc[m][j][2 * e]), fabsf(acc[m][j][2 * e + 1])));
+          for (int j = 0; j < 8; ++j) top[m][e] = fmaxf(top[m][e], fmaxf(fabsf(acc[j][2 * e]), fabsf(acc[j][2 * e + 1])));
           top[m][e] = fmaxf(top[m][e], __shfl_xor_sync(0xffffffffu, top[m][e], 1));
           top[m][e] = fmaxf(top[m][e], __shfl_xor_sync(0xffffffffu, top[m][e], 2));
         }
-    }
-    if (pass == 0 && blocks == 2) continue;
-    uint8_t* block = q_tile + (rank0 >> 6) * kGroupRows * 128;
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
+      }
+      if (pass == 0 && blocks == 2) continue;
+      uint8_t* block = q_tile + (rank0 >> 6) * kGroupRows * 128;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int ex = exponent_of(top[m][e]) - 8, row = first + 16 * m + 8 * e + g;      // entries end up below 2^9
+        const int ex = exponent_of(top[m][e]) - 8, row = first + 8 * e + g;      // entries end up below 2^9
         const float x = pow2i(-ex);
         if (t == 0) s.scale[row] = pow2i(ex);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (rank0 + 8 * j < rk)
-            *reinterpret_cast<uint32_t*>(block + swizzled(row & (kGroupRows - 1), j) + 4 * t) = pack_half2(acc[m][j][2 * e] * x, acc[m][j][2 * e + 1] * x);
+            *reinterpret_cast<uint32_t*>(block + swizzled(row & (kGroupRows - 1), j) + 4 * t) = pack_half2(acc[j][2 * e] * x, acc[j][2 * e + 1] * x);
       }
+    }
   }
 }
 
@@ -208,44 +220,49 @@ __device__ __forceinline__ void chunk_tile_up(const ChunkParams& p, const TileSh
   const int rv = H.nv * 16, q_bytes = ((max(H.nk, H.nv) + 3) >> 2) * kGroupRows * 128;
   const ChunkRequest r = chunk_request(p, s.b, false);
   const int row0 = s.tile * kTileRows, rows = min(kTileRows, r.n - row0);
-  __half* up = reinterpret_cast<__half*>(smem + kGroups * q_bytes);
-  for (int x = tid; x < rv * (p.head_dim >> 2); x += kTileThreads) {
-    const int rank = x / (p.head_dim >> 2), d = (x - rank * (p.head_dim >> 2)) * 4;
-    *reinterpret_cast<uint2*>(up + rank * p.head_dim + d) =
-        load_halves4(p.up_v + static_cast<int64_t>(H.v_col + rank) * p.up_v_row_stride + d, 4, p.up_v_vec);
+  const int stride = p.head_dim * 2 + 16, quads = p.head_dim >> 2;
+  uint8_t* up = smem + kGroups * q_bytes;
+#pragma unroll 4
+  for (int x = tid; x < rv * quads; x += kTileThreads) {
+    const int rank = x / quads, d = (x - rank * quads) * 4;
+    *reinterpret_cast<uint2*>(up + rank * stride + d * 2) = load_halves4(p.up_v + static_cast<int64_t>(H.v_col + rank) * p.up_v_row_stride + d, 4, p.up_v_vec);
   }
   __syncthreads();
-  if (warp >= kSoftmaxWarps || warp * 32 >= rows) return;
 #pragma unroll 1
-  for (int m = 0; m < 2; ++m) {
-    const int ra = warp * 32 + 16 * m + g, rb = ra + 8, la = ra & (kGroupRows - 1), lb = la + 8;
+  for (int w = warp; w * 16 < rows; w += kTileThreads / 32) {
+    const int ra = w * 16 + g, la = ra & (kGroupRows - 1), lb = la + 8;
     uint32_t a[8][4];
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
+    for (int q = 0; q < 8; ++q) {
+      const uint8_t* block = smem + (w >> 3) * q_bytes + (q >> 2) * kGroupRows * 128 + 4 * t;
+      const int c = 2 * (q & 3);
+      a[q][0] = a[q][1] = a[q][2] = a[q][3] = 0u;
       if (q < H.nv) {
-        const uint8_t* block = smem + (warp >> 2) * q_bytes + (q >> 2) * kGroupRows * 128;
-        const int c = 2 * (q & 3);
-        a[q][0] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c) + 4 * t);
-        a[q][1] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c) + 4 * t);
-        a[q][2] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c + 1) + 4 * t);
-        a[q][3] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c + 1) + 4 * t);
+        a[q][0] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c));
+        a[q][1] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c));
+        a[q][2] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c + 1));
+        a[q][3] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c + 1));
       }
-    for (int d0 = 0; d0 < p.head_dim; d0 += 8) {
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll 1
+    for (int d0 = 0; d0 < p.head_dim; d0 += 16) {      // 16 columns: two products a step, their B fragments by one transposing load
+      const bool both = d0 + 8 < p.head_dim;
+      const uint8_t* from = up + (lane & 15) * stride + (d0 + (both ? (lane >> 4) * 8 : 0)) * 2;
+      float y[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
-        if (q < H.nv) {
-          const uint16_t* at = reinterpret_cast<const uint16_t*>(up) + (16 * q + 2 * t) * p.head_dim + d0 + g;
-          const uint32_t b0 = at[0] | (static_cast<uint32_t>(at[p.head_dim]) << 16);
-          const uint32_t b1 = at[8 * p.head_dim] | (static_cast<uint32_t>(at[9 * p.head_dim]) << 16);
-          mma_f16_16x8x16(y, a[q][0], a[q][1], a[q][2], a[q][3], b0, b1);
-        }
+      for (int q = 0; q < 8; ++q) {
+        if (q >= H.nv) continue;
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, from + 16 * q * stride);
+        mma_f16_16x8x16(y[0], a[q][0], a[q][1], a[q][2], a[q][3], b[0], b[1]);
+        mma_f16_16x8x16(y[1], a[q][0], a[q][1], a[q][2], a[q][3], b[2], b[3]);
+      }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = e == 0 ? ra : rb;
-        if (row >= rows) continue;
-        __half* dst = p.out + static_cast<int64_t>(r.start + row0 + row) * p.out_stride_t + h * p.out_stride_h + d0 + 2 * t;
-        const uint32_t v = pack_half2(y[2 * e], y[2 * e + 1]);
+      for (int e = 0; e < 4; ++e) {
+        const int row = ra + 8 * (e & 1), d = d0 + 8 * (e >> 1) + 2 * t;
+        if (row >= rows || d >= p.head_dim) continue;
+        __half* dst = p.out + static_cast<int64_t>(r.start + row0 + row) * p.out_stride_t + h * p.out_stride_h + d;
+        const uint32_t v = pack_half2(y[e >> 1][2 * (e & 1)], y[e >> 1][2 * (e & 1) + 1]);
         if (p.out_vec2) {
           *reinterpret_cast<uint32_t*>(dst) = v;
         } else {
@@ -495,7 +512,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       copy_commit();
     }
     load_scales(0);
+    // the K up-factor is in the stages' place until every row is absorbed
     bool ok = true;
+    for (int i = 0; i < groups; ++i) ok = ok && tile_wait(s, &s.q_full[i], 0, p.status_word);
+    ok = __all_sync(0xffffffffu, ok);
     for (int j = 0; j < ntiles; ++j) {
       const int st = j & (stages - 1);
       copy_wait<kCodeStages - 2>();
@@ -549,7 +569,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     int E = -200;
     bool go = true;
     if (ntiles > 0) {
-      absorb_tile_rows(p, H, h, r, row0, rows, s, q_tile);
+      absorb_tile_rows(p, H, h, r, row0, rows, live_warps, s, q_tile, stage0);
       __syncwarp();
       f = s.scale[tid];
       f = fmaxf(f * p.score_scale * (kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e), 1e-37f);
