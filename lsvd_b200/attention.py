@@ -428,25 +428,18 @@ class LatentDecodeAttention(nn.Module):
         """A step with any number of new tokens per request (``state``: a ``ChunkState``): appends their latents ``[T, sum r]``
         at ``state.mem_index`` when they are given, then attends from ``q [T, H, D]``.  ``scores``: ``causal``, ``window``,
         ``b_prefix_len``, ``key_begin``, ``softcap``, ``alibi_slopes``, ``sm_scale`` as in ``chunk_attention_int8_latent_absorb``."""
-        from .chunk import attn_chunk_workspace_bytes, chunk_attention_int8_latent_absorb
+        from .chunk import chunk_attention_int8_latent_absorb, kept_workspace      # (chunk.py imports this file)
         if self.up_v is None and out is not None:
             raise ValueError("without up_v the result is out_latent")
         hm = self.layout.head_major
         if not hm:
             cache_k, cache_v = cache_k.view(cache_k.shape[0], -1), cache_v.view(cache_v.shape[0], -1)
         if latent_k is not None or latent_v is not None:
-            cache_append(self.layout, latent_k, latent_v, state.mem_index, cache_k, scale_k, cache_v, scale_v, rounding=self.rounding)
-        with torch.cuda.device(q.device):
-            need = attn_chunk_workspace_bytes(state, self.layout, q.shape[0])
-        kept = self._chunk_workspaces
-        if not kept or kept[-1].numel() < need or kept[-1].device != q.device:
-            # an outgrown workspace stays: a captured step may still point to it (each is twice the last, so all of them
-            # together are at most twice the largest)
-            size = max(need, 2 * kept[-1].numel() if kept and kept[-1].device == q.device else 0)
-            kept.append(torch.empty(size, dtype=torch.uint8, device=q.device))
+            cache_append(self.layout, latent_k, latent_v, state.mem_index[:q.shape[0]], cache_k, scale_k, cache_v, scale_v, rounding=self.rounding)
         return chunk_attention_int8_latent_absorb(
             q, state, self.layout.num_heads, self.head_dim, cache_k, scale_k, cache_v, scale_v, self.up_k, self.up_v,
-            layout=self.layout, out=out, out_latent=out_latent, workspace=kept[-1], **scores)
+            layout=self.layout, out=out, out_latent=out_latent,
+            workspace=kept_workspace(self._chunk_workspaces, state, self.layout, q.shape[0], q.device), **scores)
 
 
 @torch.no_grad()

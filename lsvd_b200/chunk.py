@@ -151,6 +151,17 @@ def attn_chunk_workspace_bytes(state, layout: LatentCacheLayout, num_tokens: int
                                                            int(state.max_new_in_batch), int(state.max_len_in_batch)))
 
 
+def kept_workspace(kept: list, state, layout: LatentCacheLayout, num_tokens: int, device) -> torch.Tensor:
+    """The workspace for a step out of ``kept``, which grows as steps need it.  An outgrown workspace stays there: a captured step
+    may still point to it (each is at least twice the last, so all of them together are at most twice the largest)."""
+    with torch.cuda.device(device):
+        need = max(attn_chunk_workspace_bytes(state, layout, num_tokens), 256)
+    last = kept[-1].numel() if kept and kept[-1].device == device else 0
+    if last < need:
+        kept.append(torch.empty(max(need, 2 * last), dtype=torch.uint8, device=device))
+    return kept[-1]
+
+
 def _row_view(name, t, rows, cols, dev):
     if t.dtype != torch.float16 or tuple(t.shape) != (rows, cols) or t.stride(-1) != 1 or t.device != dev:
         raise ValueError(f"{name} must be fp16 [{rows}, {cols}] with unit inner stride on {dev}")

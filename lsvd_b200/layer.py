@@ -25,6 +25,7 @@ from torch import nn
 
 from . import _lib
 from .attention import LatentCacheLayout, cache_append, token_decode_attention_int8_latent_absorb, attn_decode_workspace_bytes
+from .chunk import chunk_attention_int8_latent_absorb, kept_workspace
 from .ffn import HybridFFN, act_quant, w8a8_gemv, quantize_weight_rtn, i8gemm
 
 
@@ -40,6 +41,7 @@ class LSVDDecoderLayer(nn.Module):
         self.Rq = layout.num_heads * rank_q
         self._ws = None
         self._side = None
+        self._chunk_workspaces = []
 
     @torch.no_grad()
     def forward(self, x, cache_k, scale_k, cache_v, scale_v, infer_state, stages: Optional[dict] = None, out=None,
@@ -88,7 +90,7 @@ def _layer_prefill(self, x, cache_k, scale_k, cache_v, scale_v, dest_slots, stag
     kernels/layer_bench/fd_kernel/): between the cache write and the output projection this step lets every token attend
     to ITSELF only, i.e. the attention output is the token's own (fp16) V latent.  Everything BASELINE config 5 names for
     the prefill -- the latent-projection, gate / up / down GEMMs and the cache write -- runs as in a real prefill; the
-    values that reach the decode steps differ from a causal-attention prefill, which this library does not have."""
+    values that reach the decode steps differ from a causal-attention prefill, which is ``forward_chunk``."""
     lay = self.layout
     xq, xs, xn = act_quant(x, want_rotated=True, norm_weight=self.ln1, norm_eps=1e-5)
     lat, _ = i8gemm(xq, xs, self.W_lat_q, self.W_lat_s)
@@ -105,6 +107,43 @@ def _layer_prefill(self, x, cache_k, scale_k, cache_v, scale_v, dest_slots, stag
 
 
 LSVDDecoderLayer.forward_prefill = torch.no_grad()(_layer_prefill)
+
+
+@torch.no_grad()
+def _layer_chunk(self, x, cache_k, scale_k, cache_v, scale_v, state, stages=None, out=None, **scores):
+    """The layer for a step with any number of new tokens per request: ``x [T, hidden]`` holds them request after request as
+    ``state`` (a ``ChunkState``) lays them out, in at most as many rows as the state has slots for.  Their latents go to the cache slots ``state.mem_index`` and every token attends
+    to what its request has cached and to the step's tokens before it: a prompt or a piece of one, drafted tokens to verify, or
+    one token (then the same as ``forward``).  ``scores``: ``causal``, ``window``, ``b_prefix_len``, ``key_begin``, ``softcap``
+    and ``alibi_slopes`` as in ``chunk_attention_int8_latent_absorb``.  Rows behind the last token hold no result.
+    The products take the decode kernels up to 64 tokens and the tcgen05 GEMM beyond, as the FFN does."""
+    lay, T = self.layout, x.shape[0]
+    few = T <= 64
+
+    def product(q, s, w, ws, residual=None):
+        if few:
+            return w8a8_gemv(q, s, w, ws, residual=residual, prefetch_weights=2)[0]
+        return i8gemm(q, s, w, ws, residual=residual)[0]
+
+    xq, xs, xn = act_quant(x, want_rotated=True, norm_weight=self.ln1, norm_eps=1e-5)
+    lat = product(xq, xs, self.W_lat_q, self.W_lat_s)
+    lk = lat[:, self.Rq:self.Rq + lay.sum_k]
+    lv = None if lay.shared_kv else lat[:, self.Rq + lay.sum_k:]
+    cache_append(lay, lk, lv, state.mem_index[:T], cache_k, scale_k, cache_v, scale_v)
+    o_lat = torch.zeros(T, lay.sum_v, dtype=torch.float16, device=x.device)      # (rows behind the last token are quantised too)
+    chunk_attention_int8_latent_absorb(lat[:, :self.Rq].unflatten(1, (lay.num_heads, self.rank_q)), state, lay.num_heads, self.rank_q,
+                                       cache_k, scale_k, cache_v, scale_v, self.C, None, layout=lay, out_latent=o_lat,
+                                       workspace=kept_workspace(self._chunk_workspaces, state, lay, T, x.device),
+                                       sm_scale=1.0 / math.sqrt(self.head_dim), **scores)
+    oq, os_, _ = act_quant(o_lat)
+    y1 = product(oq, os_, self.W_uvo_q, self.W_uvo_s, residual=xn)
+    out = self.ffn(y1, out=out, norm_weight=self.ln2, norm_eps=1e-6, residual=y1)
+    if stages is not None:
+        stages.update(xn=xn, lat=lat, o_lat=o_lat, y1=y1, out=out)
+    return out
+
+
+LSVDDecoderLayer.forward_chunk = _layer_chunk
 
 
 def make_layer_weights(hidden: int, num_heads: int, head_dim: int, rank_q: int, k_ranks, v_ranks, seed: int = 0, device=None,

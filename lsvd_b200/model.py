@@ -15,6 +15,7 @@ from torch import nn
 
 from . import synth
 from .attention import InferState, LatentCacheLayout, decode_advance
+from .chunk import ChunkState
 from .ffn import HybridFFN
 from .layer import LSVDDecoderLayer, TPDecoderLayer, make_layer_weights
 from .parallel import shard_layer
@@ -25,7 +26,8 @@ class LSVDModel(nn.Module):
 
     ``prefill(x, dest_slots)`` runs ``x [T, hidden]`` through every layer's prefill form (cache rows written at
     ``dest_slots``); ``decode_step(x, state)`` runs one token per request through every layer (each layer appends to its
-    own cache at ``state.mem_index`` and attends over ``state.b_seq_len`` tokens) and returns the last hidden state.
+    own cache at ``state.mem_index`` and attends over ``state.b_seq_len`` tokens) and returns the last hidden state;
+    ``chunk_step(x, state)`` is the form for any number of tokens per request, with attention among them.
     """
 
     def __init__(self, n_layers: int, hidden: int, num_heads: int, head_dim: int, d_ffn: int, rank_q: int, k_ranks, v_ranks,
@@ -47,11 +49,23 @@ class LSVDModel(nn.Module):
             layers.append(LSVDDecoderLayer(self.layout, head_dim, rank_q, to(lw), HybridFFN(to(fw))))
             self.caches.append(self.layout.alloc(num_slots, device))
         self.layers = nn.ModuleList(layers)
+        for layer in layers[1:]:           # the layers of a step run one after another: one attention workspace serves all
+            layer._chunk_workspaces = layers[0]._chunk_workspaces
 
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, dest_slots: torch.Tensor) -> torch.Tensor:
         for layer, (ck, sk, cv, sv) in zip(self.layers, self.caches):
             x = layer.forward_prefill(x, ck, sk, cv, sv, dest_slots)
+        return x
+
+    @torch.no_grad()
+    def chunk_step(self, x: torch.Tensor, state: ChunkState, **scores) -> torch.Tensor:
+        """A step with any number of new tokens per request through every layer (``LSVDDecoderLayer.forward_chunk``): whole
+        prompts, pieces of them beside requests that decode, drafted tokens.  ``x [T, hidden]`` holds the tokens as ``state``
+        lays them out (``ChunkState.begin`` takes their slots); each layer writes its own cache there.  ``scores`` are the score
+        options of ``chunk_attention_int8_latent_absorb``."""
+        for layer, (ck, sk, cv, sv) in zip(self.layers, self.caches):
+            x = layer.forward_chunk(x, ck, sk, cv, sv, state, **scores)
         return x
 
     @torch.no_grad()
