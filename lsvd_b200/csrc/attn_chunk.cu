@@ -626,7 +626,8 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   if (a->up_k_row_stride < a->head_dim || (a->out != nullptr && a->up_v_row_stride < a->head_dim)) return LSVD_ERR_INVALID_ARG;
   if (a->req_to_token_rows <= 0 || (a->req_to_token_rows > 1 && a->req_to_token_stride < a->max_len_in_batch)) return LSVD_ERR_INVALID_ARG;
   if (a->max_len_in_batch > (1 << 30)) return LSVD_ERR_UNSUPPORTED;
-  if (std::isnan(a->softcap) || std::isinf(a->softcap)) return LSVD_ERR_INVALID_ARG;
+  if (!std::isfinite(a->softcap) || !std::isfinite(a->sm_scale) || a->softcap < 0.f || a->window < 0) return LSVD_ERR_INVALID_ARG;
+  if (a->softcap > 0.f && a->softcap < 1e-6f) return LSVD_ERR_UNSUPPORTED;      // (the scores' factor 1 / softcap has to stay in range)
   const ChunkPlan c = chunk_plan(a->batch, a->num_heads, a->num_tokens, a->max_new_in_batch, a->max_len_in_batch);
   if (a->batch > 65535 || c.tiles > 65535 || (a->num_tokens + kMergeRows - 1) / kMergeRows > 65535) return LSVD_ERR_UNSUPPORTED;
   const bool stream_partials = c.stream && (c.stream_splits > 1 || a->out != nullptr);
