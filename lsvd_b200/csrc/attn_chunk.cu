@@ -42,6 +42,12 @@ struct __align__(16) ChunkShared {
   int32_t lo[kStreamRows], hi[kStreamRows];
 };
 
+// One product of the stream form.  With at most eight rows (kFew) the lower half of A is zero.
+template <bool kFew>
+__device__ __forceinline__ void mma_rows(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  mma_f16_16x8x16(d, a0, a1, a2, a3, b0, b1);
+}
+
 // q~ of up to 16 rows into shared memory, by all warps of the block: warp w takes the 8-rank tiles w, w + 4, ...
 // (mma lane (g, t): rows g and g + 8, k = halves 4t .. 4t + 3 of a 16-wide step, ranks 8 j + g).
 __device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int rows,
@@ -71,7 +77,7 @@ __device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHea
 }
 
 // grid: (heads, batch, splits)
-template <bool kCap, bool kBias>
+template <bool kCap, bool kBias, bool kFew>
 __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __grid_constant__ ChunkParams p) {
   extern __shared__ __align__(16) uint8_t ring_mem[];
   __shared__ ChunkShared s;
@@ -81,7 +87,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   const int h = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
   const ChunkRequest r = chunk_request(p, b, h == 0 && split == 0 && threadIdx.x == 0);
   const int rows = r.n;
-  if (rows <= 0 || rows > kStreamRows) return;      // none, or the tile form's
+  if (rows <= 0 || rows > (kFew ? 8 : kStreamRows)) return;      // none, or the tile form's
   const ChunkHead H = p.head[h];
   const int rk = H.nk * 16, rv = H.nv * 16;
 
@@ -116,7 +122,8 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   const int32_t* r2t = p.req_to_token + static_cast<int64_t>(r.req) * p.req_to_token_stride;
   const int8_t* kbase = p.cache_k + (p.head_major ? static_cast<int64_t>(H.k_col) * p.num_slots : H.k_col);
   const int8_t* vbase = p.cache_v + (p.head_major ? static_cast<int64_t>(H.v_col) * p.num_slots : H.v_col);
-  const int64_t kstride = p.head_major ? rk : p.cache_k_row_stride, vstride = p.head_major ? rv : p.cache_v_row_stride;
+  const uint32_t kstride = static_cast<uint32_t>(p.head_major ? rk : p.cache_k_row_stride);      // (the host has checked the strides)
+  const uint32_t vstride = static_cast<uint32_t>(p.head_major ? rv : p.cache_v_row_stride);
   const __half* ksc = p.scale_k + (p.head_major ? static_cast<int64_t>(h) * p.num_slots : h);
   const __half* vsc = p.scale_v + (p.head_major ? static_cast<int64_t>(h) * p.num_slots : h);
   const int64_t kss = p.head_major ? 1 : p.scale_k_row_stride, vss = p.head_major ? 1 : p.scale_v_row_stride;
@@ -147,12 +154,12 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       const int tok = (x * inv_k) >> 16, piece = x - tok * H.nk;
       const int sl = __shfl_sync(0xffffffffu, slot, tok);
       const int row = k_row_of(tok);
-      copy16_or_zero(kd + row * rk + k_piece_at(row, piece, H.nk) * 16, kbase + static_cast<int64_t>(max(sl, 0)) * kstride + piece * 16, sl >= 0);
+      copy16_or_zero(kd + row * rk + k_piece_at(row, piece, H.nk) * 16, kbase + static_cast<uint64_t>(static_cast<uint32_t>(max(sl, 0))) * kstride + piece * 16, sl >= 0);
     }
     for (int x = lane; x < 32 * H.nv; x += 32) {
       const int tok = (x * inv_v) >> 16, piece = x - tok * H.nv;
       const int sl = __shfl_sync(0xffffffffu, slot, tok);
-      copy16_or_zero(vd + tok * rv + v_piece_at(tok, piece, H.nv) * 16, vbase + static_cast<int64_t>(max(sl, 0)) * vstride + piece * 16, sl >= 0);
+      copy16_or_zero(vd + tok * rv + v_piece_at(tok, piece, H.nv) * 16, vbase + static_cast<uint64_t>(static_cast<uint32_t>(max(sl, 0))) * vstride + piece * 16, sl >= 0);
     }
   };
   // (kept as loaded until the tile is in hand: a conversion here would wait for the load)
@@ -210,9 +217,13 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
         if (rank < rk) {
           const float4 x = *reinterpret_cast<const float4*>(qt_a + rank), y = *reinterpret_cast<const float4*>(qt_b + rank);
           qa[mb][i][0] = pack_half2(x.x * xa, x.y * xa);
-          qa[mb][i][1] = pack_half2(y.x * xb, y.y * xb);
           qa[mb][i][2] = pack_half2(x.z * xa, x.w * xa);
-          qa[mb][i][3] = pack_half2(y.z * xb, y.w * xb);
+          if (kFew) {             // (each a register of its own: the product takes A from four neighbouring ones)
+            asm volatile("" : "+r"(qa[mb][i][1]), "+r"(qa[mb][i][3]));
+          } else {
+            qa[mb][i][1] = pack_half2(y.x * xb, y.y * xb);
+            qa[mb][i][3] = pack_half2(y.z * xb, y.w * xb);
+          }
         }
       }
   }
@@ -281,13 +292,13 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
           }
           uint32_t b0, b1;
           codes_to_half(w.x, b0, b1);
-          mma_f16_16x8x16(x[j], qa[mb][0][0], qa[mb][0][1], qa[mb][0][2], qa[mb][0][3], b0, b1);
+          mma_rows<kFew>(x[j], qa[mb][0][0], qa[mb][0][1], qa[mb][0][2], qa[mb][0][3], b0, b1);
           codes_to_half(w.y, b0, b1);
-          mma_f16_16x8x16(x[j], qa[mb][1][0], qa[mb][1][1], qa[mb][1][2], qa[mb][1][3], b0, b1);
+          mma_rows<kFew>(x[j], qa[mb][1][0], qa[mb][1][1], qa[mb][1][2], qa[mb][1][3], b0, b1);
           codes_to_half(w.z, b0, b1);
-          mma_f16_16x8x16(x[j], qa[mb][2][0], qa[mb][2][1], qa[mb][2][2], qa[mb][2][3], b0, b1);
+          mma_rows<kFew>(x[j], qa[mb][2][0], qa[mb][2][1], qa[mb][2][2], qa[mb][2][3], b0, b1);
           codes_to_half(w.w, b0, b1);
-          mma_f16_16x8x16(x[j], qa[mb][3][0], qa[mb][3][1], qa[mb][3][2], qa[mb][3][3], b0, b1);
+          mma_rows<kFew>(x[j], qa[mb][3][0], qa[mb][3][1], qa[mb][3][2], qa[mb][3][3], b0, b1);
         }
       }
     }
@@ -300,30 +311,34 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       for (int e = 0; e < 2; ++e) {
         const int k = 8 * j + t4 + 4 * e;
         const float c = s.sk[warp][k];
-        float xa = x[j][e] * (c * fa), xb = x[j][2 + e] * (c * fb);
+        float xa = x[j][e] * (c * fa), xb = kFew ? 0.f : x[j][2 + e] * (c * fb);
         if (kCap) {
           xa = capped_log2(xa, cap_log2e);
-          xb = capped_log2(xb, cap_log2e);
+          if (!kFew) xb = capped_log2(xb, cap_log2e);
         }
         if (kBias) {
           xa -= slope * fabsf(static_cast<float>(pos_a - key0 - k));
-          xb -= slope * fabsf(static_cast<float>(pos_b - key0 - k));
+          if (!kFew) xb -= slope * fabsf(static_cast<float>(pos_b - key0 - k));
         }
         if (masked) {
           const bool live = (valid >> k) & 1u;
           if (!live || key0 + k < lo_a || key0 + k >= hi_a) xa = -INFINITY;
-          if (!live || key0 + k < lo_b || key0 + k >= hi_b) xb = -INFINITY;
+          if (!kFew && (!live || key0 + k < lo_b || key0 + k >= hi_b)) xb = -INFINITY;
         }
         x[j][e] = xa;
-        x[j][2 + e] = xb;
         top_a = fmaxf(top_a, xa);
-        top_b = fmaxf(top_b, xb);
+        if (!kFew) {
+          x[j][2 + e] = xb;
+          top_b = fmaxf(top_b, xb);
+        }
       }
     }
     top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, 1));
     top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, 2));
-    top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 1));
-    top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 2));
+    if (!kFew) {
+      top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 1));
+      top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 2));
+    }
     const float n_a = fmaxf(m_a, top_a), n_b = fmaxf(m_b, top_b);
     const float base_a = n_a == -INFINITY ? 0.f : n_a, base_b = n_b == -INFINITY ? 0.f : n_b;
     if (__any_sync(0xffffffffu, n_a != m_a || n_b != m_b || e_new != E)) {
@@ -338,8 +353,10 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
         for (int j = 0; j < 8; ++j) {
           o[vb][j][0] *= s_a;
           o[vb][j][1] *= s_a;
-          o[vb][j][2] *= s_b;
-          o[vb][j][3] *= s_b;
+          if (!kFew) {
+            o[vb][j][2] *= s_b;
+            o[vb][j][3] *= s_b;
+          }
         }
       m_a = n_a;
       m_b = n_b;
@@ -348,16 +365,20 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     uint32_t w[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float p0 = ex2(x[j][0] - base_a), p1 = ex2(x[j][1] - base_a), p2 = ex2(x[j][2] - base_b), p3 = ex2(x[j][3] - base_b);
+      const float p0 = ex2(x[j][0] - base_a), p1 = ex2(x[j][1] - base_a);
       l_a += p0 + p1;
-      l_b += p2 + p3;
       const float v0 = s.sv[warp][8 * j + t4], v1 = s.sv[warp][8 * j + t4 + 4];
       // a masked key's weight is zero whatever its scale holds
       w[j][0] = pack_half2(p0 == 0.f ? 0.f : p0 * v0, p1 == 0.f ? 0.f : p1 * v1);
-      w[j][1] = pack_half2(p2 == 0.f ? 0.f : p2 * v0, p3 == 0.f ? 0.f : p3 * v1);
+      w[j][1] = 0u;
+      if (!kFew) {
+        const float p2 = ex2(x[j][2] - base_b), p3 = ex2(x[j][3] - base_b);
+        l_b += p2 + p3;
+        w[j][1] = pack_half2(p2 == 0.f ? 0.f : p2 * v0, p3 == 0.f ? 0.f : p3 * v1);
+      }
     }
     // values: rank 64 vb + 8 g + n of lane (g, t) is column g of tile n; the keys of step m are the score columns' keys
-#pragma unroll
+#pragma unroll 1
     for (int m = 0; m < 2; ++m) {
 #pragma unroll
       for (int vb = 0; vb < 2; ++vb) {
@@ -381,11 +402,15 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
             uint32_t b0, b1, c0, c1;
             codes_to_half(u, b0, c0);         // {key t, key t + 4} of the first rank, of the second
             codes_to_half(v, b1, c1);         // {key t + 8, key t + 12}
-            mma_f16_16x8x16(o[vb][2 * q], w[2 * m][0], w[2 * m][1], w[2 * m + 1][0], w[2 * m + 1][1], b0, b1);
-            mma_f16_16x8x16(o[vb][2 * q + 1], w[2 * m][0], w[2 * m][1], w[2 * m + 1][0], w[2 * m + 1][1], c0, c1);
+            mma_rows<kFew>(o[vb][2 * q], w[0][0], w[0][1], w[1][0], w[1][1], b0, b1);
+            mma_rows<kFew>(o[vb][2 * q + 1], w[0][0], w[0][1], w[1][0], w[1][1], c0, c1);
           }
         }
       }
+      w[0][0] = w[2][0];
+      w[0][1] = w[2][1];
+      w[1][0] = w[3][0];
+      w[1][1] = w[3][1];
     }
   }
   copy_wait<0>();
@@ -421,6 +446,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
         float4* db = reinterpret_cast<float4*>(sums + (g + 8) * LSVD_MAX_RANK + rank);
         da[0] = make_float4(o[vb][0][e] * s_a, o[vb][1][e] * s_a, o[vb][2][e] * s_a, o[vb][3][e] * s_a);
         da[1] = make_float4(o[vb][4][e] * s_a, o[vb][5][e] * s_a, o[vb][6][e] * s_a, o[vb][7][e] * s_a);
+        if (kFew) continue;
         db[0] = make_float4(o[vb][0][2 + e] * s_b, o[vb][1][2 + e] * s_b, o[vb][2][2 + e] * s_b, o[vb][3][2 + e] * s_b);
         db[1] = make_float4(o[vb][4][2 + e] * s_b, o[vb][5][2 + e] * s_b, o[vb][6][2 + e] * s_b, o[vb][7][2 + e] * s_b);
       }
@@ -551,7 +577,7 @@ static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_ne
   c.stream = !c.tile || batch > 1;
   c.tile_min = c.stream ? kStreamRows : 0;
   c.stream_stride = std::min(kStreamRows, longest);
-  chunk_split(static_cast<int64_t>(num_heads) * batch, 6 * 3 * sms, 256, 128, max_len, &c.stream_splits, &c.stream_split_len);
+  chunk_split(static_cast<int64_t>(num_heads) * batch, 4 * 3 * sms, 256, 128, max_len, &c.stream_splits, &c.stream_split_len);
   const int64_t of_tokens = num_tokens / kChunkTileRows + std::min<int64_t>(batch, num_tokens / (c.tile_min + 1));
   const int64_t of_requests = static_cast<int64_t>(batch) * ((longest + kChunkTileRows - 1) / kChunkTileRows);
   c.tiles = static_cast<int>(std::max<int64_t>(1, std::min(of_tokens, of_requests)));
@@ -699,8 +725,14 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (c.stream) {
     const bool cap = a->softcap > 0.f, bias = a->alibi_slopes != nullptr;
-    void (*kern)(ChunkParams) = cap ? (bias ? chunk_stream_kernel<true, true> : chunk_stream_kernel<true, false>)
-                                    : (bias ? chunk_stream_kernel<false, true> : chunk_stream_kernel<false, false>);
+    void (*kern)(ChunkParams) = nullptr;
+    if (c.stream_stride <= 8) {             // (no request has more rows)
+      kern = cap ? (bias ? chunk_stream_kernel<true, true, true> : chunk_stream_kernel<true, false, true>)
+                 : (bias ? chunk_stream_kernel<false, true, true> : chunk_stream_kernel<false, false, true>);
+    } else {
+      kern = cap ? (bias ? chunk_stream_kernel<true, true, false> : chunk_stream_kernel<true, false, false>)
+                 : (bias ? chunk_stream_kernel<false, true, false> : chunk_stream_kernel<false, false, false>);
+    }
     const int smem = kChunkWarps * kRingBytes;
     LSVD_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem));
     LSVD_CUDA_TRY(launch_chained(kern, dim3(a->num_heads, a->batch, c.stream_splits), dim3(kChunkThreads), smem, st, 1, true, p));
