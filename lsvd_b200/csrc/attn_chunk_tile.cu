@@ -28,7 +28,7 @@ constexpr int kGroups = 2;
 constexpr int kTileRows = kChunkTileRows;
 static_assert(kTileRows == kGroups * kGroupRows, "two products' rows");
 constexpr int kTileKeys = 64;
-constexpr int kSoftmaxWarps = 4 * kGroups, kLoadWarps = 3;
+constexpr int kSoftmaxWarps = 4 * kGroups, kLoadWarps = 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
 constexpr int kTileThreads = (kMmaWarp + 1) * 32;
 constexpr int kLoadThreads = kLoadWarps * 32;
