@@ -153,7 +153,9 @@ def attn_chunk_workspace_bytes(state, layout: LatentCacheLayout, num_tokens: int
 
 def kept_workspace(kept: list, state, layout: LatentCacheLayout, num_tokens: int, device) -> torch.Tensor:
     """The workspace for a step out of ``kept``, which grows as steps need it.  An outgrown workspace stays there: a captured step
-    may still point to it (each is at least twice the last, so all of them together are at most twice the largest)."""
+    may still point to it (each is at least twice the last, so all of them together are at most twice the largest).
+    Steps that take their workspace from one list run one after another, captured or not; for steps side by side on two streams
+    give each its own ``workspace``."""
     with torch.cuda.device(device):
         need = max(attn_chunk_workspace_bytes(state, layout, num_tokens), 256)
     last = kept[-1].numel() if kept and kept[-1].device == device else 0

@@ -4,16 +4,22 @@
 // latents with q~, and the values stay in the latent space until the end:
 //   x_t = sm_scale scale_k[t] (z_k[t] . q~) [capped, biased],  o_lat = sum_t softmax(x)_t scale_v[t] z_v[t],  o = B_v^T o_lat.
 //
-// Stream form (up to 16 query rows of a request share one pass over its cache): a block owns (request, head, 16 query rows,
+// Stream form (up to 8 query rows of a request share one pass over its cache): a block owns (request, head, the rows,
 // split of the keys); each of its four warps walks its own 32-key tiles.  The rows arrive by 16-byte asynchronous copies in
 // a ring of shared memory per warp (gathered slot by slot: any page table, both cache layouts); codes become fp16 exactly
 // (|code| <= 128) and meet q~ and the weights on the tensor cores (mma m16n8k16, fp32 accumulators).  With few rows the bytes
-// of the cache bound it: r_k + r_v + 4 bytes per key and head.
+// of the cache would bound it, r_k + r_v + 4 bytes per key and head; what does is the instruction stream of a tile (widening,
+// two products of 16-row fragments that few rows fill, softmax) at twelve warps an SM.  Measured: 16 single tokens over 4096 keys, 32
+// heads, mean ranks 64 + 64: 201 us (268 MB, 1.3 TB/s); five tokens of eight requests 139 us.  Softmax for the lower
+// half of the fragments as well (requests of 9 to 16 rows in this form) cost 230 against 215 us; the value loop is rolled for
+// the instruction cache (215 -> 201 us).
 //
-// Roundings.  q~ is kept in fp16 relative to its row's largest entry (a power of two taken out, so no entry overflows and
-// small ones keep their bits down to 2^-23 of the largest), the weights p * scale_v in fp16 relative to the largest V scale
-// seen: 2^-11 of each term, the size of the rounding of the fp16 result.  Maxima, sums and accumulators are fp32.  Scales are
-// applied in fp32 to scores and weights, never to the codes: a masked key's scale, were it infinite or NaN, touches nothing.
+// Roundings.  q~ enters the products as two fp16 numbers, what fp16 keeps of it and the rest, relative to its row's largest entry (a
+// power of two taken out, so no entry overflows and small ones keep their bits down to 2^-23 of the largest).  The weights
+// p * scale_v are fp16 relative to the largest V scale seen: 2^-11 of each term, the size of the rounding of the fp16 result, in the
+// tile form; the stream form carries their rest too, in the half of the fragment that its few rows leave free.  Maxima, sums and
+// accumulators are fp32.  Scales are applied in fp32 to scores and weights, never to the codes: a masked key's scale, were it
+// infinite or NaN, touches nothing.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -42,42 +48,33 @@ struct __align__(16) ChunkShared {
   int32_t lo[kStreamRows], hi[kStreamRows];
 };
 
-// One product of the stream form.  With at most eight rows (kFew) the lower half of A is zero.
-template <bool kFew>
-__device__ __forceinline__ void mma_rows(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  mma_f16_16x8x16(d, a0, a1, a2, a3, b0, b1);
-}
-
-// q~ of up to 16 rows into shared memory, by all warps of the block: warp w takes the 8-rank tiles w, w + 4, ...
-// (mma lane (g, t): rows g and g + 8, k = halves 4t .. 4t + 3 of a 16-wide step, ranks 8 j + g).
+// q~ of up to 8 rows into shared memory, by all warps of the block: warp w takes the 8-rank tiles w, w + 4, ...
+// (mma lane (g, t): row g, rows 8 .. 15 zero, k = halves 4t .. 4t + 3 of a 16-wide step, ranks 8 j + g).
 __device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int rows,
                                             uint8_t* ring_mem) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const __half* qa = p.q + static_cast<int64_t>(r.start + min(g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
-  const __half* qb = p.q + static_cast<int64_t>(r.start + min(g + 8, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
   const int tiles = H.nk * 2;
   for (int j = warp; j < tiles; j += kChunkWarps) {
     const __half* up = p.up_k + static_cast<int64_t>(H.k_col + j * 8 + g) * p.up_k_row_stride;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int d0 = 0; d0 < p.head_dim; d0 += 64) {
-      uint2 a0[4], a1[4], b[4];
+      uint2 a0[4], b[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = d0 + 16 * i + 4 * t;
         a0[i] = load_halves4(qa + d, p.head_dim - d, p.q_vec);
-        a1[i] = load_halves4(qb + d, p.head_dim - d, p.q_vec);
         b[i] = load_halves4(up + d, p.head_dim - d, p.up_k_vec);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mma_f16_16x8x16(acc, a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
+      for (int i = 0; i < 4; ++i) mma_f16_16x8x16(acc, a0[i].x, 0u, a0[i].y, 0u, b[i].x, b[i].y);
     }
     *reinterpret_cast<float2*>(absorbed_row(ring_mem, g) + j * 8 + 2 * t) = make_float2(acc[0], acc[1]);
-    *reinterpret_cast<float2*>(absorbed_row(ring_mem, g + 8) + j * 8 + 2 * t) = make_float2(acc[2], acc[3]);
   }
 }
 
 // grid: (heads, batch, splits)
-template <bool kCap, bool kBias, bool kFew>
+template <bool kCap, bool kBias>
 __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __grid_constant__ ChunkParams p) {
   extern __shared__ __align__(16) uint8_t ring_mem[];
   __shared__ ChunkShared s;
@@ -87,7 +84,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   const int h = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
   const ChunkRequest r = chunk_request(p, b, h == 0 && split == 0 && threadIdx.x == 0);
   const int rows = r.n;
-  if (rows <= 0 || rows > (kFew ? 8 : kStreamRows)) return;      // none, or the tile form's
+  if (rows <= 0 || rows > kStreamRows) return;      // none, or the tile form's
   const ChunkHead H = p.head[h];
   const int rk = H.nk * 16, rv = H.nv * 16;
 
@@ -183,31 +180,28 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
 
   absorb_rows(p, H, h, r, rows, ring_mem);
   __syncthreads();
-  const float *qt_a = absorbed_row(ring_mem, g), *qt_b = absorbed_row(ring_mem, g + 8);
-  // q~ as fp16 A fragments: step (mb, i) of a 64-rank block holds ranks 64 mb + 16 t + 4 i .. + 3 of lane (g, t)
+  const float* qt = absorbed_row(ring_mem, g);
+  // q~ as fp16 A fragments: step (mb, i) of a 64-rank block holds ranks 64 mb + 16 t + 4 i .. + 3 of lane (g, t).  Row g is what
+  // fp16 keeps of q~, row g + 8 of the fragment the rest, so that the products see 22 bits of it at no further cost.
   uint32_t qa[2][4][4];
-  float fa, fb;                       // score scale of rows g and g + 8, with the power of two that was taken out
+  float f;                            // score scale of the row, with the power of two that was taken out
   {
-    float ma = 0.f, mb_ = 0.f;
+    float big = 0.f;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int rank = 64 * mb + 16 * t4 + 4 * i;
         if (rank < rk) {
-          const float4 x = *reinterpret_cast<const float4*>(qt_a + rank), y = *reinterpret_cast<const float4*>(qt_b + rank);
-          ma = fmaxf(ma, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-          mb_ = fmaxf(mb_, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+          const float4 x = *reinterpret_cast<const float4*>(qt + rank);
+          big = fmaxf(big, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
         }
       }
-    ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
-    ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, 2));
-    mb_ = fmaxf(mb_, __shfl_xor_sync(0xffffffffu, mb_, 1));
-    mb_ = fmaxf(mb_, __shfl_xor_sync(0xffffffffu, mb_, 2));
-    const int ea = exponent_of(ma) - 8, eb = exponent_of(mb_) - 8;       // entries end up below 2^9
-    const float xa = pow2i(-ea), xb = pow2i(-eb);
-    fa = p.score_scale * pow2i(ea);
-    fb = p.score_scale * pow2i(eb);
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const int ex = exponent_of(big) - 8;                                 // entries end up below 2^9
+    const float by = pow2i(-ex);
+    f = p.score_scale * pow2i(ex);
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -215,32 +209,19 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
         const int rank = 64 * mb + 16 * t4 + 4 * i;
         qa[mb][i][0] = qa[mb][i][1] = qa[mb][i][2] = qa[mb][i][3] = 0u;
         if (rank < rk) {
-          const float4 x = *reinterpret_cast<const float4*>(qt_a + rank), y = *reinterpret_cast<const float4*>(qt_b + rank);
-          qa[mb][i][0] = pack_half2(x.x * xa, x.y * xa);
-          qa[mb][i][2] = pack_half2(x.z * xa, x.w * xa);
-          if (kFew) {             // (each a register of its own: the product takes A from four neighbouring ones)
-            asm volatile("" : "+r"(qa[mb][i][1]), "+r"(qa[mb][i][3]));
-          } else {
-            qa[mb][i][1] = pack_half2(y.x * xb, y.y * xb);
-            qa[mb][i][3] = pack_half2(y.z * xb, y.w * xb);
-          }
+          const float4 x = *reinterpret_cast<const float4*>(qt + rank);
+          pack_half2_rest(x.x * by, x.y * by, qa[mb][i][0], qa[mb][i][1]);
+          pack_half2_rest(x.z * by, x.w * by, qa[mb][i][2], qa[mb][i][3]);
         }
       }
   }
   __syncthreads();                    // the rings' last stages may be written from here on
   const float cap_log2e = p.softcap * kChunkLog2e;
-  if (kCap) {
-    fa *= 2.f * kChunkLog2e / p.softcap;
-    fb *= 2.f * kChunkLog2e / p.softcap;
-  } else {
-    fa *= kChunkLog2e;
-    fb *= kChunkLog2e;
-  }
-  const int lo_a = s.lo[g], hi_a = s.hi[g], lo_b = s.lo[g + 8], hi_b = s.hi[g + 8];
-  const int pos_a = r.len - r.n + g, pos_b = pos_a + 8;
+  f *= kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e;
+  const int lo = s.lo[g], hi = s.hi[g], pos = r.len - r.n + g;
   const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
 
-  float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+  float m = -INFINITY, l = 0.f;
   int E = -200;                       // exponent of the largest V scale so far
   float o[2][8][4];
 #pragma unroll
@@ -292,90 +273,60 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
           }
           uint32_t b0, b1;
           codes_to_half(w.x, b0, b1);
-          mma_rows<kFew>(x[j], qa[mb][0][0], qa[mb][0][1], qa[mb][0][2], qa[mb][0][3], b0, b1);
+          mma_f16_16x8x16(x[j], qa[mb][0][0], qa[mb][0][1], qa[mb][0][2], qa[mb][0][3], b0, b1);
           codes_to_half(w.y, b0, b1);
-          mma_rows<kFew>(x[j], qa[mb][1][0], qa[mb][1][1], qa[mb][1][2], qa[mb][1][3], b0, b1);
+          mma_f16_16x8x16(x[j], qa[mb][1][0], qa[mb][1][1], qa[mb][1][2], qa[mb][1][3], b0, b1);
           codes_to_half(w.z, b0, b1);
-          mma_rows<kFew>(x[j], qa[mb][2][0], qa[mb][2][1], qa[mb][2][2], qa[mb][2][3], b0, b1);
+          mma_f16_16x8x16(x[j], qa[mb][2][0], qa[mb][2][1], qa[mb][2][2], qa[mb][2][3], b0, b1);
           codes_to_half(w.w, b0, b1);
-          mma_rows<kFew>(x[j], qa[mb][3][0], qa[mb][3][1], qa[mb][3][2], qa[mb][3][3], b0, b1);
+          mma_f16_16x8x16(x[j], qa[mb][3][0], qa[mb][3][1], qa[mb][3][2], qa[mb][3][3], b0, b1);
         }
       }
     }
     const int key0 = kbeg + (warp + i * kChunkWarps) * 32;
     const bool masked = key0 < inner_lo || key0 + 32 > inner_hi || valid != 0xffffffffu;
-    float top_a = -INFINITY, top_b = -INFINITY;
+    float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int k = 8 * j + t4 + 4 * e;
         const float c = s.sk[warp][k];
-        float xa = x[j][e] * (c * fa), xb = kFew ? 0.f : x[j][2 + e] * (c * fb);
-        if (kCap) {
-          xa = capped_log2(xa, cap_log2e);
-          if (!kFew) xb = capped_log2(xb, cap_log2e);
-        }
-        if (kBias) {
-          xa -= slope * fabsf(static_cast<float>(pos_a - key0 - k));
-          if (!kFew) xb -= slope * fabsf(static_cast<float>(pos_b - key0 - k));
-        }
-        if (masked) {
-          const bool live = (valid >> k) & 1u;
-          if (!live || key0 + k < lo_a || key0 + k >= hi_a) xa = -INFINITY;
-          if (!kFew && (!live || key0 + k < lo_b || key0 + k >= hi_b)) xb = -INFINITY;
-        }
-        x[j][e] = xa;
-        top_a = fmaxf(top_a, xa);
-        if (!kFew) {
-          x[j][2 + e] = xb;
-          top_b = fmaxf(top_b, xb);
-        }
+        float v = (x[j][e] + x[j][2 + e]) * (c * f);
+        if (kCap) v = capped_log2(v, cap_log2e);
+        if (kBias) v -= slope * fabsf(static_cast<float>(pos - key0 - k));
+        if (masked && (!((valid >> k) & 1u) || key0 + k < lo || key0 + k >= hi)) v = -INFINITY;
+        x[j][e] = v;
+        top = fmaxf(top, v);
       }
     }
-    top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, 1));
-    top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, 2));
-    if (!kFew) {
-      top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 1));
-      top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 2));
-    }
-    const float n_a = fmaxf(m_a, top_a), n_b = fmaxf(m_b, top_b);
-    const float base_a = n_a == -INFINITY ? 0.f : n_a, base_b = n_b == -INFINITY ? 0.f : n_b;
-    if (__any_sync(0xffffffffu, n_a != m_a || n_b != m_b || e_new != E)) {
-      const float c_a = ex2(m_a - base_a), c_b = ex2(m_b - base_b);       // a first maximum: 2^-inf = 0
-      l_a *= c_a;
-      l_b *= c_b;
-      const float shift = pow2i(max(E - e_new, -126));
-      const float s_a = c_a * shift, s_b = c_b * shift;
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
+    if (__any_sync(0xffffffffu, m_new != m || e_new != E)) {
+      const float c = ex2(m - base);       // a first maximum: 2^-inf = 0
+      l *= c;
+      const float by = c * pow2i(max(E - e_new, -126));
 #pragma unroll
       for (int vb = 0; vb < 2; ++vb)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          o[vb][j][0] *= s_a;
-          o[vb][j][1] *= s_a;
-          if (!kFew) {
-            o[vb][j][2] *= s_b;
-            o[vb][j][3] *= s_b;
-          }
+          o[vb][j][0] *= by;
+          o[vb][j][1] *= by;
+          o[vb][j][2] *= by;
+          o[vb][j][3] *= by;
         }
-      m_a = n_a;
-      m_b = n_b;
+      m = m_new;
       E = e_new;
     }
     uint32_t w[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float p0 = ex2(x[j][0] - base_a), p1 = ex2(x[j][1] - base_a);
-      l_a += p0 + p1;
+      const float p0 = ex2(x[j][0] - base), p1 = ex2(x[j][1] - base);
+      l += p0 + p1;
       const float v0 = s.sv[warp][8 * j + t4], v1 = s.sv[warp][8 * j + t4 + 4];
-      // a masked key's weight is zero whatever its scale holds
-      w[j][0] = pack_half2(p0 == 0.f ? 0.f : p0 * v0, p1 == 0.f ? 0.f : p1 * v1);
-      w[j][1] = 0u;
-      if (!kFew) {
-        const float p2 = ex2(x[j][2] - base_b), p3 = ex2(x[j][3] - base_b);
-        l_b += p2 + p3;
-        w[j][1] = pack_half2(p2 == 0.f ? 0.f : p2 * v0, p3 == 0.f ? 0.f : p3 * v1);
-      }
+      // a masked key's weight is zero whatever its scale holds; what fp16 leaves of a weight goes to row g + 8
+      pack_half2_rest(p0 == 0.f ? 0.f : p0 * v0, p1 == 0.f ? 0.f : p1 * v1, w[j][0], w[j][1]);
     }
     // values: rank 64 vb + 8 g + n of lane (g, t) is column g of tile n; the keys of step m are the score columns' keys
 #pragma unroll 1
@@ -402,8 +353,8 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
             uint32_t b0, b1, c0, c1;
             codes_to_half(u, b0, c0);         // {key t, key t + 4} of the first rank, of the second
             codes_to_half(v, b1, c1);         // {key t + 8, key t + 12}
-            mma_rows<kFew>(o[vb][2 * q], w[0][0], w[0][1], w[1][0], w[1][1], b0, b1);
-            mma_rows<kFew>(o[vb][2 * q + 1], w[0][0], w[0][1], w[1][0], w[1][1], c0, c1);
+            mma_f16_16x8x16(o[vb][2 * q], w[0][0], w[0][1], w[1][0], w[1][1], b0, b1);
+            mma_f16_16x8x16(o[vb][2 * q + 1], w[0][0], w[0][1], w[1][0], w[1][1], c0, c1);
           }
         }
       }
@@ -416,39 +367,31 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   copy_wait<0>();
 
   // join the four warps: common maximum per row, sums in shared memory (the rings are done with)
-  l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
-  l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
-  l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
-  l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
   if (t4 == 0) {
-    s.m[warp][g] = m_a;
-    s.m[warp][g + 8] = m_b;
-    s.l[warp][g] = l_a;
-    s.l[warp][g + 8] = l_b;
+    s.m[warp][g] = m;
+    s.l[warp][g] = l;
   }
   __syncthreads();
   float* sums = reinterpret_cast<float*>(ring_mem) + warp * (kStreamRows * LSVD_MAX_RANK);
-  float top_a = s.m[0][g], top_b = s.m[0][g + 8];
+  float top = s.m[0][g];
 #pragma unroll
-  for (int w = 1; w < kChunkWarps; ++w) {
-    top_a = fmaxf(top_a, s.m[w][g]);
-    top_b = fmaxf(top_b, s.m[w][g + 8]);
-  }
+  for (int w = 1; w < kChunkWarps; ++w) top = fmaxf(top, s.m[w][g]);
   const float back = E > -200 ? pow2i(E - kWeightShift) : 1.f;
-  const float s_a = ex2(m_a - (top_a == -INFINITY ? 0.f : top_a)) * back, s_b = ex2(m_b - (top_b == -INFINITY ? 0.f : top_b)) * back;
+  const float by = ex2(m - (top == -INFINITY ? 0.f : top)) * back;
 #pragma unroll
   for (int vb = 0; vb < 2; ++vb)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int rank = 64 * vb + 16 * t4 + 8 * e;
       if (rank < rv) {
-        float4* da = reinterpret_cast<float4*>(sums + g * LSVD_MAX_RANK + rank);
-        float4* db = reinterpret_cast<float4*>(sums + (g + 8) * LSVD_MAX_RANK + rank);
-        da[0] = make_float4(o[vb][0][e] * s_a, o[vb][1][e] * s_a, o[vb][2][e] * s_a, o[vb][3][e] * s_a);
-        da[1] = make_float4(o[vb][4][e] * s_a, o[vb][5][e] * s_a, o[vb][6][e] * s_a, o[vb][7][e] * s_a);
-        if (kFew) continue;
-        db[0] = make_float4(o[vb][0][2 + e] * s_b, o[vb][1][2 + e] * s_b, o[vb][2][2 + e] * s_b, o[vb][3][2 + e] * s_b);
-        db[1] = make_float4(o[vb][4][2 + e] * s_b, o[vb][5][2 + e] * s_b, o[vb][6][2 + e] * s_b, o[vb][7][2 + e] * s_b);
+        float4* dst = reinterpret_cast<float4*>(sums + g * LSVD_MAX_RANK + rank);
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = (o[vb][j][e] + o[vb][j][2 + e]) * by;
+        dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+        dst[1] = make_float4(y[4], y[5], y[6], y[7]);
       }
     }
   __syncthreads();
@@ -565,10 +508,11 @@ static void chunk_split(int64_t blocks, int64_t want, int least, int unit, int m
   *splits = std::max(1, (max_len + *len - 1) / *len);
 }
 
-// Requests of up to 16 new tokens go to the stream form, longer ones to the tile form; a single request of a step that may
-// bring more than 16 always goes to the tile form (one launch).  The keys are split where the rows alone are too few
-// blocks: stream form, six rounds of the resident blocks (three per SM), pieces of 256 keys or more; tile form, two
-// rounds (one per SM), 512 keys or more.
+// Requests of up to 8 new tokens go to the stream form, longer ones to the tile form; a single request of a step that may
+// bring more than 8 always goes to the tile form (one launch).  The keys are split where the rows alone are too few
+// blocks: stream form, four rounds of the resident blocks (three per SM), pieces of 256 keys or more (at two, three, four, six
+// and eight rounds: eight requests of five tokens 140, 147, 152, 171, 192 us, 16 single tokens 257, 228, 225, 245, 257 us); tile
+// form, two rounds (one per SM), 512 keys or more.
 static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_new, int max_len) {
   ChunkPlan c{};
   const int64_t sms = std::max(1, device_sm_count());
@@ -725,14 +669,8 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (c.stream) {
     const bool cap = a->softcap > 0.f, bias = a->alibi_slopes != nullptr;
-    void (*kern)(ChunkParams) = nullptr;
-    if (c.stream_stride <= 8) {             // (no request has more rows)
-      kern = cap ? (bias ? chunk_stream_kernel<true, true, true> : chunk_stream_kernel<true, false, true>)
-                 : (bias ? chunk_stream_kernel<false, true, true> : chunk_stream_kernel<false, false, true>);
-    } else {
-      kern = cap ? (bias ? chunk_stream_kernel<true, true, false> : chunk_stream_kernel<true, false, false>)
-                 : (bias ? chunk_stream_kernel<false, true, false> : chunk_stream_kernel<false, false, false>);
-    }
+    void (*kern)(ChunkParams) = cap ? (bias ? chunk_stream_kernel<true, true> : chunk_stream_kernel<true, false>)
+                                    : (bias ? chunk_stream_kernel<false, true> : chunk_stream_kernel<false, false>);
     const int smem = kChunkWarps * kRingBytes;
     LSVD_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem));
     LSVD_CUDA_TRY(launch_chained(kern, dim3(a->num_heads, a->batch, c.stream_splits), dim3(kChunkThreads), smem, st, 1, true, p));

@@ -7,7 +7,7 @@
 namespace lsvd {
 
 constexpr float kChunkLog2e = 1.4426950408889634f;
-constexpr int kStreamRows = 16;      // query rows of a block of the stream form
+constexpr int kStreamRows = 8;      // query rows of a block of the stream form
 constexpr int kChunkTileRows = 256;  // and of the tile form
 
 struct ChunkHead {
@@ -138,6 +138,13 @@ __device__ __forceinline__ void codes_to_half(uint32_t u, uint32_t& lo, uint32_t
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Two values as fp16 and what that leaves of them, as fp16 too.  (An infinity or a NaN leaves nothing.)
+__device__ __forceinline__ void pack_half2_rest(float a, float b, uint32_t& most, uint32_t& rest) {
+  most = pack_half2(a, b);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&most));
+  const float x = a - h.x, y = b - h.y;
+  rest = pack_half2(fabsf(x) < INFINITY ? x : 0.f, fabsf(y) < INFINITY ? y : 0.f);
 }
 
 // Four consecutive halves, zero beyond `n` of them.

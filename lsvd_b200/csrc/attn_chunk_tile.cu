@@ -1,20 +1,31 @@
-// Attention of new tokens over the paged int8 latent cache, tile form: 128 query rows of one request and head per block, on
+// Attention of new tokens over the paged int8 latent cache, tile form: 256 query rows of one request and head per block, on
 // tcgen05.  (The mathematics and the stream form, for requests of few rows, are in attn_chunk.cu.)
 //
-// Per 64 keys a block does two products with the weights' softmax between them:
-//   S[128 x 64] = q~[128 x r_k] . z_k^T     A and B from shared memory, accumulator in tensor memory (two buffers)
+// The rows are two groups of 128.  Per 64 keys a block does, for each group, two products with the weights' softmax between them:
+//   S[128 x 64] = q~[128 x r_k] . z_k^T     A and B from shared memory, accumulator in tensor memory (two buffers); A twice,
+//                                           what fp16 keeps of q~ and the rest (22 bits in all)
 //   O[128 x r_v] += P[128 x 64] . z_v       A = P, fp16, written over S in tensor memory; B = the codes, ranks contiguous
-// 16384 exponentials per 128 x 128 scores take 1024 cycles of an SM (16 a cycle) while the products take 512 at ranks of
-// 64 + 64: the exponentials bound it, then the issue slots of the softmax (about six per score).  So the softmax warps must never
-// wait.  Eight warps: four for the softmax (thread = row, no exchange between threads), three that gather the rows by slot,
-// widen the int8 codes to fp16 (exact) and store them in the 128-byte-swizzled layouts that the products read, one that issues
-// the products.  The score product of tile j + 2 runs while the softmax is at tile j + 1, and two blocks share an SM (256 tensor
-// memory columns and at most 113 KB of shared memory each), so that one's waits are the other's cycles.
+// Thirteen warps: eight for the softmax (thread = row, no exchange between threads), four that gather the rows by slot, widen
+// the int8 codes to fp16 (exact) and store them in the 128-byte-swizzled layouts that the products read, one that issues the
+// products.  The codes are widened once for both groups; the score product of tile j + 2 runs while the softmax is at tile j + 1.
 //
-// The prologue computes q~ = B_k q with the same unit; the epilogue applies the V up-factor likewise (o_lat rounded to fp16,
-// as in the latent result).  O is rescaled only when a row's maximum has grown by more than 2^8 since its last
-// reference, or when a larger V scale arrives: weights are held as p * scale_v * 2^(6 - E) with p < 2^8 and 2^E the power of
-// two below the largest V scale seen, so fp16 neither overflows (< 2^15) nor loses bits above 2^-20 of the reference.
+// What bounds it.  The 16384 exponentials of 64 keys take 1024 cycles of an SM (16 a cycle), the products 768 at ranks of
+// 64 + 64; a step takes about 2600, and of these the softmax warps wait a quarter (clocks read inside the kernel): the issue of
+// two dependent chains per scheduler, then the load warps.  What moved it, for a prompt of 8191 tokens, 32 heads, ranks 64 + 64:
+//   * code size: the load warps' passes fully unrolled (compile-time widths) took 1.38 ms, as loops shared by K and V 0.97 ms:
+//     with all roles unrolled a third of the instruction fetches missed the SM's cache;
+//   * the prologue (q~ = B_k q) and the epilogue (o = B_v^T o_lat) with their factors read by every warp from global memory
+//     were 65 of 250 thousand cycles of an average block; with the factors in shared memory 0.88 ms;
+//   * four load warps instead of three 0.83 ms (five 0.85, seven 0.84);
+//   * both halves of q~ in the products, and of o_lat in the up-projection, 0.90 ms: the error against 64 bits went from 1.8 times
+//     that of a rounding of the result alone to 1.3 times.
+// Tried and slower: two threads a row with sixteen softmax warps (1.05 ms), the scores read twice instead of kept in registers
+// between the maximum and the weights (1.08 ms).  128 rows a block (mma m16n8k16) took 2.6 ms.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since its last reference, or when a larger V scale
+// arrives: weights are held as p * scale_v * 2^(6 - E) with p < 2^8 and 2^E the power of two below the largest V scale seen, so
+// fp16 neither overflows (< 2^15) nor loses bits above 2^-20 of the reference.  o_lat meets the up-factor as two
+// fp16 numbers, what fp16 keeps of it and the rest.
 #include <algorithm>
 
 #include "attn_chunk.cuh"
@@ -32,9 +43,9 @@ constexpr int kSoftmaxWarps = 4 * kGroups, kLoadWarps = 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
 constexpr int kTileThreads = (kMmaWarp + 1) * 32;
 constexpr int kLoadThreads = kLoadWarps * 32;
-constexpr int kTileSmem = 192 * 1024 + 1024;     // q~ (or o_lat), widened stages, copied codes; 1024 to align
+constexpr int kTileSmem = 208 * 1024 + 1024;     // q~ (or o_lat), widened stages, copied codes; 1024 to align
 constexpr int kTileMaxStages = 4;
-constexpr int kCodeStages = 4;                   // stages of codes on their way
+constexpr int kCodeStages = 4;                   // stages of codes on their way (one where four do not fit)
 constexpr int kTileSlotRing = 8;
 constexpr int kTileCols = 512;                   // tensor memory, 256 columns a group: S0 0..63, S1 64..127, O 128..255
 constexpr int kGroupCols = 256;
@@ -143,7 +154,7 @@ __device__ __forceinline__ void store_codes(uint8_t* tile, int row, int piece, u
 // `warps` warps that come here (read from global memory by every warp, 8 bytes a lane, the block's prologue took 34000 cycles).
 // With more than 64 ranks the first block is computed again once the row's largest entry over both is known.
 __device__ __forceinline__ void absorb_tile_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int row0, int rows,
-                                                 int warps, TileShared& s, uint8_t* q_tile, uint8_t* up) {
+                                                 int warps, TileShared& s, uint8_t* q_tile, int half_bytes, uint8_t* up) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int rk = H.nk * 16, blocks = rk > 64 ? 2 : 1;
   const int steps = (p.head_dim + 15) >> 4, stride = ((p.head_dim * 2 + 127) & ~127) + 32;      // (rows of lanes g on other banks)
@@ -205,8 +216,13 @@ __device__ __forceinline__ void absorb_tile_rows(const ChunkParams& p, const Chu
         if (t == 0) s.scale[row] = pow2i(ex);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (rank0 + 8 * j < rk)
-            *reinterpret_cast<uint32_t*>(block + swizzled(row & (kGroupRows - 1), j) + 4 * t) = pack_half2(acc[j][2 * e] * x, acc[j][2 * e + 1] * x);
+          if (rank0 + 8 * j < rk) {
+            uint32_t most, rest;
+            pack_half2_rest(acc[j][2 * e] * x, acc[j][2 * e + 1] * x, most, rest);
+            uint8_t* at = block + swizzled(row & (kGroupRows - 1), j) + 4 * t;
+            *reinterpret_cast<uint32_t*>(at) = most;
+            *reinterpret_cast<uint32_t*>(at + half_bytes) = rest;
+          }
       }
     }
   }
@@ -217,7 +233,7 @@ __device__ __forceinline__ void absorb_tile_rows(const ChunkParams& p, const Chu
 __device__ __forceinline__ void chunk_tile_up(const ChunkParams& p, const TileShared& s, uint8_t* smem) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, h = blockIdx.x;
   const ChunkHead H = p.head[h];
-  const int rv = H.nv * 16, q_bytes = ((max(H.nk, H.nv) + 3) >> 2) * kGroupRows * 128;
+  const int rv = H.nv * 16, half_bytes = ((max(H.nk, H.nv) + 3) >> 2) * kGroupRows * 128, q_bytes = 2 * half_bytes;
   const ChunkRequest r = chunk_request(p, s.b, false);
   const int row0 = s.tile * kTileRows, rows = min(kTileRows, r.n - row0);
   const int stride = p.head_dim * 2 + 16, quads = p.head_dim >> 2;
@@ -231,19 +247,21 @@ __device__ __forceinline__ void chunk_tile_up(const ChunkParams& p, const TileSh
 #pragma unroll 1
   for (int w = warp; w * 16 < rows; w += kTileThreads / 32) {
     const int ra = w * 16 + g, la = ra & (kGroupRows - 1), lb = la + 8;
-    uint32_t a[8][4];
+    uint32_t a[2][8][4];             // o_lat as fp16 and what that leaves of it
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const uint8_t* block = smem + (w >> 3) * q_bytes + (q >> 2) * kGroupRows * 128 + 4 * t;
-      const int c = 2 * (q & 3);
-      a[q][0] = a[q][1] = a[q][2] = a[q][3] = 0u;
-      if (q < H.nv) {
-        a[q][0] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c));
-        a[q][1] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c));
-        a[q][2] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c + 1));
-        a[q][3] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c + 1));
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint8_t* block = smem + (w >> 3) * q_bytes + x * half_bytes + (q >> 2) * kGroupRows * 128 + 4 * t;
+        const int c = 2 * (q & 3);
+        a[x][q][0] = a[x][q][1] = a[x][q][2] = a[x][q][3] = 0u;
+        if (q < H.nv) {
+          a[x][q][0] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c));
+          a[x][q][1] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c));
+          a[x][q][2] = *reinterpret_cast<const uint32_t*>(block + swizzled(la, c + 1));
+          a[x][q][3] = *reinterpret_cast<const uint32_t*>(block + swizzled(lb, c + 1));
+        }
       }
-    }
 #pragma unroll 1
     for (int d0 = 0; d0 < p.head_dim; d0 += 16) {      // 16 columns: two products a step, their B fragments by one transposing load
       const bool both = d0 + 8 < p.head_dim;
@@ -254,8 +272,11 @@ __device__ __forceinline__ void chunk_tile_up(const ChunkParams& p, const TileSh
         if (q >= H.nv) continue;
         uint32_t b[4];
         ldmatrix_x4_trans(b, from + 16 * q * stride);
-        mma_f16_16x8x16(y[0], a[q][0], a[q][1], a[q][2], a[q][3], b[0], b[1]);
-        mma_f16_16x8x16(y[1], a[q][0], a[q][1], a[q][2], a[q][3], b[2], b[3]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          mma_f16_16x8x16(y[0], a[x][q][0], a[x][q][1], a[x][q][2], a[x][q][3], b[0], b[1]);
+          mma_f16_16x8x16(y[1], a[x][q][0], a[x][q][1], a[x][q][2], a[x][q][3], b[2], b[3]);
+        }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -287,10 +308,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
   const ChunkHead H = p.head[h];
   const int rk = H.nk * 16, rv = H.nv * 16;
   const int kblocks = (H.nk + 3) >> 2, vblocks = (H.nv + 3) >> 2;            // 64-rank blocks
-  const int q_bytes = max(kblocks, vblocks) * kGroupRows * 128;              // of a group
+  const int half_bytes = max(kblocks, vblocks) * kGroupRows * 128, q_bytes = 2 * half_bytes;      // of a group: fp16, and the rest
   const int k_bytes = kblocks * kTileKeys * 128, stage_bytes = k_bytes + vblocks * kTileKeys * 128;
   const int code_bytes = kTileKeys * (rk + rv);
-  const int stages = kGroups * q_bytes + 4 * stage_bytes + kCodeStages * code_bytes <= kTileSmem - 1024 ? 4 : 2;
+  // four stages of each kind up to ranks of 64 + 64, two and one at 128 + 128
+  const int room = kTileSmem - 1024 - kGroups * q_bytes;
+  const int stages = 4 * stage_bytes + kCodeStages * code_bytes <= room ? 4 : 2;
+  const int code_stages = stages * stage_bytes + kCodeStages * code_bytes <= room ? kCodeStages : 1;
   uint8_t* stage0 = smem + kGroups * q_bytes;
   uint8_t* codes = stage0 + stages * stage_bytes;
 
@@ -396,9 +420,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
         tc_fence_after();
         if (elect_one()) {
           const uint64_t qdesc = smem_desc_k_major_sw128(smem + grp * q_bytes), kdesc = smem_desc_k_major_sw128(stage0 + st * stage_bytes);
-          for (int q = 0; q < H.nk; ++q)        // 16 ranks a step: 32 bytes of a row; a 64-rank block is a tile of its own
-            umma_f16_ss(tmem + grp * kGroupCols + (j & 1) * kTileKeys, qdesc + ((q >> 2) * (kGroupRows * 128 >> 4) + (q & 3) * 2),
-                        kdesc + ((q >> 2) * (kTileKeys * 128 >> 4) + (q & 3) * 2), idesc_s, q > 0 ? 1u : 0u);
+          // 16 ranks a step: 32 bytes of a row; a 64-rank block is a tile of its own.  First what fp16 keeps of q~, then the rest.
+          for (int rest = 0; rest < 2; ++rest)
+            for (int q = 0; q < H.nk; ++q)
+              umma_f16_ss(tmem + grp * kGroupCols + (j & 1) * kTileKeys,
+                          qdesc + (rest * (half_bytes >> 4) + (q >> 2) * (kGroupRows * 128 >> 4) + (q & 3) * 2),
+                          kdesc + ((q >> 2) * (kTileKeys * 128 >> 4) + (q & 3) * 2), idesc_s, (rest | q) != 0 ? 1u : 0u);
           umma_commit(&s.s_full[grp][j & 1]);
         }
         __syncwarp();
@@ -461,7 +488,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     const int k_piece = lt % H.nk, v_piece = lt % H.nv;
     auto request = [&](int j) {
       const int32_t* slots = s.slot[j & (kTileSlotRing - 1)];
-      uint8_t* dst = codes + (j & (kCodeStages - 1)) * code_bytes;
+      uint8_t* dst = codes + (j & (code_stages - 1)) * code_bytes;
 #pragma unroll 1
       for (int part = 0; part < 2; ++part) {
         const int step = part ? v_step : k_step, bytes = part ? rv : rk;
@@ -507,7 +534,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     }
     int slot_ahead = fetch_slot(kCodeStages);
     named_barrier(1, kLoadThreads);
-    for (int j = 0; j < kCodeStages - 1; ++j) {
+    const int deep = code_stages - 1;               // tiles requested ahead of the one in hand
+    for (int j = 0; j < max(deep, 1); ++j) {
       if (j < ntiles) request(j);
       copy_commit();
     }
@@ -518,16 +546,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     ok = __all_sync(0xffffffffu, ok);
     for (int j = 0; j < ntiles; ++j) {
       const int st = j & (stages - 1);
-      copy_wait<kCodeStages - 2>();
+      if (deep > 0) {
+        copy_wait<kCodeStages - 2>();
+      } else {
+        copy_wait<0>();
+      }
       // tile j's codes are here for every load warp, and all are done with the stage of tile j - 1.  Every load warp comes
       // here, whatever its waits returned, and all stop together.
       if (named_barrier_or(1, kLoadThreads, !ok)) break;
       keep_slot(j + kCodeStages, slot_ahead);
       slot_ahead = fetch_slot(j + kCodeStages + 1);
-      if (j + kCodeStages - 1 < ntiles) request(j + kCodeStages - 1);
-      copy_commit();
+      if (deep > 0) {
+        if (j + deep < ntiles) request(j + deep);
+        copy_commit();
+      }
       uint8_t* kd = stage0 + st * stage_bytes;
-      const uint8_t* kc = codes + (j & (kCodeStages - 1)) * code_bytes;
+      const uint8_t* kc = codes + (j & (code_stages - 1)) * code_bytes;
       ok = __all_sync(0xffffffffu, tile_wait(s, &s.empty[st], ((j / stages) & 1) ^ 1, p.status_word));
       if (!ok) continue;
       // the scales go first: the softmax reads them once K is there
@@ -556,6 +590,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.full[st]);
+      if (deep == 0) {                 // (what a thread copies it has widened itself)
+        if (j + 1 < ntiles) request(j + 1);
+        copy_commit();
+      }
     }
     copy_wait<0>();
   } else if (warp < live_warps) {
@@ -569,7 +607,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     int E = -200;
     bool go = true;
     if (ntiles > 0) {
-      absorb_tile_rows(p, H, h, r, row0, rows, live_warps, s, q_tile, stage0);
+      absorb_tile_rows(p, H, h, r, row0, rows, live_warps, s, q_tile, half_bytes, stage0);
       __syncwarp();
       f = s.scale[tid];
       f = fmaxf(f * p.score_scale * (kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e), 1e-37f);
@@ -771,10 +809,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
           store_halves8(dst + 8, hi, p.out_lat_vec16);
         }
         if (to_up && ntiles > 0) {
-          uint8_t* block = q_tile + (c >> 6) * kGroupRows * 128;
-          const int piece = (c & 63) >> 3, row = tid & (kGroupRows - 1);
-          *reinterpret_cast<uint4*>(block + swizzled(row, piece)) = lo;
-          *reinterpret_cast<uint4*>(block + swizzled(row, piece + 1)) = hi;
+          uint8_t* block = smem + grp * q_bytes + (c >> 6) * kGroupRows * 128;
+          uint32_t most[8], rest[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pack_half2_rest(y[2 * i], y[2 * i + 1], most[i], rest[i]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint8_t* at = block + swizzled(tid & (kGroupRows - 1), ((c & 63) >> 3) + i);
+            *reinterpret_cast<uint4*>(at) = make_uint4(most[4 * i], most[4 * i + 1], most[4 * i + 2], most[4 * i + 3]);
+            *reinterpret_cast<uint4*>(at + half_bytes) = make_uint4(rest[4 * i], rest[4 * i + 1], rest[4 * i + 2], rest[4 * i + 3]);
+          }
         }
       }
       if (to_up && ntiles == 0 && tid < rows)

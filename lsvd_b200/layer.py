@@ -118,6 +118,8 @@ def _layer_chunk(self, x, cache_k, scale_k, cache_v, scale_v, state, stages=None
     and ``alibi_slopes`` as in ``chunk_attention_int8_latent_absorb``.  Rows behind the last token hold no result.
     The products take the decode kernels up to 64 tokens and the tcgen05 GEMM beyond, as the FFN does."""
     lay, T = self.layout, x.shape[0]
+    if T == 0:
+        return torch.empty_like(x) if out is None else out
     few = T <= 64
 
     def product(q, s, w, ws, residual=None):
