@@ -287,7 +287,7 @@ typedef struct lsvd_attn_chunk_args {
   int32_t* status_word;          /* device int32 or NULL                                                           */
   int32_t cache_layout;          /* LSVD_CACHE_*                                                                   */
   int32_t req_to_token_rows;     /* a b_req_idx outside [0, rows) makes the request an empty one and is reported   */
-  int32_t causal, window;        /* window <= 0: none                                                              */
+  int32_t causal, window;        /* window 0: none                                                                 */
   float softcap;                 /* 0: none; otherwise at least 1e-6 (smaller: LSVD_ERR_UNSUPPORTED), finite       */
   const float* alibi_slopes;     /* device fp32 [num_heads] or NULL                                                */
   const int32_t* b_prefix_len;   /* device int32 [batch] or NULL                                                   */
