@@ -431,3 +431,64 @@ def test_two_streams_at_once():
 def test_either_side_of_the_two_forms(news, olds):
     """Eight new tokens are the most that the form for few rows takes."""
     _check(_case(news, olds, [128, 16], [128, 64], seed=8))
+
+
+@pytest.mark.parametrize("head_major", [False, True])
+@pytest.mark.parametrize("news", [[4], [20]])
+def test_slots_behind_the_first_four_gigabytes(news, head_major):
+    """The case's rows at the end of a cache whose K side has 5 GB: byte offsets pass 32 bits."""
+    c = _case(news, [40], [64, 64], [16, 16])
+    o, _, o_tol, _ = _want(c)
+    n, N = c["cache_k"].shape[0], 40_000_000
+    lay = LatentCacheLayout([64, 64], [16, 16], head_major=head_major)
+    big = lay.alloc(N, DEV)
+    for side, cache, scale, ranks in (("k", big[0], big[1], 64), ("v", big[2], big[3], 16)):
+        rows, scales = c["cache_" + side].to(DEV), c["scale_" + side].to(DEV)
+        if head_major:
+            for h in range(2):
+                cache.view(2, N, ranks)[h, N - n:] = rows[:, h * ranks:(h + 1) * ranks]
+                scale[h, N - n:] = scales[:, h]
+        else:
+            cache.view(N, 2 * ranks)[N - n:] = rows
+            scale[N - n:] = scales
+    r2t = torch.where(c["req_to_token"] >= 0, c["req_to_token"] + (N - n), c["req_to_token"]).to(DEV)
+    st = ChunkState(c["b_req_idx"].to(DEV), c["b_seq_len"].to(DEV), c["start"].to(DEV), r2t, c["max_len"], max(news))
+    ck, cv = (big[0], big[2]) if head_major else (big[0].view(N, -1), big[2].view(N, -1))
+    got = chunk_attention_int8_latent_absorb(c["q"].to(DEV), st, 2, 64, ck, big[1], cv, big[3], c["up_k"].to(DEV), c["up_v"].to(DEV), layout=lay)
+    _close(got.cpu(), o, o_tol)
+
+
+@pytest.mark.parametrize("news", [[3], [30]])
+def test_shared_key_and_value_latent(news):
+    """One cached latent per head serves K and V: appended once, read as both."""
+    ranks, D = [64, 32], 64
+    lay, flat = LatentCacheLayout(ranks, shared_kv=True), LatentCacheLayout(ranks, ranks)
+    g = torch.Generator().manual_seed(9)
+    state = ChunkState.paged(rows=1, max_len_in_batch=100, max_tokens=50, max_new_in_batch=50, num_pages=7, page_size=16)
+    cache = lay.alloc(112, DEV)
+    plain = flat.alloc(112, "cpu")
+    up_k, up_v = (torch.randn(lay.sum_k, D, generator=g) / 8).half(), (torch.randn(lay.sum_k, D, generator=g) / 8).half()
+    attn = LatentDecodeAttention(lay, D, up_k.to(DEV), up_v.to(DEV))
+    for n in (50, news[0]):
+        z, q = torch.randn(n, lay.sum_k, generator=g).half(), torch.randn(n, 2, D, generator=g).half()
+        state.begin(torch.tensor([n], dtype=torch.int32, device=DEV))
+        out = attn.forward_chunk(q.to(DEV), *cache, state, latent_k=z.to(DEV))
+        mem = state.mem_index.cpu()[:n]
+        for side in (0, 2):
+            oattn.cache_append(z, mem, flat.k_off, plain[side], plain[side + 1])
+        o, _, tol, _ = oattn.chunk_absorb(q, *plain, up_k, up_v, flat.k_off, flat.v_off, state.req_manager.req_to_token_indexs.cpu(),
+                                          state.b_req_idx.cpu(), state.b_seq_len.cpu(), state.b_start_loc.cpu())
+        assert ((out.cpu().double() - o).abs() <= tol).all()
+
+
+def test_no_tokens():
+    c = _case([2], [3], [64, 32], [48, 64])
+    lay = c["layout"]
+    st = ChunkState(c["b_req_idx"].to(DEV), c["b_seq_len"].to(DEV), torch.zeros(2, dtype=torch.int32, device=DEV), c["req_to_token"].to(DEV), c["max_len"], 0)
+    attn = LatentDecodeAttention(lay, 64, c["up_k"].to(DEV), c["up_v"].to(DEV))
+    caches = [c[k].to(DEV) for k in ("cache_k", "scale_k", "cache_v", "scale_v")]
+    assert attn.forward_chunk(c["q"][:0].to(DEV), *caches, st).shape == (0, 2, 64)
+    out = torch.full((2, 2, 64), 77.0, dtype=torch.float16, device=DEV)
+    attn.forward_chunk(c["q"].to(DEV), *caches, st, out=out)             # rows, but no request's
+    torch.cuda.synchronize()
+    assert (out == 77.0).all()
