@@ -10,8 +10,9 @@
 // products.  The codes are widened once for both groups; the score product of tile j + 2 runs while the softmax is at tile j + 1.
 //
 // What bounds it.  The 16384 exponentials of 64 keys take 1024 cycles of an SM (16 a cycle), the products 768 at ranks of
-// 64 + 64; a step takes about 2600, and of these the softmax warps wait a quarter (clocks read inside the kernel): the issue of
-// two dependent chains per scheduler, then the load warps.  What moved it, for a prompt of 8191 tokens, 32 heads, ranks 64 + 64:
+// 64 + 64; a step takes about 2900 (clocks read inside the kernel).  With three load warps the softmax warps waited a quarter to a
+// third of it and the load warps hardly ever; with four the dependent chains of the softmax, two warps a scheduler, are what is left
+// (fixed-latency waits lead the stalls, 41 % of the issue slots are used).  What moved it, for a prompt of 8191 tokens, 32 heads, ranks 64 + 64:
 //   * code size: the load warps' passes fully unrolled (compile-time widths) took 1.38 ms, as loops shared by K and V 0.97 ms:
 //     with all roles unrolled a third of the instruction fetches missed the SM's cache;
 //   * the prologue (q~ = B_k q) and the epilogue (o = B_v^T o_lat) with their factors read by every warp from global memory
