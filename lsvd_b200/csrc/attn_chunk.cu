@@ -4,14 +4,14 @@
 // latents with q~, and the values stay in the latent space until the end:
 //   x_t = sm_scale scale_k[t] (z_k[t] . q~) [capped, biased],  o_lat = sum_t softmax(x)_t scale_v[t] z_v[t],  o = B_v^T o_lat.
 //
-// Stream form (up to 8 query rows of a request share one pass over its cache): a block owns (request, head, the rows,
+// Stream form (8 query rows of a request share one pass over its cache): a block owns (request, head, the rows,
 // split of the keys); each of its four warps walks its own 32-key tiles.  The rows arrive by 16-byte asynchronous copies in
 // a ring of shared memory per warp (gathered slot by slot: any page table, both cache layouts); codes become fp16 exactly
 // (|code| <= 128) and meet q~ and the weights on the tensor cores (mma m16n8k16, fp32 accumulators).  With few rows the bytes
 // of the cache would bound it, r_k + r_v + 4 bytes per key and head; what does is the instruction stream of a tile (widening,
 // two products of 16-row fragments that few rows fill, softmax) at twelve warps an SM.  Measured: 16 single tokens over 4096 keys, 32
-// heads, mean ranks 64 + 64: 201 us (268 MB, 1.3 TB/s); five tokens of eight requests 139 us.  Softmax for the lower
-// half of the fragments as well (requests of 9 to 16 rows in this form) cost 230 against 215 us; the value loop is rolled for
+// heads, mean ranks 64 + 64: 201 us (268 MB, 1.3 TB/s); five tokens of eight requests 139 us.  Sixteen rows a
+// block, with the lower half of the fragments for rows 9 to 16, cost the few-row cases 230 against 215 us; the value loop is rolled for
 // the instruction cache (215 -> 201 us).
 //
 // Roundings.  q~ enters the products as two fp16 numbers, what fp16 keeps of it and the rest, relative to its row's largest entry (a
@@ -50,10 +50,10 @@ struct __align__(16) ChunkShared {
 
 // q~ of up to 8 rows into shared memory, by all warps of the block: warp w takes the 8-rank tiles w, w + 4, ...
 // (mma lane (g, t): row g, rows 8 .. 15 zero, k = halves 4t .. 4t + 3 of a 16-wide step, ranks 8 j + g).
-__device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int rows,
+__device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHead& H, int h, const ChunkRequest& r, int row0, int rows,
                                             uint8_t* ring_mem) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const __half* qa = p.q + static_cast<int64_t>(r.start + min(g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
+  const __half* qa = p.q + static_cast<int64_t>(r.start + row0 + min(g, rows - 1)) * p.q_stride_t + h * p.q_stride_h;
   const int tiles = H.nk * 2;
   for (int j = warp; j < tiles; j += kChunkWarps) {
     const __half* up = p.up_k + static_cast<int64_t>(H.k_col + j * 8 + g) * p.up_k_row_stride;
@@ -73,7 +73,7 @@ __device__ __forceinline__ void absorb_rows(const ChunkParams& p, const ChunkHea
   }
 }
 
-// grid: (heads, batch, splits)
+// grid: (heads, requests' first rows and, where some request may have more than 8, their second ones, splits)
 template <bool kCap, bool kBias>
 __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __grid_constant__ ChunkParams p) {
   extern __shared__ __align__(16) uint8_t ring_mem[];
@@ -81,10 +81,11 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   grid_dependency_release();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-  const int h = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
-  const ChunkRequest r = chunk_request(p, b, h == 0 && split == 0 && threadIdx.x == 0);
-  const int rows = r.n;
-  if (rows <= 0 || rows > kStreamRows) return;      // none, or the tile form's
+  const int h = blockIdx.x, split = blockIdx.z;
+  const int row0 = static_cast<int>(blockIdx.y) >= p.batch ? kStreamRows : 0, b = blockIdx.y - (row0 > 0 ? p.batch : 0);
+  const ChunkRequest r = chunk_request(p, b, h == 0 && split == 0 && row0 == 0 && threadIdx.x == 0);
+  if (r.n <= row0 || r.n > kStreamMost) return;      // none, or the tile form's
+  const int rows = min(r.n - row0, kStreamRows);
   const ChunkHead H = p.head[h];
   const int rk = H.nk * 16, rv = H.nv * 16;
 
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     KeyRange k;
     k.lo = k.hi = 0;
     if (static_cast<int>(threadIdx.x) < rows)
-      k = visible_keys(p, r, p.b_prefix_len != nullptr ? p.b_prefix_len[b] : 0, threadIdx.x);
+      k = visible_keys(p, r, p.b_prefix_len != nullptr ? p.b_prefix_len[b] : 0, row0 + threadIdx.x);
     s.lo[threadIdx.x] = k.lo;
     s.hi[threadIdx.x] = k.hi;
   }
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
 
   if (ntiles == 0 && p.stream_partials) {      // the merge reads no sums where the weights' sum is zero
     if (static_cast<int>(threadIdx.x) < rows)
-      p.stream_ml[(static_cast<int64_t>(split) * p.batch * p.stream_stride + b * p.stream_stride + threadIdx.x) * p.num_heads + h] =
+      p.stream_ml[(static_cast<int64_t>(split) * p.batch * p.stream_stride + b * p.stream_stride + row0 + threadIdx.x) * p.num_heads + h] =
           make_float2(-INFINITY, 0.f);
     return;
   }
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   __half sk_next = __ushort_as_half(0), sv_next = sk_next;
   load_scales(0, sk_next, sv_next);
 
-  absorb_rows(p, H, h, r, rows, ring_mem);
+  absorb_rows(p, H, h, r, row0, rows, ring_mem);
   __syncthreads();
   const float* qt = absorbed_row(ring_mem, g);
   // q~ as fp16 A fragments: step (mb, i) of a 64-rank block holds ranks 64 mb + 16 t + 4 i .. + 3 of lane (g, t).  Row g is what
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   __syncthreads();                    // the rings' last stages may be written from here on
   const float cap_log2e = p.softcap * kChunkLog2e;
   f *= kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e;
-  const int lo = s.lo[g], hi = s.hi[g], pos = r.len - r.n + g;
+  const int lo = s.lo[g], hi = s.hi[g], pos = r.len - r.n + row0 + g;
   const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
 
   float m = -INFINITY, l = 0.f;
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   const float* all = reinterpret_cast<const float*>(ring_mem);
   for (int x = threadIdx.x; x < rows * rv; x += kChunkThreads) {
     const int row = x / rv, rank = x - row * rv;
-    const int token = r.start + row;
+    const int token = r.start + row0 + row;
     float top = s.m[0][row], sum = 0.f, v = 0.f;
 #pragma unroll
     for (int w = 1; w < kChunkWarps; ++w) top = fmaxf(top, s.m[w][row]);
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       v += all[w * (kStreamRows * LSVD_MAX_RANK) + row * LSVD_MAX_RANK + rank];
     }
     if (p.stream_partials) {
-      const int64_t at = (static_cast<int64_t>(split) * p.batch + b) * p.stream_stride + row;
+      const int64_t at = (static_cast<int64_t>(split) * p.batch + b) * p.stream_stride + row0 + row;
       p.stream_o[at * p.sum_rv + H.v_col + rank] = v;
       if (rank == 0) p.stream_ml[at * p.num_heads + h] = make_float2(top, sum);
     } else {
@@ -508,8 +509,10 @@ static void chunk_split(int64_t blocks, int64_t want, int least, int unit, int m
   *splits = std::max(1, (max_len + *len - 1) / *len);
 }
 
-// Requests of up to 8 new tokens go to the stream form, longer ones to the tile form; a single request of a step that may
-// bring more than 8 always goes to the tile form (one launch).  The keys are split where the rows alone are too few
+// Requests of up to 16 new tokens go to the stream form (from 9 on as two blocks, each with its own pass over the keys), longer ones
+// to the tile form: eight requests over 4091 keys with 8, 9 and 16 new tokens each take 147, 233 and
+// 238 us so, 369 in the tile form.  A single
+// request of a step that may bring more than 16 always goes to the tile form (one launch).  The keys are split where the rows alone are too few
 // blocks: stream form, four rounds of the resident blocks (three per SM), pieces of 256 keys or more (at two, three, four, six
 // and eight rounds: eight requests of five tokens 140, 147, 152, 171, 192 us, 16 single tokens 257, 228, 225, 245, 257 us); tile
 // form, two rounds (one per SM), 512 keys or more.
@@ -517,10 +520,10 @@ static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_ne
   ChunkPlan c{};
   const int64_t sms = std::max(1, device_sm_count());
   const int longest = std::max(1, std::min(max_new, num_tokens));
-  c.tile = longest > kStreamRows;
+  c.tile = longest > kStreamMost;
   c.stream = !c.tile || batch > 1;
-  c.tile_min = c.stream ? kStreamRows : 0;
-  c.stream_stride = std::min(kStreamRows, longest);
+  c.tile_min = c.stream ? kStreamMost : 0;
+  c.stream_stride = std::min(kStreamMost, longest);
   chunk_split(static_cast<int64_t>(num_heads) * batch, 4 * 3 * sms, 256, 128, max_len, &c.stream_splits, &c.stream_split_len);
   const int64_t of_tokens = num_tokens / kChunkTileRows + std::min<int64_t>(batch, num_tokens / (c.tile_min + 1));
   const int64_t of_requests = static_cast<int64_t>(batch) * ((longest + kChunkTileRows - 1) / kChunkTileRows);
@@ -599,7 +602,8 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   if (!std::isfinite(a->softcap) || !std::isfinite(a->sm_scale) || a->softcap < 0.f || a->window < 0) return LSVD_ERR_INVALID_ARG;
   if (a->softcap > 0.f && a->softcap < 1e-6f) return LSVD_ERR_UNSUPPORTED;      // (the scores' factor 1 / softcap has to stay in range)
   const ChunkPlan c = chunk_plan(a->batch, a->num_heads, a->num_tokens, a->max_new_in_batch, a->max_len_in_batch);
-  if (a->batch > 65535 || c.tiles > 65535 || (a->num_tokens + kMergeRows - 1) / kMergeRows > 65535) return LSVD_ERR_UNSUPPORTED;
+  const int64_t stream_blocks = static_cast<int64_t>(a->batch) * (c.stream_stride > kStreamRows ? 2 : 1);
+  if (a->batch > 65535 || stream_blocks > 65535 || c.tiles > 65535 || (a->num_tokens + kMergeRows - 1) / kMergeRows > 65535) return LSVD_ERR_UNSUPPORTED;
   const bool stream_partials = c.stream && (c.stream_splits > 1 || a->out != nullptr);
   const bool merge = stream_partials || c.tile_splits > 1;
   const ChunkWorkspace w = chunk_workspace(c, a->batch, a->num_heads, sum_rv, a->num_tokens);
@@ -673,7 +677,7 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
                                     : (bias ? chunk_stream_kernel<false, true> : chunk_stream_kernel<false, false>);
     const int smem = kChunkWarps * kRingBytes;
     LSVD_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem));
-    LSVD_CUDA_TRY(launch_chained(kern, dim3(a->num_heads, a->batch, c.stream_splits), dim3(kChunkThreads), smem, st, 1, true, p));
+    LSVD_CUDA_TRY(launch_chained(kern, dim3(a->num_heads, static_cast<unsigned>(stream_blocks), c.stream_splits), dim3(kChunkThreads), smem, st, 1, true, p));
   }
   if (c.tile) LSVD_CUDA_TRY(launch_chunk_tile(p, c.tiles, st));
   if (merge)

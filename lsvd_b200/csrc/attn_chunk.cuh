@@ -8,6 +8,7 @@ namespace lsvd {
 
 constexpr float kChunkLog2e = 1.4426950408889634f;
 constexpr int kStreamRows = 8;      // query rows of a block of the stream form
+constexpr int kStreamMost = 2 * kStreamRows;      // of a request of the stream form: one or two blocks
 constexpr int kChunkTileRows = 256;  // and of the tile form
 
 struct ChunkHead {

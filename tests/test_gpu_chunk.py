@@ -427,9 +427,9 @@ def test_two_streams_at_once():
 
 
 @pytest.mark.parametrize("news,olds", [([8], [33]), ([9], [33]), ([8, 9, 16], [500, 0, 64]), ([8] * 5 + [1], [3, 200, 31, 32, 0, 700]),
-                                       ([256, 8], [0, 256])])
+                                       ([256, 8], [0, 256]), ([16, 17, 15], [300, 70, 0])])
 def test_either_side_of_the_two_forms(news, olds):
-    """Eight new tokens are the most that the form for few rows takes."""
+    """A block of the form for few rows takes eight, a request sixteen."""
     _check(_case(news, olds, [128, 16], [128, 64], seed=8))
 
 
