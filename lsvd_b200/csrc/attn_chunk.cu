@@ -16,8 +16,8 @@
 //
 // Roundings.  q~ enters the products as two fp16 numbers, what fp16 keeps of it and the rest, relative to its row's largest entry (a
 // power of two taken out, so no entry overflows and small ones keep their bits down to 2^-23 of the largest).  The weights
-// p * scale_v are fp16 relative to the largest V scale seen: 2^-11 of each term, the size of the rounding of the fp16 result, in the
-// tile form; the stream form carries their rest too, in the half of the fragment that its few rows leave free.  Maxima, sums and
+// p * scale_v enter as two fp16 numbers as well, relative to the largest V scale seen; the stream form carries the second ones in the
+// half of the fragment that its few rows leave free, the tile form in a product of their own.  Maxima, sums and
 // accumulators are fp32.  Scales are applied in fp32 to scores and weights, never to the codes: a masked key's scale, were it
 // infinite or NaN, touches nothing.
 #include <algorithm>
