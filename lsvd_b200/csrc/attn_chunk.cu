@@ -16,10 +16,10 @@
 //
 // Roundings.  q~ enters the products as two fp16 numbers, what fp16 keeps of it and the rest, relative to its row's largest entry (a
 // power of two taken out, so no entry overflows and small ones keep their bits down to 2^-23 of the largest).  The weights
-// p * scale_v enter as two fp16 numbers as well, relative to the largest V scale seen; the stream form carries the second ones in the
-// half of the fragment that its few rows leave free, the tile form in a product of their own.  Maxima, sums and
-// accumulators are fp32.  Scales are applied in fp32 to scores and weights, never to the codes: a masked key's scale, were it
-// infinite or NaN, touches nothing.
+// p * scale_v enter as two fp16 numbers as well, relative to the largest one that the row sees (attn_chunk.cuh); the stream form
+// carries the second ones in the half of the fragment that its few rows leave free, the tile form in a product of their own.
+// References, sums and accumulators are fp32.  Scales are applied in fp32 to scores and weights, never to the codes: a masked key's
+// scale, were it huge, infinite or NaN, touches nothing.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -33,7 +33,6 @@ constexpr int kChunkWarps = 4;
 constexpr int kChunkThreads = kChunkWarps * 32;
 constexpr int kRingBytes = 16 * 1024;         // per warp: 2 to 8 stages of 32 keys x (r_k + r_v) bytes
 constexpr int kMaxStages = 8;
-constexpr int kWeightShift = 10;              // weights are held as p * scale_v * 2^(10 - E), 2^E <= largest scale < 2^(E+1)
 
 // Absorbed query row `row` [128] fp32: four rows in the last 2 KB of every warp's ring, which no copy reaches before the
 // first tile is consumed (stages 0 .. n - 2 are requested ahead of that; the last stage, or what lies behind it, is free).
@@ -43,6 +42,7 @@ __device__ __forceinline__ float* absorbed_row(uint8_t* ring_mem, int row) {
 
 struct __align__(16) ChunkShared {
   float sk[kChunkWarps][32], sv[kChunkWarps][32];             // scales of the tile in hand
+  float se[kChunkWarps][32];                                  // exponents of the V scales
   int32_t slot[kChunkWarps][kMaxStages][32];                  // slot of every key in the ring, -1: none
   float m[kChunkWarps][kStreamRows], l[kChunkWarps][kStreamRows];
   int32_t lo[kStreamRows], hi[kStreamRows];
@@ -222,8 +222,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   const int lo = s.lo[g], hi = s.hi[g], pos = r.len - r.n + row0 + g;
   const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
 
-  float m = -INFINITY, l = 0.f;
-  int E = -200;                       // exponent of the largest V scale so far
+  float R = -INFINITY, l = 0.f;       // reference and sum of the weights
   float o[2][8][4];
 #pragma unroll
   for (int vb = 0; vb < 2; ++vb)
@@ -243,15 +242,11 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     const float sk = my_slot >= 0 ? __half2float(sk_next) : 0.f, sv = my_slot >= 0 ? __half2float(sv_next) : 0.f;
     const uint32_t valid = __ballot_sync(0xffffffffu, my_slot >= 0);
     load_scales(i + 1, sk_next, sv_next);
-    // V scales relative to the largest one: a larger one than before moves the accumulators' exponent
-    int e_new = E;
-    {
-      const float av = fabsf(sv);
-      const int e = (av > 0.f && av < INFINITY) ? exponent_of(av) : -200;
-      e_new = max(E, __reduce_max_sync(0xffffffffu, e));
-    }
+    const float se = scale_exponent(sv);
+    const float e_top = static_cast<float>(__reduce_max_sync(0xffffffffu, static_cast<int>(se)));      // of all keys, seen or not
     s.sk[warp][lane] = sk;
-    s.sv[warp][lane] = sv * pow2i(kWeightShift - e_new);
+    s.sv[warp][lane] = sv;
+    s.se[warp][lane] = se;
     if (stages == 8) copy_wait<7>();
     else if (stages == 4) copy_wait<3>();
     else copy_wait<1>();
@@ -301,25 +296,33 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
         top = fmaxf(top, v);
       }
     }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
-    if (__any_sync(0xffffffffu, m_new != m || e_new != E)) {
-      const float c = ex2(m - base);       // a first maximum: 2^-inf = 0
-      l *= c;
-      const float by = c * pow2i(max(E - e_new, -126));
+    // top + e_top bounds what the row sees here: only where that is past the reference is the row's own value looked for
+    if (__any_sync(0xffffffffu, R == -INFINITY ? top > -INFINITY : top + e_top > R + kLazy)) {
+      float need = -INFINITY;
 #pragma unroll
-      for (int vb = 0; vb < 2; ++vb)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          o[vb][j][0] *= by;
-          o[vb][j][1] *= by;
-          o[vb][j][2] *= by;
-          o[vb][j][3] *= by;
-        }
-      m = m_new;
-      E = e_new;
+        for (int e = 0; e < 2; ++e) need = fmaxf(need, x[j][e] + s.se[warp][8 * j + t4 + 4 * e]);
+      need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, 1));
+      need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, 2));
+      const bool first = R == -INFINITY;
+      const bool grown = first ? need > -INFINITY : need > R + kLazy;
+      if (__any_sync(0xffffffffu, grown && !first)) {
+        const float by = grown && !first ? ex2(R - need) : 1.f;
+        l *= by;
+#pragma unroll
+        for (int vb = 0; vb < 2; ++vb)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            o[vb][j][0] *= by;
+            o[vb][j][1] *= by;
+            o[vb][j][2] *= by;
+            o[vb][j][3] *= by;
+          }
+      }
+      if (grown) R = need;
     }
+    const float base = R == -INFINITY ? 0.f : R - kWeightShift;
     uint32_t w[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -367,11 +370,11 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   }
   copy_wait<0>();
 
-  // join the four warps: common maximum per row, sums in shared memory (the rings are done with)
+  // join the four warps: common reference per row, sums in shared memory (the rings are done with)
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
   if (t4 == 0) {
-    s.m[warp][g] = m;
+    s.m[warp][g] = R;
     s.l[warp][g] = l;
   }
   __syncthreads();
@@ -379,8 +382,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
   float top = s.m[0][g];
 #pragma unroll
   for (int w = 1; w < kChunkWarps; ++w) top = fmaxf(top, s.m[w][g]);
-  const float back = E > -200 ? pow2i(E - kWeightShift) : 1.f;
-  const float by = ex2(m - (top == -INFINITY ? 0.f : top)) * back;
+  const float by = ex2(R - (top == -INFINITY ? 0.f : top));
 #pragma unroll
   for (int vb = 0; vb < 2; ++vb)
 #pragma unroll

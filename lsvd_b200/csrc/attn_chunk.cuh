@@ -11,6 +11,14 @@ constexpr int kStreamRows = 8;      // query rows of a block of the stream form
 constexpr int kStreamMost = 2 * kStreamRows;      // of a request of the stream form: one or two blocks
 constexpr int kChunkTileRows = 256;  // and of the tile form
 
+// Weights are 2^(x - R + kWeightShift) with R, the row's reference, the largest x + exponent of |V scale| among the keys that the row
+// SEES when R was last moved (x: score in units of log2).  R moves when that has grown by more than kLazy, so |weight * scale| stays
+// below 2^15, fits fp16, and keeps its bits down to 2^-31 of the largest.  Keys that a row does not see have no part in it, nor has
+// a large scale whose weight is nothing.  R and the weights' sum go through splits and joins like a maximum and its sum.
+constexpr float kWeightShift = 6.f;
+constexpr float kLazy = 8.f;
+constexpr int kLeastExponent = -24;      // of a finite fp16 scale; also for zero, infinity and NaN
+
 struct ChunkHead {
   int32_t k_col, v_col;      // byte offsets of the head inside a K / V cache row
   int16_t nk, nv;            // 16-entry pieces of K and V
@@ -36,7 +44,7 @@ struct ChunkParams {
   int64_t out_stride_t, out_stride_h;
   __half* out_latent;
   int64_t out_latent_stride_t;
-  // partial results, for the merge: running maximum (log2 domain) and sum [split][row][head], unnormalised sums
+  // partial results, for the merge: reference (log2 domain) and sum of weights [split][row][head], unnormalised sums
   // [split][row][sum r_v]; a row is request * stream_stride + i in the stream form, the token's row in the tile form
   float2* stream_ml;
   float* stream_o;
@@ -124,6 +132,10 @@ __device__ __forceinline__ float capped_log2(float u, float cap_log2e) {
 // Exponent e with 2^e <= x < 2^(e+1) for a positive normal x (0 for what is not positive and finite).
 __device__ __forceinline__ int exponent_of(float x) {
   return (x > 0.f && x < INFINITY) ? static_cast<int>((__float_as_uint(x) >> 23) & 255u) - 127 : 0;
+}
+__device__ __forceinline__ float scale_exponent(float x) {
+  const int e = static_cast<int>((__float_as_uint(x) >> 23) & 255u);
+  return static_cast<float>(e > 0 && e < 255 ? e - 127 : kLeastExponent);
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23); }
 

@@ -24,9 +24,8 @@
 // Tried and slower: two threads a row with sixteen softmax warps (1.05 ms), the scores read twice instead of kept in registers
 // between the maximum and the weights (1.08 ms).  128 rows a block (mma m16n8k16) took 2.6 ms.
 //
-// O is rescaled only when a row's maximum has grown by more than 2^8 since its last reference, or when a larger V scale
-// arrives: weights are held as p * scale_v * 2^(6 - E) with p < 2^8 and 2^E the power of two below the largest V scale seen, so
-// fp16 neither overflows (< 2^15) nor loses bits above 2^-31 of the reference.  Each weight enters the product as two fp16 numbers, its
+// O is rescaled only when a row's reference moves (attn_chunk.cuh): a reference is looked for where a tile's largest score and largest
+// V scale together are past it, over the keys that the row sees.  Each weight enters the product as two fp16 numbers, its
 // first eleven bits and the rest: one rounding to fp16 instead, 2^-11 of every term, made the error against 64 bits 1.2 to 1.4 times that
 // of rounding the exact result, the second half costs 4 to 15 % (a prompt of 8191 tokens, 32 heads, ranks 64 + 64: 897 -> 1000 us).  o_lat meets the up-factor as two
 // fp16 numbers, what fp16 keeps of it and the rest.
@@ -54,15 +53,13 @@ constexpr int kTileSlotRing = 8;
 constexpr int kTileCols = 512;                   // tensor memory, 256 columns a group: S0 0..63, S1 64..127, O 128..255
 constexpr int kGroupCols = 256;
 constexpr int kColO = 128;
-constexpr float kLazy = 8.f;                     // growth of a row's maximum (log2) that rescales O
-constexpr int kTileShift = 6;
 
 struct __align__(16) TileShared {
-  float sk[kTileMaxStages][kTileKeys], sv[kTileMaxStages][kTileKeys];      // first: read in 16-byte pieces
+  float sk[kTileMaxStages][kTileKeys], sv[kTileMaxStages][kTileKeys], se[kTileMaxStages][kTileKeys];      // first: read in 16-byte pieces
   uint64_t full[kTileMaxStages], empty[kTileMaxStages];
   uint64_t s_full[kGroups][2], p_full[kGroups][2], o_done[kGroups], q_full[kGroups], last;
   uint32_t live[kTileMaxStages][2];              // keys with a slot, one bit each
-  int32_t E[kTileMaxStages];
+  float e_top[kTileMaxStages];                   // largest of se
   int32_t slot[kTileSlotRing][kTileKeys];
   uint32_t tmem;
   volatile uint32_t abort;
@@ -531,7 +528,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       }
     };
     __half raw0 = __ushort_as_half(0), raw1 = raw0;
-    int sl0 = -1, sl1 = -1, E = -200;
+    int sl0 = -1, sl1 = -1;
     auto load_scales = [&](int j) {
       if (lw > 1 || j >= ntiles) return;
       sl0 = s.slot[j & (kTileSlotRing - 1)][lane];
@@ -581,17 +578,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       // the scales go first: the softmax reads them once K is there
       const float sc0 = sl0 >= 0 ? __half2float(raw0) : 0.f, sc1 = sl1 >= 0 ? __half2float(raw1) : 0.f;
       if (lw == 0) {
-        const float a0 = fabsf(sc0), a1 = fabsf(sc1);
-        int e = -200;
-        if (a0 > 0.f && a0 < INFINITY) e = exponent_of(a0);
-        if (a1 > 0.f && a1 < INFINITY) e = max(e, exponent_of(a1));
-        E = max(E, __reduce_max_sync(0xffffffffu, e));
-        const float x = pow2i(kTileShift - E);
-        s.sv[st][lane] = sc0 * x;
-        s.sv[st][lane + 32] = sc1 * x;
+        const float e0 = scale_exponent(sc0), e1 = scale_exponent(sc1);
+        const int e_top = __reduce_max_sync(0xffffffffu, static_cast<int>(fmaxf(e0, e1)));
+        s.sv[st][lane] = sc0;
+        s.sv[st][lane + 32] = sc1;
+        s.se[st][lane] = e0;
+        s.se[st][lane + 32] = e1;
         const uint32_t m0 = __ballot_sync(0xffffffffu, sl0 >= 0), m1 = __ballot_sync(0xffffffffu, sl1 >= 0);
         if (lane == 0) {
-          s.E[st] = E;
+          s.e_top[st] = static_cast<float>(e_top);
           s.live[st][0] = m0;
           s.live[st][1] = m1;
         }
@@ -617,8 +612,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     const uint32_t lane_addr = tmem + grp * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const int token = r.start + row0 + tid;
     const int pos = r.len - r.n + row0 + tid;
-    float f = 0.f, m = -INFINITY, l = 0.f;
-    int E = -200;
+    float f = 0.f, R = -INFINITY, l = 0.f;
     bool go = true;
     if (ntiles > 0) {
       absorb_tile_rows(p, H, h, r, row0, rows, live_warps, s, q_tile, half_bytes, stage0);
@@ -646,7 +640,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
         break;
       }
       tc_fence_after();
-      const int e_new = s.E[st];
       const bool nothing = k0 >= outer_hi || k0 + kTileKeys <= outer_lo;      // of this warp's rows
       const uint32_t live0 = s.live[st][0], live1 = s.live[st][1];
       const bool masked = k0 < inner_lo || k0 + kTileKeys > inner_hi || (live0 & live1) != 0xffffffffu;
@@ -705,21 +698,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
         top = fmaxf(t0, t1);
         if (!kCap && !kBias) top *= f;
       }
-      // a new reference: the first maximum of a row, one that has grown by more than 2^8, or a larger V scale
-      const bool first = m == -INFINITY;
-      const bool grown = first ? top > -INFINITY : top > m + kLazy;
-      if (__any_sync(0xffffffffu, grown) || e_new != E) {
-        const float m_new = grown ? top : m;
-        const float c = first ? 0.f : ex2(m - m_new);
-        l *= c;
-        if (j > 0 && __any_sync(0xffffffffu, (grown && !first) || e_new != E)) {
+      // top + e_top bounds what a row sees here: only where that is past a row's reference are the rows' own values looked for
+      if (__any_sync(0xffffffffu, R == -INFINITY ? top > -INFINITY : top + s.e_top[st] > R + kLazy)) {
+        float need = -INFINITY;
+        if (!nothing) {
+          const float4* se = reinterpret_cast<const float4*>(s.se[st]);
+          const float2 ff = make_float2(f, f);
+#pragma unroll
+          for (int i = 0; i < kTileKeys / 4; ++i) {
+            const float4 e = se[i];
+            const float2 a = (kCap || kBias) ? add2(x[2 * i], make_float2(e.x, e.y)) : fma2(x[2 * i], ff, make_float2(e.x, e.y));
+            const float2 b = (kCap || kBias) ? add2(x[2 * i + 1], make_float2(e.z, e.w)) : fma2(x[2 * i + 1], ff, make_float2(e.z, e.w));
+            need = max3(need, a.x, a.y);
+            need = max3(need, b.x, b.y);
+          }
+        }
+        const bool first = R == -INFINITY;
+        const bool grown = first ? need > -INFINITY : need > R + kLazy;
+        if (__any_sync(0xffffffffu, grown && !first)) {        // (so j > 0)
+          const float by = grown && !first ? ex2(R - need) : 1.f;
+          l *= by;
           go = tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
           if (!__all_sync(0xffffffffu, go)) {
             go = false;
             break;
           }
           tc_fence_after();
-          const float by = (first ? 1.f : c) * pow2i(max(E - e_new, -126));
           __syncwarp();
 #pragma unroll 1
           for (int col = 0; col < rv; col += 16) {
@@ -730,8 +734,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
             tmem_st16(lane_addr + kColO + col, v);
           }
         }
-        m = m_new;
-        E = e_new;
+        if (grown) R = need;
       }
       __syncwarp();
       if (nothing) {
@@ -742,7 +745,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
         for (int i = 0; i < kTileKeys; i += 16) tmem_st16(s_addr + i, z);
       } else {
         // exponentials in place (the unit that bounds the kernel works without a pause), then the weights
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = R == -INFINITY ? 0.f : R - kWeightShift;
         const float2 nb = make_float2(-base, -base), ff = make_float2(f, f);
         float2 sum[4];
 #pragma unroll
@@ -793,11 +796,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     go = __all_sync(0xffffffffu, go);
     tc_fence_after();
     if (go) {
-      const float back = ntiles > 0 ? (E > -200 ? pow2i(E - kTileShift) : 1.f) : 0.f;
-      const float by = p.tile_splits > 1 ? back : (l == 0.f ? 0.f : back / l);
+      const float by = p.tile_splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       const bool to_up = p.out != nullptr && p.tile_splits == 1;
       const int64_t part = static_cast<int64_t>(split) * p.num_tokens + token;
-      if (p.tile_splits > 1 && tid < rows) p.tile_ml[part * p.num_heads + h] = make_float2(m, l);
+      if (p.tile_splits > 1 && tid < rows) p.tile_ml[part * p.num_heads + h] = make_float2(R, l);
 #pragma unroll 1
       for (int c = 0; c < rv; c += 16) {
         uint32_t v[16];

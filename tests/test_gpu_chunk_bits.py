@@ -35,3 +35,66 @@ def test_error_with_cap_and_bias(news):
     scores = {"softcap": 20.0, "alibi_slopes": _slopes(2)}
     _, lat, _, _ = _want(c, **scores)
     assert rounding_ratio(_run(c, latent=True, **scores), lat) <= 1.05
+
+
+def _ratio_where(got, want, keep):
+    rows = torch.where(keep)[0]
+    return rounding_ratio(got[rows], want[rows])
+
+
+@pytest.mark.parametrize("small,large", [(1e-4, 512.0), (1e-4, 65504.0), (0.02, 65504.0)])
+@pytest.mark.parametrize("news", [[7, 3], [16, 1], [150, 40]])
+@pytest.mark.parametrize("mask", ["window", "docs", "future"])
+def test_large_scales_of_masked_keys_cost_no_bits(mask, news, small, large):
+    """V scales of the smallest and the largest size: the large ones on keys that a row does not see, in the same tiles as those
+    that it sees."""
+    c = _case(news, [70, 130], [64, 32], [48, 64], seed=23)
+    c["scale_v"][:] = small
+    scores, keep = {}, torch.ones(sum(news), dtype=torch.bool)
+    if mask == "docs":                       # every row sees its request's keys from 40 on
+        scores["key_begin"] = torch.full((sum(news),), 40, dtype=torch.int32)
+    if mask == "window":
+        scores["window"] = 30
+    for b in range(2):
+        L, n = int(c["b_seq_len"][b]), news[b]
+        rows = c["req_to_token"][int(c["b_req_idx"][b])].long()
+        if mask == "docs":
+            c["scale_v"][rows[5:40:7]] = large
+        elif mask == "window":                # keys that no row sees, and (with many rows) some that only the first rows see
+            c["scale_v"][rows[:L - n - 29:5]] = large
+            if n > 60:
+                c["scale_v"][rows[L - n + 2]] = large
+                keep[int(c["start"][b]) + 2:int(c["start"][b]) + 33] = False
+        elif n > 1:                           # the last new token, which only its own row sees
+            c["scale_v"][rows[L - 1]] = large
+            keep[int(c["start"][b]) + n - 1] = False
+    o, lat, _, _ = _want(c, **scores)
+    got = _run(c, latent=True, **scores)
+    assert torch.isfinite(got[keep].float()).all() and _ratio_where(got, lat, keep) <= 1.05
+    assert _ratio_where(_run(c, True, **scores), o, keep) <= 1.05
+
+
+@pytest.mark.parametrize("news", [[5], [140]])
+def test_large_scales_of_keys_whose_weight_is_nothing_cost_no_bits(news):
+    """The first keys are seen by every row, at distances where the bias leaves less than e^-190 of their weight: 65504 times that is
+    nothing to the others, whose scales are 1e-4."""
+    c = _case(news, [200], [64, 32], [48, 64], seed=24)
+    c["scale_v"][:] = 1e-4
+    c["scale_v"][c["req_to_token"][int(c["b_req_idx"][0]), :4].long()] = 65504.0
+    scores = {"alibi_slopes": torch.ones(2)}
+    _, lat, _, _ = _want(c, **scores)
+    assert rounding_ratio(_run(c, latent=True, **scores), lat) <= 1.05
+
+
+@pytest.mark.parametrize("news", [[5, 1], [140, 33]])
+def test_scales_of_zero(news):
+    """No V scale, or none of the first keys, has an exponent."""
+    c = _case(news, [200, 64], [64, 32], [48, 64], seed=25)
+    keep = c["scale_v"].clone()
+    c["scale_v"][:] = 0
+    assert (_run(c, latent=True) == 0).all()
+    for b in range(2):
+        rows = c["req_to_token"][int(c["b_req_idx"][b]), 60:int(c["b_seq_len"][b])].long()
+        c["scale_v"][rows] = keep[rows]
+    _, lat, _, _ = _want(c)
+    assert rounding_ratio(_run(c, latent=True), lat) <= 1.05
