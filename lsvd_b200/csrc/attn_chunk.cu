@@ -21,6 +21,7 @@
 // References, sums and accumulators are fp32.  Scales are applied in fp32 to scores and weights, never to the codes: a masked key's
 // scale, were it huge, infinite or NaN, touches nothing.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 
@@ -217,8 +218,7 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
       }
   }
   __syncthreads();                    // the rings' last stages may be written from here on
-  const float cap_log2e = p.softcap * kChunkLog2e;
-  f *= kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e;
+  f *= kChunkLog2e;
   const int lo = s.lo[g], hi = s.hi[g], pos = r.len - r.n + row0 + g;
   const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
 
@@ -284,12 +284,18 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_stream_kernel(const __
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      if (kCap) {
+        const float2 v = mul2(make_float2(x[j][0] + x[j][2], x[j][1] + x[j][3]),
+                              make_float2(s.sk[warp][8 * j + t4] * f, s.sk[warp][8 * j + t4 + 4] * f));
+        const float2 y = capped_log2(v, mul2(v, make_float2(p.cap_u, p.cap_u)), p.cap_log2e);
+        x[j][0] = y.x;
+        x[j][1] = y.y;
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int k = 8 * j + t4 + 4 * e;
         const float c = s.sk[warp][k];
-        float v = (x[j][e] + x[j][2 + e]) * (c * f);
-        if (kCap) v = capped_log2(v, cap_log2e);
+        float v = kCap ? x[j][e] : (x[j][e] + x[j][2 + e]) * (c * f);
         if (kBias) v -= slope * fabsf(static_cast<float>(pos - key0 - k));
         if (masked && (!((valid >> k) & 1u) || key0 + k < lo || key0 + k >= hi)) v = -INFINITY;
         x[j][e] = v;
@@ -602,7 +608,7 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   if (a->req_to_token_rows <= 0 || (a->req_to_token_rows > 1 && a->req_to_token_stride < a->max_len_in_batch)) return LSVD_ERR_INVALID_ARG;
   if (a->max_len_in_batch > (1 << 30)) return LSVD_ERR_UNSUPPORTED;
   if (!std::isfinite(a->softcap) || !std::isfinite(a->sm_scale) || a->softcap < 0.f || a->window < 0) return LSVD_ERR_INVALID_ARG;
-  if (a->softcap > 0.f && a->softcap < 1e-6f) return LSVD_ERR_UNSUPPORTED;      // (the scores' factor 1 / softcap has to stay in range)
+  if (a->softcap > 0.f && a->softcap < 1e-6f) return LSVD_ERR_UNSUPPORTED;      // (2 / softcap times a score has to stay in range)
   const ChunkPlan c = chunk_plan(a->batch, a->num_heads, a->num_tokens, a->max_new_in_batch, a->max_len_in_batch);
   const int64_t stream_blocks = static_cast<int64_t>(a->batch) * (c.stream_stride > kStreamRows ? 2 : 1);
   if (a->batch > 65535 || stream_blocks > 65535 || c.tiles > 65535 || (a->num_tokens + kMergeRows - 1) / kMergeRows > 65535) return LSVD_ERR_UNSUPPORTED;
@@ -642,6 +648,8 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   p.key_begin = a->key_begin;
   p.score_scale = a->sm_scale > 0.f ? a->sm_scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
   p.softcap = a->softcap;
+  p.cap_u = a->softcap > 0.f ? 2.f / a->softcap : 0.f;
+  p.cap_log2e = std::min(a->softcap * kChunkLog2e, FLT_MAX);
   p.batch = a->batch;
   p.num_heads = a->num_heads;
   p.head_dim = a->head_dim;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "devfn.cuh"
 
 namespace lsvd {
 
@@ -55,7 +56,8 @@ struct ChunkParams {
   const int32_t* b_prefix_len;
   const int32_t* key_begin;
   float score_scale;         // sm_scale
-  float softcap;
+  float softcap;             // 0: none
+  float cap_u, cap_log2e;    // 2 / softcap, softcap * log2(e)
   int32_t batch, num_heads, head_dim, max_len, num_tokens, max_new, num_slots, r2t_rows;
   int32_t causal, window, head_major, sum_rv;
   int32_t q_vec, up_k_vec;   // rows of q / up_k can be read in 8-byte pieces
@@ -123,10 +125,20 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// cap * tanh(x / cap) * log2(e) of u = x * 2 log2(e) / cap: tanh(y) = 1 - 2 / (1 + e^(2y)), off by a few 2^-24 of the cap
-// (the hardware's tanh is off by 2^-11 of it, half a unit of a score at a cap of 1000, 2 % of a weight at 50).
-__device__ __forceinline__ float capped_log2(float u, float cap_log2e) {
-  return fmaf(__fdividef(-2.f, 1.f + ex2(u)), cap_log2e, cap_log2e);
+// cap * tanh(x / cap) in units of log2, of v = x * log2(e), by u = 2 v / cap (so e^(2 x / cap) = 2^u).  For |x / cap| below a quarter the
+// series of tanh(y) / y up to y^6 (what follows is below 2^-21 of it): v stands as a factor, so a cap far above the scores leaves
+// them as they are.  Above it 1 - 2 / (1 + 2^u), whose rounding, 2^-22 of the cap, is below 2^-19 of such a score.
+// (The hardware's tanh is off by 2^-11 of the cap, half a unit of a score at a cap of 1000, 2 % of a weight at 50.)
+constexpr float kCapSeries = 0.5f * kChunkLog2e;      // u at x / cap = 1/4
+__device__ __forceinline__ float2 capped_series(float2 v, float2 u) {
+  auto both = [](float c) { return make_float2(c, c); };
+  const float2 s = mul2(u, u);
+  return mul2(v, fma2(fma2(fma2(s, both(-9.35214345e-5f), both(1.92362582e-3f)), s, both(-4.00377512e-2f)), s, both(1.f)));
+}
+__device__ __forceinline__ float2 capped_log2(float2 v, float2 u, float cap_log2e) {
+  const float2 y = capped_series(v, u);
+  return make_float2(fabsf(u.x) < kCapSeries ? y.x : fmaf(__fdividef(-2.f, 1.f + ex2(u.x)), cap_log2e, cap_log2e),
+                     fabsf(u.y) < kCapSeries ? y.y : fmaf(__fdividef(-2.f, 1.f + ex2(u.y)), cap_log2e, cap_log2e));
 }
 
 // Exponent e with 2^e <= x < 2^(e+1) for a positive normal x (0 for what is not positive and finite).

@@ -618,12 +618,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       absorb_tile_rows(p, H, h, r, row0, rows, live_warps, s, q_tile, half_bytes, stage0);
       __syncwarp();
       f = s.scale[tid];
-      f = fmaxf(f * p.score_scale * (kCap ? 2.f * kChunkLog2e / p.softcap : kChunkLog2e), 1e-37f);
+      f = fmaxf(f * p.score_scale * kChunkLog2e, 1e-37f);
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.q_full[grp]);
     }
-    const float cap_log2e = p.softcap * kChunkLog2e;
     const float slope = kBias ? p.alibi_slopes[h] * kChunkLog2e : 0.f;
     // keys that every row of the warp sees
     const int inner_lo = __reduce_max_sync(0xffffffffu, tid < rows ? keys.lo : 0);
@@ -661,20 +660,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
           }
         }
         if (kCap || kBias) {
+          const float2 ff = make_float2(f, f);
+#pragma unroll
+          for (int i = 0; i < kTileKeys / 2; ++i) x[i] = mul2(x[i], ff);
+        }
+        if (kCap) {
+          const float2 cu = make_float2(p.cap_u, p.cap_u);
+          float far = 0.f;
+#pragma unroll
+          for (int i = 0; i < kTileKeys / 2; ++i) far = max3(far, fabsf(x[i].x), fabsf(x[i].y));
+          if (__any_sync(0xffffffffu, far * p.cap_u >= kCapSeries)) {
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 2; ++i) x[i] = capped_log2(x[i], mul2(x[i], cu), p.cap_log2e);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 2; ++i) x[i] = capped_series(x[i], mul2(x[i], cu));
+          }
+        }
+        if (kBias) {
           const float away = static_cast<float>(pos - k0);
 #pragma unroll
-          for (int i = 0; i < kTileKeys / 2; ++i) {
-            float a = x[i].x * f, b = x[i].y * f;
-            if (kCap) {
-              a = capped_log2(a, cap_log2e);
-              b = capped_log2(b, cap_log2e);
-            }
-            if (kBias) {
-              a = fmaf(-slope, fabsf(away - static_cast<float>(2 * i)), a);
-              b = fmaf(-slope, fabsf(away - static_cast<float>(2 * i + 1)), b);
-            }
-            x[i] = make_float2(a, b);
-          }
+          for (int i = 0; i < kTileKeys / 2; ++i)
+            x[i] = make_float2(fmaf(-slope, fabsf(away - static_cast<float>(2 * i)), x[i].x),
+                               fmaf(-slope, fabsf(away - static_cast<float>(2 * i + 1)), x[i].y));
         }
         if (masked) {
           const int a = min(max(keys.lo - k0, 0), 64), b = min(max(keys.hi - k0, 0), 64);

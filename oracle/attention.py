@@ -207,7 +207,7 @@ def chunk_absorb(q16, cache_k, scale_k, cache_v, scale_v, up_k16, up_v16, k_off,
     o = B_v^T o_lat.  Returns (o [T, H, D], o_lat [T, sum r_v], their bounds); rows of no request are NaN.
 
     The bounds follow from the kernels' roundings, each half a step: the absorbed query in fp16 (2^-11 of every term of a
-    score: dx), fp32 arithmetic on scores (2^-21 of the largest score or bias, or of the cap), weights p s_v in fp16 (2^-11 of
+    score: dx), fp32 arithmetic on scores (2^-19 of the largest score, capped, or bias, whatever the cap), weights p s_v in fp16 (2^-11 of
     every term), sums in fp32 (2^-20), the result in fp16 (2^-11, or half a step of 2^-24 below the normal range).  A score
     off by dx changes a weight by e^dx and the sum of weights by as much: 2 dx of every term.
     """
@@ -241,13 +241,13 @@ def chunk_absorb(q16, cache_k, scale_k, cache_v, scale_v, up_k16, up_v16, k_off,
             big = x.abs()
             if softcap > 0:
                 x = softcap * torch.tanh(x / softcap)
-                big = big.clamp_min(softcap)
+                big = x.abs()
             if slopes is not None:
                 bias = float(slopes[h]) * (i - t).abs().double()
                 x = x - bias
                 big = torch.maximum(big, bias)
             none = torch.zeros((), dtype=torch.float64)
-            dx = torch.where(sees, dx + 2.0 ** -21 * big, none).amax(1, keepdim=True) if L else torch.zeros(n, 1, dtype=torch.float64)
+            dx = torch.where(sees, dx + 2.0 ** -19 * big, none).amax(1, keepdim=True) if L else torch.zeros(n, 1, dtype=torch.float64)
             x = x.masked_fill(~sees, float("-inf"))
             if L:
                 x = x - x.amax(1, keepdim=True).clamp_min(-1e300)

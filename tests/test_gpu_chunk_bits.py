@@ -98,3 +98,15 @@ def test_scales_of_zero(news):
         c["scale_v"][rows] = keep[rows]
     _, lat, _, _ = _want(c)
     assert rounding_ratio(_run(c, latent=True), lat) <= 1.05
+
+
+@pytest.mark.parametrize("cap", [1e-6, 0.5, 30.0, 1e3, 1e4, 1e6, 1e8, 1e30, 3e38])
+@pytest.mark.parametrize("news", [[5, 2], [140, 20]])
+def test_caps_of_any_size(news, cap):
+    """A capped score is off by 2^-19 of itself, never of the cap: one far above the scores changes nothing."""
+    c = _case(news, [300, 64], [64, 32], [48, 64], seed=26, scale=6.0)
+    _, lat, _, _ = _want(c, softcap=cap)
+    assert rounding_ratio(_run(c, latent=True, softcap=cap), lat) <= 1.05
+    if cap >= 1e8:
+        _, lat, _, _ = _want(c)
+        assert rounding_ratio(_run(c, latent=True, softcap=cap), lat) <= 1.05
