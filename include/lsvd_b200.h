@@ -222,8 +222,10 @@ typedef struct lsvd_chunk_maps_args {
   int32_t* req_to_token;         /* device int32 [table_rows][req_to_token_stride], max_len columns used            */
   int64_t req_to_token_stride;
   int32_t max_len, rebuild;
-  const int32_t* free_pages;     /* device int32 [num_free], or NULL: block_table already lists every page          */
-  const int32_t* free_head;      /* device int32 [1]: entries of free_pages taken so far (NULL without free_pages)  */
+  const int32_t* free_pages;     /* device int32 [num_free]; may be NULL where num_free is 0                        */
+  const int32_t* free_head;      /* device int32 [1]: entries of free_pages taken so far, or NULL: there is no free */
+                                 /* list, block_table already lists every page.  (A list of no entries is one that  */
+                                 /* has run out, not a missing one.)                                                */
   int32_t num_free;
   int32_t* free_head_out;        /* device int32 [1]                                                                */
   int32_t* b_start_loc;          /* device int32 [batch + 1]                                                        */

@@ -55,8 +55,8 @@ def chunk_maps(b_req_idx, b_ready_cache_len, b_new_len, block_table, page_size: 
 
     Entry b of the batch is row ``b_req_idx[b]`` of the tables, holds ``b_ready_cache_len[b]`` tokens and gets
     ``b_new_len[b]`` more.  Pages of ``page_size`` slots that it needs beyond the ones it has come from
-    ``free_pages[free_head:]`` in batch order and are entered into ``block_table [rows, max_blocks]`` (without a free list the
-    table lists every page already); ``req_to_token [rows, width]`` gets the slots of the new positions -- of all positions
+    ``free_pages[free_head:]`` in batch order and are entered into ``block_table [rows, max_blocks]`` (without a free list,
+    ``free_pages`` None, the table lists every page already; a free list of no entries has run out); ``req_to_token [rows, width]`` gets the slots of the new positions -- of all positions
     with ``rebuild``, for pages that were taken over from elsewhere.  All tensors are int32 on one device; ``num_tokens`` is
     the capacity of the token maps and ``num_slots`` the number of cache rows.  ``out`` receives the results;
     ``out.b_seq_len`` may be ``b_ready_cache_len`` and ``out.free_head`` may be ``free_head``, so that a captured step

@@ -104,7 +104,8 @@ __global__ void __launch_bounds__(kMapsThreads) chunk_maps_kernel(const __grid_c
   s.key = s.count + B;
   s.first = s.key + hash_size;
   s.hash_mask = hash_size - 1;
-  const int32_t head = p.free_pages != nullptr ? *p.free_head : 0;
+  const bool paged = p.free_head != nullptr;       // (a free list of no entries has no address)
+  const int32_t head = paged ? *p.free_head : 0;
   const bool head_ok = head >= 0 && head <= p.num_free;
   if (threadIdx.x == 0) taken_end = head;
   for (int i = threadIdx.x; i < hash_size; i += kMapsThreads) {
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kMapsThreads) chunk_maps_kernel(const __grid_c
       uint32_t at = (static_cast<uint32_t>(row[i]) * 2654435761u) >> 7;
       while (s.key[at & s.hash_mask] != row[i]) ++at;      // it was entered above
       if (s.first[at & s.hash_mask] != b) ok[i] = false;
-      if (ok[i] && p.free_pages != nullptr) v[i] = pages_of(ready[i] + add[i], P) - pages_of(ready[i], P);
+      if (ok[i] && paged) v[i] = pages_of(ready[i] + add[i], P) - pages_of(ready[i], P);
     }
   }
   int32_t need[kMapsPer];
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(kMapsThreads) chunk_maps_kernel(const __grid_c
     }
     if (threadIdx.x == 0) {
       p.b_start_loc[B] = static_cast<int32_t>(min(total_new, static_cast<int64_t>(p.num_tokens)));
-      if (p.free_pages != nullptr) *p.free_head_out = taken_end;
+      if (paged) *p.free_head_out = taken_end;
     }
     if (bad) report_status(p.status_word, LSVD_ERR_BOUNDS);
   }
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(kMapsThreads) chunk_maps_kernel(const __grid_c
   };
   auto slot_of = [&](int b, int pos) {
     const int block = pos / P;
-    const int have = p.free_pages != nullptr ? pages_of(s.ready[b], P) : 0x7fffffff;
+    const int have = paged ? pages_of(s.ready[b], P) : 0x7fffffff;
     const int page = page_of(b, block, have);
     if (page < 0 || (static_cast<int64_t>(page) + 1) * P > p.num_slots) {
       outside = true;
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kMapsThreads) chunk_maps_kernel(const __grid_c
     p.mem_index[t] = slot;
     p.position_ids[t] = pos;
   }
-  if (p.free_pages != nullptr) {                 // the new pages' columns of the block table
+  if (paged) {                                   // the new pages' columns of the block table
     const int pages = taken_end - head;          // (a refused entry's pages lie behind taken_end)
     for (int64_t j = tid; j < pages; j += step) {
       const int b = owner_of(s.nscan, B, static_cast<int32_t>(j));
@@ -278,7 +279,8 @@ extern "C" int lsvd_chunk_maps(const lsvd_chunk_maps_args* a, void* stream) {
   if (!a->b_req_idx || !a->b_ready_cache_len || !a->b_new_len || !a->block_table || !a->req_to_token || !a->b_start_loc ||
       !a->b_seq_len || (a->num_tokens > 0 && (!a->mem_index || !a->position_ids)))
     return LSVD_ERR_INVALID_ARG;
-  if (a->free_pages != nullptr && (!a->free_head || !a->free_head_out || a->num_free < 0)) return LSVD_ERR_INVALID_ARG;
+  if (a->free_pages != nullptr && !a->free_head) return LSVD_ERR_INVALID_ARG;
+  if (a->free_head != nullptr && (!a->free_head_out || a->num_free < 0 || (a->num_free > 0 && !a->free_pages))) return LSVD_ERR_INVALID_ARG;
   if (a->table_rows > 1 && (a->block_table_stride < a->max_blocks || a->req_to_token_stride < a->max_len)) return LSVD_ERR_INVALID_ARG;
   const void* words[] = {a->b_req_idx, a->b_ready_cache_len, a->b_new_len, a->block_table, a->req_to_token, a->free_pages,
                          a->free_head, a->free_head_out, a->b_start_loc, a->b_seq_len, a->mem_index, a->position_ids};

@@ -1,0 +1,18 @@
+"""Steps of several new tokens per request, without a GPU: refusals of the entry points, and what the oracle says of requests that a
+step cannot take."""
+import ctypes as C
+
+import pytest
+
+from lsvd_b200 import _lib
+from test_chunk_cpu import _maps_args, lib      # noqa: F401  (a fixture)
+
+
+def test_maps_tell_an_empty_free_list_from_a_missing_one(lib):      # noqa: F811
+    """A list of no entries may have no address; then its head still has to be there, and its length is zero."""
+    a = _maps_args()
+    a.free_pages = None                                   # four entries, no address
+    assert lib.lsvd_chunk_maps(C.byref(a), None) == _lib.ERR_INVALID_ARG
+    a = _maps_args()
+    a.free_pages, a.num_free, a.free_head_out = None, 0, None
+    assert lib.lsvd_chunk_maps(C.byref(a), None) == _lib.ERR_INVALID_ARG
