@@ -294,6 +294,8 @@ typedef struct lsvd_attn_chunk_args {
   const float* alibi_slopes;     /* device fp32 [num_heads] or NULL                                                */
   const int32_t* b_prefix_len;   /* device int32 [batch] or NULL                                                   */
   const int32_t* key_begin;      /* device int32 [num_tokens] or NULL                                              */
+  const int32_t* mem_index;      /* device int32 [num_tokens] or NULL: cache slots of the rows' tokens, as lsvd_chunk_maps     */
+                                 /* gives them.  A row whose token has none (negative: its request was refused) sees nothing.  */
 } lsvd_attn_chunk_args;
 /* Bytes of workspace for this problem on the current device (0: bad sizes). */
 size_t lsvd_attn_chunk_workspace_bytes(int32_t batch, int32_t num_heads, int32_t sum_rank_v, int32_t num_tokens,

@@ -95,6 +95,7 @@ class AttnChunkArgs(C.Structure):
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status_word", C.c_void_p),
         ("cache_layout", C.c_int32), ("req_to_token_rows", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32),
         ("softcap", C.c_float), ("alibi_slopes", C.c_void_p), ("b_prefix_len", C.c_void_p), ("key_begin", C.c_void_p),
+        ("mem_index", C.c_void_p),
     ]
 
 

@@ -191,7 +191,8 @@ def chunk_attention_int8_latent_absorb(
       * ``causal=False``: every key of the request (with a window: ``|pos - t| < window``).
 
     ``softcap > 0`` replaces a score x by ``softcap * tanh(x / softcap)``; ``alibi_slopes [H]`` fp32 subtracts
-    ``slope * |pos - t|`` after that.  Returns ``out [num_tokens, H, D]`` fp16 when ``up_v`` is given, otherwise the latent
+    ``slope * |pos - t|`` after that.  A token without a cache slot (``state.mem_index`` negative: ``chunk_maps`` has refused its
+    request) sees nothing.  Returns ``out [num_tokens, H, D]`` fp16 when ``up_v`` is given, otherwise the latent
     result ``[num_tokens, sum r_v]``.  Rows of tokens that see nothing are zero; rows behind the last token are not written.
     """
     _require_cuda(q, cache_latent_k, cache_latent_v, up_k, up_v, alibi_slopes, b_prefix_len, key_begin)
@@ -279,6 +280,11 @@ def chunk_attention_int8_latent_absorb(
         a.alibi_slopes = alibi_slopes.data_ptr()
     if b_prefix_len is not None:
         a.b_prefix_len = _i32("b_prefix_len", b_prefix_len, B, device=dev)
+    slots = getattr(state, "mem_index", None)
+    if slots is not None:
+        if slots.numel() < T:
+            raise ValueError(f"state.mem_index has {slots.numel()} slots for {T} rows")
+        a.mem_index = _i32("state.mem_index", slots, device=dev)
     if key_begin is not None:
         a.key_begin = _i32("key_begin", key_begin, T, device=dev)
     with torch.cuda.device(dev):       # the workspace is sized, and the kernels run, on the tensors' device

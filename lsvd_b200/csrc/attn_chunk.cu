@@ -601,7 +601,7 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   for (const void* x : halves)
     if (!aligned(x, 2)) return LSVD_ERR_INVALID_ARG;
   const void* words[] = {a->req_to_token, a->b_req_idx, a->b_seq_len, a->b_start_loc, a->alibi_slopes, a->b_prefix_len, a->key_begin,
-                         a->status_word};
+                         a->mem_index, a->status_word};
   for (const void* x : words)
     if (!aligned(x, 4)) return LSVD_ERR_INVALID_ARG;
   if (a->up_k_row_stride < a->head_dim || (a->out != nullptr && a->up_v_row_stride < a->head_dim)) return LSVD_ERR_INVALID_ARG;
@@ -646,6 +646,7 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   p.alibi_slopes = a->alibi_slopes;
   p.b_prefix_len = a->b_prefix_len;
   p.key_begin = a->key_begin;
+  p.mem_index = a->mem_index;
   p.score_scale = a->sm_scale > 0.f ? a->sm_scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
   p.softcap = a->softcap;
   p.cap_u = a->softcap > 0.f ? 2.f / a->softcap : 0.f;

@@ -55,6 +55,7 @@ struct ChunkParams {
   const float* alibi_slopes;
   const int32_t* b_prefix_len;
   const int32_t* key_begin;
+  const int32_t* mem_index;
   float score_scale;         // sm_scale
   float softcap;             // 0: none
   float cap_u, cap_log2e;    // 2 / softcap, softcap * log2(e)
@@ -115,6 +116,7 @@ __device__ __forceinline__ KeyRange visible_keys(const ChunkParams& p, const Chu
     if (!p.causal) k.hi = static_cast<int>(min(static_cast<int64_t>(r.len), static_cast<int64_t>(pos) + p.window));
   }
   if (p.key_begin != nullptr) k.lo = max(k.lo, p.key_begin[r.start + i]);
+  if (p.mem_index != nullptr && p.mem_index[r.start + i] < 0) k.hi = 0;      // a token that was refused is not in the cache
   if (k.hi <= k.lo) k.lo = k.hi = 0;
   return k;
 }

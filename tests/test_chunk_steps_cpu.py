@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 from lsvd_b200 import _lib
-from test_chunk_cpu import _maps_args, lib      # noqa: F401  (a fixture)
+from test_chunk_cpu import _chunk_args, _maps_args, lib      # noqa: F401  (a fixture)
 
 
 def test_maps_tell_an_empty_free_list_from_a_missing_one(lib):      # noqa: F811
@@ -16,3 +16,9 @@ def test_maps_tell_an_empty_free_list_from_a_missing_one(lib):      # noqa: F811
     a = _maps_args()
     a.free_pages, a.num_free, a.free_head_out = None, 0, None
     assert lib.lsvd_chunk_maps(C.byref(a), None) == _lib.ERR_INVALID_ARG
+
+
+def test_attention_refuses_misaligned_slots(lib):      # noqa: F811
+    a = _chunk_args()
+    a.mem_index = 4097
+    assert lib.lsvd_attn_chunk(C.byref(a), None) == _lib.ERR_INVALID_ARG

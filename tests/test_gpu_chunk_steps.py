@@ -3,7 +3,8 @@ tokens -- through the slot maps, the attention and the layer."""
 import pytest
 import torch
 
-from lsvd_b200 import _lib
+from lsvd_b200 import ChunkState, LatentCacheLayout, LatentDecodeAttention, _lib
+from oracle import attention as oattn
 from test_gpu_chunk import _check_maps, _maps_case, _run_maps
 
 pytestmark = pytest.mark.gpu
@@ -21,3 +22,51 @@ def test_a_free_list_without_entries_has_run_out(in_place):
     _check_maps(c, refused=[0, 2, 3], in_place=in_place)
     got, table, _, status = _run_maps(c)
     assert status == _lib.ERR_BOUNDS and table == c["table"] and got[4] == [3]
+
+
+class Steps:
+    """A paged state over a cache of random latents, with the oracle's copy of it."""
+
+    def __init__(self, rows, num_pages, max_new, page=16, max_len=400, max_tokens=300):
+        self.ranks, self.D = ([64, 32], [48, 64]), 64
+        self.lay, self.flat = LatentCacheLayout(*self.ranks, head_major=True), LatentCacheLayout(*self.ranks)
+        self.g = torch.Generator().manual_seed(31)
+        self.state = ChunkState.paged(rows=rows, max_len_in_batch=max_len, max_tokens=max_tokens, max_new_in_batch=max_new,
+                                      num_pages=num_pages, page_size=page)
+        slots = num_pages * page
+        self.cache, self.plain = self.lay.alloc(slots, DEV), self.flat.alloc(slots, "cpu")
+        up = lambda n: (torch.randn(n, self.D, generator=self.g) / 8).half()
+        self.up = up(self.lay.sum_k), up(self.lay.sum_v)
+        self.attn = LatentDecodeAttention(self.lay, self.D, *[u.to(DEV) for u in self.up])
+
+    def step(self, news, **kw):
+        """(output with 77 where nothing was written, the oracle's, its bound) of a step; the oracle goes by the state's lengths."""
+        T = sum(news)
+        make = lambda w: torch.randn(T, w, generator=self.g).half()
+        lk, lv, q = make(self.lay.sum_k), make(self.lay.sum_v), make(2 * self.D).view(T, 2, self.D)
+        self.state.begin(torch.tensor(news, dtype=torch.int32, device=DEV), **kw)
+        out = torch.full((T, 2, self.D), 77.0, dtype=torch.float16, device=DEV)
+        self.attn.forward_chunk(q.to(DEV), *self.cache, self.state, latent_k=lk.to(DEV), latent_v=lv.to(DEV), out=out)
+        torch.cuda.synchronize()
+        st, mem = self.state, self.state.mem_index.cpu()[:T]
+        ok = mem >= 0
+        oattn.cache_append(lk[ok], mem[ok], self.flat.k_off, self.plain[0], self.plain[1])
+        oattn.cache_append(lv[ok], mem[ok], self.flat.v_off, self.plain[2], self.plain[3])
+        o, _, tol, _ = oattn.chunk_absorb(q, *self.plain, *self.up, self.flat.k_off, self.flat.v_off,
+                                          st.req_manager.req_to_token_indexs.cpu(), st.b_req_idx.cpu(), st.b_seq_len.cpu(), st.b_start_loc.cpu())
+        return out.cpu().double(), o, tol
+
+
+@pytest.mark.parametrize("second", [[2, 8, 1], [2, 40, 1]])
+def test_requests_that_find_no_pages_get_zeros(second):
+    """The first step takes all five pages of 16; in the second one the second request needs another."""
+    s = Steps(rows=3, num_pages=5, max_new=64)
+    s.step([20, 9, 30])
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got, want, tol = s.step(second, status_word=status)
+    a, e = second[0], second[0] + second[1]
+    assert status.item() == _lib.ERR_BOUNDS and s.state.b_seq_len.tolist() == [22, 9, 31]
+    assert (s.state.mem_index.cpu()[a:e] == -1).all()
+    assert (got[a:e] == 0).all()
+    got[a:e], want[a:e] = 0, 0
+    assert ((got - want).abs() <= tol).all()
