@@ -205,8 +205,8 @@ int lsvd_attn_decode_static(const lsvd_attn_decode_args* args, void* stream);
  * Entries of mem_index / position_ids behind the last token, up to num_tokens, become -1 / 0.  b_seq_len may be the array
  * b_ready_cache_len and free_head_out the word free_head (a captured step then advances the lengths at every replay).
  * An entry is refused -- it takes no page, its length stays `ready`, its tokens get slot -1 and position 0, LSVD_ERR_BOUNDS
- * is reported -- when its row, a length or its tokens do not fit the tables or num_tokens, when an earlier entry adds tokens to the same
- * row, or when the free pages run out (with every later entry that needs a page).  A page outside the cache gives slot -1.
+ * is reported -- when its row, a length or its tokens do not fit the tables, num_tokens or max_new_in_batch, when an earlier entry
+ * adds tokens to the same row, or when the free pages run out (with every later entry that needs a page).  A page outside the cache gives slot -1.
  * ------------------------------------------------------------------------------------------- */
 #define LSVD_MAX_BATCH 4096     /* entries of a batch in lsvd_chunk_maps */
 typedef struct lsvd_chunk_maps_args {
@@ -233,6 +233,7 @@ typedef struct lsvd_chunk_maps_args {
   int32_t* mem_index;            /* device int32 [num_tokens]                                                       */
   int32_t* position_ids;         /* device int32 [num_tokens]                                                       */
   int32_t* status_word;          /* device int32 or NULL                                                            */
+  int32_t max_new_in_batch;      /* upper bound of the new tokens of one entry (the step's attention has the same); 0: none   */
 } lsvd_chunk_maps_args;
 int lsvd_chunk_maps(const lsvd_chunk_maps_args* args, void* stream);
 

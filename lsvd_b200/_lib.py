@@ -72,7 +72,7 @@ class ChunkMapsArgs(C.Structure):
         ("req_to_token", C.c_void_p), ("req_to_token_stride", C.c_int64), ("max_len", C.c_int32), ("rebuild", C.c_int32),
         ("free_pages", C.c_void_p), ("free_head", C.c_void_p), ("num_free", C.c_int32), ("free_head_out", C.c_void_p),
         ("b_start_loc", C.c_void_p), ("b_seq_len", C.c_void_p), ("mem_index", C.c_void_p), ("position_ids", C.c_void_p),
-        ("status_word", C.c_void_p),
+        ("status_word", C.c_void_p), ("max_new_in_batch", C.c_int32),
     ]
 
 

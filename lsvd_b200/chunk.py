@@ -50,7 +50,7 @@ def _table(name, t, device):
 @torch.no_grad()
 def chunk_maps(b_req_idx, b_ready_cache_len, b_new_len, block_table, page_size: int, req_to_token, num_tokens: int, num_slots: int,
                free_pages=None, free_head=None, rebuild: bool = False, out: Optional[ChunkMaps] = None,
-               alloc_tensor_func=torch.empty, status_word=None) -> ChunkMaps:
+               alloc_tensor_func=torch.empty, status_word=None, max_new_in_batch: int = 0) -> ChunkMaps:
     """Slots and positions of the tokens that a step adds, from the request lengths, in one launch.
 
     Entry b of the batch is row ``b_req_idx[b]`` of the tables, holds ``b_ready_cache_len[b]`` tokens and gets
@@ -60,15 +60,15 @@ def chunk_maps(b_req_idx, b_ready_cache_len, b_new_len, block_table, page_size: 
     with ``rebuild``, for pages that were taken over from elsewhere.  All tensors are int32 on one device; ``num_tokens`` is
     the capacity of the token maps and ``num_slots`` the number of cache rows.  ``out`` receives the results;
     ``out.b_seq_len`` may be ``b_ready_cache_len`` and ``out.free_head`` may be ``free_head``, so that a captured step
-    advances the lengths at every replay.  An entry that does not fit (its row, its length, ``num_tokens``, the free pages,
-    or a row that an earlier entry adds tokens to) gets no page and slot -1 for its tokens, its length stays, and
+    advances the lengths at every replay.  An entry that does not fit (its row, its length, ``num_tokens``, more new tokens
+    than a ``max_new_in_batch`` above zero, the free pages, or a row that an earlier entry adds tokens to) gets no page and slot -1 for its tokens, its length stays, and
     ``LSVD_ERR_BOUNDS`` is written to ``status_word``.
     """
     _require_cuda(b_req_idx, b_ready_cache_len, b_new_len, block_table, req_to_token, free_pages, free_head)
     dev, B = b_req_idx.device, b_req_idx.numel()
     if (free_pages is None) != (free_head is None):
         raise ValueError("free_pages and free_head go together")
-    if B == 0 or num_tokens < 0:
+    if B == 0 or num_tokens < 0 or max_new_in_batch < 0:
         raise ValueError("an empty batch or a negative number of tokens")
     if block_table.shape[0] != req_to_token.shape[0]:
         raise ValueError("block_table and req_to_token must have the same number of rows")
@@ -83,7 +83,7 @@ def chunk_maps(b_req_idx, b_ready_cache_len, b_new_len, block_table, page_size: 
     a.block_table, a.block_table_stride = _table("block_table", block_table, dev)
     a.req_to_token, a.req_to_token_stride = _table("req_to_token", req_to_token, dev)
     a.max_blocks, a.table_rows, a.max_len = block_table.shape[1], block_table.shape[0], req_to_token.shape[1]
-    a.rebuild = int(rebuild)
+    a.rebuild, a.max_new_in_batch = int(rebuild), int(max_new_in_batch)
     if free_pages is not None:
         a.free_pages, a.num_free = _i32("free_pages", free_pages, free_pages.numel(), device=dev), free_pages.numel()
         a.free_head = _i32("free_head", free_head, 1, device=dev)
@@ -121,7 +121,8 @@ class ChunkState:
     def paged(cls, rows: int, max_len_in_batch: int, max_tokens: int, max_new_in_batch: int, num_pages: int, page_size: int,
               b_req_idx=None, device="cuda"):
         """An empty paged state: ``rows`` requests of up to ``max_len_in_batch`` tokens, ``num_pages`` free pages of
-        ``page_size`` slots, steps of up to ``max_tokens`` tokens.  ``begin`` starts a step."""
+        ``page_size`` slots, steps of up to ``max_tokens`` tokens, ``max_new_in_batch`` of them for one request.  ``begin`` starts
+        a step."""
         i32 = dict(dtype=torch.int32, device=device)
         req = torch.arange(rows, **i32) if b_req_idx is None else b_req_idx.to(**i32).contiguous()
         blocks = -(-max_len_in_batch // page_size)
@@ -142,7 +143,7 @@ class ChunkState:
         chunk_maps(self.b_req_idx, self.b_seq_len, b_new_len, g["block_table"], g["page_size"], self.req_manager.req_to_token_indexs,
                    self.mem_index.numel(), g["num_slots"], g["free_pages"], g["free_head"], rebuild,
                    ChunkMaps(self.b_start_loc, self.b_seq_len, self.mem_index, self.position_ids, g["free_head"]),
-                   status_word=status_word)
+                   status_word=status_word, max_new_in_batch=self.max_new_in_batch)
         return self
 
 

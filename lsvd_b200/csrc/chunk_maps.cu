@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kMapsThreads) chunk_maps_kernel(const __grid_c
       add[i] = p.b_new_len[b];
       const int64_t seq = static_cast<int64_t>(ready[i]) + add[i];
       ok[i] = row[i] >= 0 && row[i] < p.table_rows && ready[i] >= 0 && add[i] >= 0 && seq <= p.max_len &&
-              seq <= static_cast<int64_t>(p.max_blocks) * P;
+              seq <= static_cast<int64_t>(p.max_blocks) * P && (p.max_new_in_batch == 0 || add[i] <= p.max_new_in_batch);
       v[i] = add[i] > 0 ? add[i] : 0;
     }
   }
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kMapsThreads) chunk_maps_kernel(const __grid_c
 
 extern "C" int lsvd_chunk_maps(const lsvd_chunk_maps_args* a, void* stream) {
   using namespace lsvd;
-  if (a == nullptr || a->batch <= 0 || a->page_size <= 0 || a->num_tokens < 0 || a->num_slots <= 0) return LSVD_ERR_INVALID_ARG;
+  if (a == nullptr || a->batch <= 0 || a->page_size <= 0 || a->num_tokens < 0 || a->num_slots <= 0 || a->max_new_in_batch < 0) return LSVD_ERR_INVALID_ARG;
   if (a->max_blocks <= 0 || a->table_rows <= 0 || a->max_len <= 0) return LSVD_ERR_INVALID_ARG;
   if (!a->b_req_idx || !a->b_ready_cache_len || !a->b_new_len || !a->block_table || !a->req_to_token || !a->b_start_loc ||
       !a->b_seq_len || (a->num_tokens > 0 && (!a->mem_index || !a->position_ids)))

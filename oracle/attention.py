@@ -161,11 +161,11 @@ def decode_rope_recon(q16, cache_k, scale_k, cache_v, scale_v, wk_q, wk_scale16,
     return out.half()
 
 
-def chunk_maps(req, ready, new, table, page, r2t, num_tokens, num_slots, free=None, head=0, rebuild=False):
+def chunk_maps(req, ready, new, table, page, r2t, num_tokens, num_slots, free=None, head=0, rebuild=False, max_new=0):
     """Slots of a step's new tokens, entry by entry (lists of Python integers; ``table`` and ``r2t`` are changed in place).
 
     Returns (start, seq, mem_index, position_ids, head, refused) with ``refused`` the entries that got nothing: their row or
-    length does not fit the tables, their tokens do not fit ``num_tokens``, an earlier entry adds tokens to the same row, or
+    length does not fit the tables, their tokens do not fit ``num_tokens`` or are more than ``max_new`` (0: any), an earlier entry adds tokens to the same row, or
     the free pages have run out.
     """
     up = lambda tokens: -(-tokens // page)
@@ -176,7 +176,7 @@ def chunk_maps(req, ready, new, table, page, r2t, num_tokens, num_slots, free=No
         first = start[-1]
         start.append(first + max(n, 0))
         ok = 0 <= row < len(table) and old >= 0 and n >= 0 and old + n <= len(r2t[0]) and old + n <= len(table[0]) * page
-        ok = ok and start[-1] <= num_tokens
+        ok = ok and start[-1] <= num_tokens and (max_new == 0 or n <= max_new)
         if ok and n > 0:
             ok = row not in seen
             seen.add(row)

@@ -5,6 +5,7 @@ import ctypes as C
 import pytest
 
 from lsvd_b200 import _lib
+from oracle import attention
 from test_chunk_cpu import _chunk_args, _maps_args, lib      # noqa: F401  (a fixture)
 
 
@@ -22,3 +23,15 @@ def test_attention_refuses_misaligned_slots(lib):      # noqa: F811
     a = _chunk_args()
     a.mem_index = 4097
     assert lib.lsvd_attn_chunk(C.byref(a), None) == _lib.ERR_INVALID_ARG
+
+
+def test_maps_refuse_a_negative_bound(lib):      # noqa: F811
+    a = _maps_args()
+    a.max_new_in_batch = -1
+    assert lib.lsvd_chunk_maps(C.byref(a), None) == _lib.ERR_INVALID_ARG
+
+
+def test_oracle_maps_refuse_more_tokens_than_the_bound():
+    table, r2t = [[0, -1], [1, -1]], [[-1] * 32 for _ in range(2)]
+    start, seq, mem, pos, head, refused = attention.chunk_maps([0, 1], [3, 3], [5, 4], table, 16, r2t, 9, 64, [2, 3], 0, max_new=4)
+    assert refused == [0] and seq == [3, 7] and start == [0, 5, 9] and mem == [-1] * 5 + [19, 20, 21, 22] and head == 0

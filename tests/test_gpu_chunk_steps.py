@@ -70,3 +70,20 @@ def test_requests_that_find_no_pages_get_zeros(second):
     assert (got[a:e] == 0).all()
     got[a:e], want[a:e] = 0, 0
     assert ((got - want).abs() <= tol).all()
+
+
+def test_more_new_tokens_than_the_bound_take_no_page():
+    """The attention skips a request of more than max_new_in_batch tokens; the maps refuse it before it takes pages or grows."""
+    s = Steps(rows=3, num_pages=12, max_new=20)
+    s.step([20, 9, 12])
+    taken = s.state.pages["free_head"].item()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got, want, tol = s.step([3, 40, 1], status_word=status)
+    assert status.item() == _lib.ERR_BOUNDS and s.state.b_seq_len.tolist() == [23, 9, 13]
+    assert s.state.pages["free_head"].item() == taken
+    assert (s.state.mem_index.cpu()[3:43] == -1).all() and (s.state.req_manager.req_to_token_indexs[1, 9:] == -1).all()
+    assert (got[3:43] == 77.0).all()                       # skipped: left as they were
+    got[3:43], want[3:43] = 0, 0
+    assert ((got - want).abs() <= tol).all()
+    got, want, tol = s.step([1, 20, 2])                    # and it goes on from where it was
+    assert s.state.b_seq_len.tolist() == [24, 29, 15] and ((got - want).abs() <= tol).all()
