@@ -106,6 +106,8 @@ class ChunkState:
     Request b is row ``b_req_idx[b]`` of ``req_manager.req_to_token_indexs``, is ``b_seq_len[b]`` tokens long with the new
     ones, and its new tokens are the rows ``b_start_loc[b] .. b_start_loc[b + 1]`` of the step's tensors; they go to the cache
     slots ``mem_index``.  ``max_len_in_batch`` and ``max_new_in_batch`` are bounds known to the host (they size the grids).
+    ``status_word`` receives what ``begin`` and the attention report (a request that was refused or skipped) unless they are given
+    another one; ``check`` raises it.
     """
 
     def __init__(self, b_req_idx, b_seq_len, b_start_loc, req_to_token, max_len_in_batch: int, max_new_in_batch: int,
@@ -115,6 +117,7 @@ class ChunkState:
         self.b_req_idx, self.b_seq_len, self.b_start_loc = b_req_idx, b_seq_len, b_start_loc
         self.req_manager = InferState._ReqManager(req_to_token)
         self.mem_index, self.position_ids = mem_index, position_ids
+        self.status_word = torch.zeros(1, dtype=torch.int32, device=b_req_idx.device)
         self.pages = None
 
     @classmethod
@@ -143,8 +146,16 @@ class ChunkState:
         chunk_maps(self.b_req_idx, self.b_seq_len, b_new_len, g["block_table"], g["page_size"], self.req_manager.req_to_token_indexs,
                    self.mem_index.numel(), g["num_slots"], g["free_pages"], g["free_head"], rebuild,
                    ChunkMaps(self.b_start_loc, self.b_seq_len, self.mem_index, self.position_ids, g["free_head"]),
-                   status_word=status_word, max_new_in_batch=self.max_new_in_batch)
+                   status_word=self.status_word if status_word is None else status_word, max_new_in_batch=self.max_new_in_batch)
         return self
+
+    def check(self) -> None:
+        """Raises ``LsvdError`` if a step since the last call has refused or skipped a request (its tokens have no slots, its rows
+        no result), and forgets it.  Reads the status word on the current stream and waits for it."""
+        code = int(self.status_word.item())
+        if code != _lib.OK:
+            self.status_word.zero_()
+            _lib.check(code)
 
 
 def attn_chunk_workspace_bytes(state, layout: LatentCacheLayout, num_tokens: int) -> int:
@@ -295,6 +306,8 @@ def chunk_attention_int8_latent_absorb(
         if workspace.device != dev:
             raise ValueError(f"workspace must be on {dev}")
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if status_word is None:
+            status_word = getattr(state, "status_word", None)
         a.status_word = status_word.data_ptr() if status_word is not None else None
         _lib.check(_lib.load().lsvd_attn_chunk(C.byref(a), _stream_ptr(q)))
     return out if out is not None else out_latent

@@ -4,7 +4,7 @@ import ctypes as C
 
 import pytest
 
-from lsvd_b200 import _lib
+from lsvd_b200 import ChunkState, LsvdError, _lib
 from oracle import attention
 from test_chunk_cpu import _chunk_args, _maps_args, lib      # noqa: F401  (a fixture)
 
@@ -35,3 +35,12 @@ def test_oracle_maps_refuse_more_tokens_than_the_bound():
     table, r2t = [[0, -1], [1, -1]], [[-1] * 32 for _ in range(2)]
     start, seq, mem, pos, head, refused = attention.chunk_maps([0, 1], [3, 3], [5, 4], table, 16, r2t, 9, 64, [2, 3], 0, max_new=4)
     assert refused == [0] and seq == [3, 7] and start == [0, 5, 9] and mem == [-1] * 5 + [19, 20, 21, 22] and head == 0
+
+
+def test_state_raises_what_was_reported_once(lib):      # noqa: F811
+    st = ChunkState.paged(rows=2, max_len_in_batch=33, max_tokens=5, max_new_in_batch=3, num_pages=7, page_size=16, device="cpu")
+    st.check()
+    st.status_word.fill_(_lib.ERR_BOUNDS)
+    with pytest.raises(LsvdError):
+        st.check()
+    st.check()

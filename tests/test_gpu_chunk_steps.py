@@ -3,7 +3,7 @@ tokens -- through the slot maps, the attention and the layer."""
 import pytest
 import torch
 
-from lsvd_b200 import ChunkState, LatentCacheLayout, LatentDecodeAttention, _lib
+from lsvd_b200 import ChunkState, LatentCacheLayout, LatentDecodeAttention, LsvdError, _lib
 from oracle import attention as oattn
 from test_gpu_chunk import _check_maps, _maps_case, _run_maps
 
@@ -87,3 +87,38 @@ def test_more_new_tokens_than_the_bound_take_no_page():
     assert ((got - want).abs() <= tol).all()
     got, want, tol = s.step([1, 20, 2])                    # and it goes on from where it was
     assert s.state.b_seq_len.tolist() == [24, 29, 15] and ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("second", [[2, 8, 1], [2, 40, 1], [2, 60, 1]])
+def test_the_state_keeps_what_a_step_reports(second):
+    """Without a status word of the caller's, eager and replayed: no page left, or more tokens than the bound."""
+    s = Steps(rows=3, num_pages=5, max_new=50)
+    s.step([20, 9, 30])
+    s.state.check()
+    s.step(second)
+    with pytest.raises(LsvdError):
+        s.state.check()
+    s.state.check()                                        # once
+    new = torch.tensor(second, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            s.state.begin(new)
+        graph.replay()
+    side.synchronize()
+    with pytest.raises(LsvdError):
+        s.state.check()
+
+
+def test_the_state_keeps_what_the_attention_reports():
+    """The slot table names a row behind the cache."""
+    s = Steps(rows=2, num_pages=8, max_new=30)
+    s.step([20, 9])
+    s.state.req_manager.req_to_token_indexs[0, 3] = 8 * 16
+    s.state.check()
+    z = torch.zeros(2, s.lay.sum_k, dtype=torch.float16, device=DEV), torch.zeros(2, s.lay.sum_v, dtype=torch.float16, device=DEV)
+    s.state.begin(torch.ones(2, dtype=torch.int32, device=DEV))
+    s.attn.forward_chunk(torch.ones(2, 2, s.D, dtype=torch.float16, device=DEV), *s.cache, s.state, latent_k=z[0], latent_v=z[1])
+    with pytest.raises(LsvdError):
+        s.state.check()
