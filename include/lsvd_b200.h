@@ -248,6 +248,8 @@ int lsvd_chunk_maps(const lsvd_chunk_maps_args* args, void* stream);
  *   x  = sm_scale * scale_k[t,h] * (z_k[t,h] . B_k q),   softcap > 0: x = softcap * tanh(x / softcap),
  *   alibi_slopes: x -= alibi_slopes[h] * |pos - t|,      p = softmax_t(x),
  *   o_lat = sum_t p_t scale_v[t,h] z_v[t,h],             o = B_v^T o_lat
+ * A request whose rows do not lie in the step's (b_start_loc negative, decreasing, or beyond num_tokens) is skipped, one with fewer
+ * tokens than rows sees nothing; both are reported as LSVD_ERR_BOUNDS.
  * A row that sees nothing (or only scores of minus infinity) gets zeros.  Cached tokens whose slot is negative are not
  * seen.  Rows behind b_start_loc[batch] are left as they were.  num_q_heads == num_kv_heads only.
  * ------------------------------------------------------------------------------------------- */

@@ -204,7 +204,8 @@ def chunk_attention_int8_latent_absorb(
 
     ``softcap > 0`` replaces a score x by ``softcap * tanh(x / softcap)``; ``alibi_slopes [H]`` fp32 subtracts
     ``slope * |pos - t|`` after that.  A token without a cache slot (``state.mem_index`` negative: ``chunk_maps`` has refused its
-    request) sees nothing.  Returns ``out [num_tokens, H, D]`` fp16 when ``up_v`` is given, otherwise the latent
+    request) sees nothing.  A request whose rows are not all in ``q``
+    (``state.b_start_loc``) is skipped and reported.  Returns ``out [num_tokens, H, D]`` fp16 when ``up_v`` is given, otherwise the latent
     result ``[num_tokens, sum r_v]``.  Rows of tokens that see nothing are zero; rows behind the last token are not written.
     """
     _require_cuda(q, cache_latent_k, cache_latent_v, up_k, up_v, alibi_slopes, b_prefix_len, key_begin)

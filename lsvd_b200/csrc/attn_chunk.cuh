@@ -79,18 +79,24 @@ struct ChunkRequest {
   int start, n, len, req;
 };
 
-// `report`: one thread per request says what was wrong.
+// `report`: one thread per request says what was wrong.  A request whose rows do not lie in the step's, or that has more of them than
+// the bound, is skipped: rows are its LAST tokens, so a part of them would stand at other positions.
 __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int b, bool report) {
   ChunkRequest r;
-  r.start = min(max(p.b_start_loc[b], 0), p.num_tokens);
-  const int end = min(max(p.b_start_loc[b + 1], 0), p.num_tokens);
-  r.n = max(end - r.start, 0);
+  const int start = p.b_start_loc[b], end = p.b_start_loc[b + 1];
+  const bool fits = start >= 0 && end >= start && end <= p.num_tokens;
+  r.start = fits ? start : 0;
+  r.n = fits ? end - start : 0;
   r.len = p.b_seq_len[b];
   r.req = p.b_req_idx[b];
-  bool bad = r.len > p.max_len || r.n > p.max_new;
+  bool bad = !fits || r.len > p.max_len || r.n > p.max_new;
   if (r.len > p.max_len) r.len = p.max_len;
   if (r.n > p.max_new) r.n = 0;
   if (r.len < 0) r.len = 0;
+  if (r.len < r.n) {                 // fewer tokens than rows: no row has a position (they see nothing)
+    bad = true;
+    r.len = 0;
+  }
   if (static_cast<uint32_t>(r.req) >= static_cast<uint32_t>(p.r2t_rows)) {
     bad = true;
     r.req = 0;

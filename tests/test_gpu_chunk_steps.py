@@ -5,7 +5,7 @@ import torch
 
 from lsvd_b200 import ChunkState, LatentCacheLayout, LatentDecodeAttention, LsvdError, _lib
 from oracle import attention as oattn
-from test_gpu_chunk import _check_maps, _maps_case, _run_maps
+from test_gpu_chunk import _case, _check_maps, _close, _maps_case, _run, _run_maps, _want
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -122,3 +122,36 @@ def test_the_state_keeps_what_the_attention_reports():
     s.attn.forward_chunk(torch.ones(2, 2, s.D, dtype=torch.float16, device=DEV), *s.cache, s.state, latent_k=z[0], latent_v=z[1])
     with pytest.raises(LsvdError):
         s.state.check()
+
+
+@pytest.mark.parametrize("news", [[3, 5, 4], [30, 50, 40]])
+def test_requests_whose_rows_are_not_all_there_are_skipped(news):
+    """Rows are a request's last tokens: with some of them missing the others would stand at wrong positions."""
+    c = _case(news, [40, 60, 9], [64, 32], [48, 64])
+    _, lat, _, tol = _want(c)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cut = dict(c, q=c["q"][:-2].contiguous())              # the last request lacks two rows
+    want = lat[:-2].clone()
+    want[news[0] + news[1]:] = float("nan")
+    _close(_run(cut, latent=True, status=status), want, tol[:-2])
+    assert status.item() == _lib.ERR_BOUNDS
+    status.zero_()
+    start = c["start"].clone()
+    start[0] = -2                                          # in front of the step's rows
+    want = lat.clone()
+    want[:news[0]] = float("nan")
+    _close(_run(dict(c, start=start), latent=True, status=status), want, tol)
+    assert status.item() == _lib.ERR_BOUNDS
+
+
+@pytest.mark.parametrize("news", [[3, 5, 4], [30, 50, 40]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_requests_with_fewer_tokens_than_rows_see_nothing(news, causal):
+    c = _case(news, [40, 60, 9], [64, 32], [48, 64])
+    _, lat, _, tol = _want(c, causal=causal)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    lens = c["b_seq_len"].clone()
+    lens[1] = news[1] - 1
+    lat[news[0]:news[0] + news[1]] = 0
+    _close(_run(dict(c, b_seq_len=lens), latent=True, status=status, causal=causal), lat, tol)
+    assert status.item() == _lib.ERR_BOUNDS
