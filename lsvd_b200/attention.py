@@ -424,10 +424,12 @@ class LatentDecodeAttention(nn.Module):
 
     @torch.no_grad()
     def forward_chunk(self, q, cache_k, scale_k, cache_v, scale_v, state, latent_k=None, latent_v=None, out=None, out_latent=None,
-                      **scores):
+                      workspace=None, **scores):
         """A step with any number of new tokens per request (``state``: a ``ChunkState``): appends their latents ``[T, sum r]``
         at ``state.mem_index`` when they are given, then attends from ``q [T, H, D]``.  ``scores``: ``causal``, ``window``,
-        ``b_prefix_len``, ``key_begin``, ``softcap``, ``alibi_slopes``, ``sm_scale`` as in ``chunk_attention_int8_latent_absorb``."""
+        ``b_prefix_len``, ``key_begin``, ``softcap``, ``alibi_slopes``, ``sm_scale`` as in ``chunk_attention_int8_latent_absorb``.
+        The kept workspace serves steps that run one after another; a step beside them on another stream, or a captured one
+        that is replayed beside them, needs a ``workspace`` of its own (``attn_chunk_workspace_bytes``)."""
         from .chunk import chunk_attention_int8_latent_absorb, kept_workspace      # (chunk.py imports this file)
         if self.up_v is None and out is not None:
             raise ValueError("without up_v the result is out_latent")
@@ -439,7 +441,8 @@ class LatentDecodeAttention(nn.Module):
         return chunk_attention_int8_latent_absorb(
             q, state, self.layout.num_heads, self.head_dim, cache_k, scale_k, cache_v, scale_v, self.up_k, self.up_v,
             layout=self.layout, out=out, out_latent=out_latent,
-            workspace=kept_workspace(self._chunk_workspaces, state, self.layout, q.shape[0], q.device), **scores)
+            workspace=kept_workspace(self._chunk_workspaces, state, self.layout, q.shape[0], q.device) if workspace is None else workspace,
+            **scores)
 
 
 @torch.no_grad()

@@ -170,10 +170,12 @@ def kept_workspace(kept: list, state, layout: LatentCacheLayout, num_tokens: int
     give each its own ``workspace``."""
     with torch.cuda.device(device):
         need = max(attn_chunk_workspace_bytes(state, layout, num_tokens), 256)
-    last = kept[-1].numel() if kept and kept[-1].device == device else 0
+    here = [w for w in kept if w.device == device]
+    last = here[-1].numel() if here else 0
     if last < need:
-        kept.append(torch.empty(max(need, 2 * last), dtype=torch.uint8, device=device))
-    return kept[-1]
+        here.append(torch.empty(max(need, 2 * last), dtype=torch.uint8, device=device))
+        kept.append(here[-1])
+    return here[-1]
 
 
 def _row_view(name, t, rows, cols, dev):

@@ -116,6 +116,7 @@ def _layer_chunk(self, x, cache_k, scale_k, cache_v, scale_v, state, stages=None
     to what its request has cached and to the step's tokens before it: a prompt or a piece of one, drafted tokens to verify, or
     one token (then the same as ``forward``).  ``scores``: ``causal``, ``window``, ``b_prefix_len``, ``key_begin``, ``softcap``
     and ``alibi_slopes`` as in ``chunk_attention_int8_latent_absorb``.  Rows behind the last token hold no result.
+    Steps of a layer (of a stack) run one after another, captured ones too: its attention and its FFN keep their workspaces.
     The products take the decode kernels up to 64 tokens and the tcgen05 GEMM beyond, as the FFN does."""
     lay, T = self.layout, x.shape[0]
     if T == 0:

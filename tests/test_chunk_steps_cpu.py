@@ -3,8 +3,9 @@ step cannot take."""
 import ctypes as C
 
 import pytest
+import torch
 
-from lsvd_b200 import ChunkState, LsvdError, _lib
+from lsvd_b200 import ChunkState, LsvdError, _lib, chunk
 from oracle import attention
 from test_chunk_cpu import _chunk_args, _maps_args, lib      # noqa: F401  (a fixture)
 
@@ -44,3 +45,17 @@ def test_state_raises_what_was_reported_once(lib):      # noqa: F811
     with pytest.raises(LsvdError):
         st.check()
     st.check()
+
+
+def test_kept_workspaces_of_two_devices(monkeypatch):
+    """Steps that alternate between devices find their own again."""
+    import contextlib
+    monkeypatch.setattr(chunk, "attn_chunk_workspace_bytes", lambda state, layout, n: 1000 * n)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    kept, cpu, meta = [], torch.device("cpu"), torch.device("meta")
+    a, b = chunk.kept_workspace(kept, None, None, 2, cpu), chunk.kept_workspace(kept, None, None, 1, meta)
+    for _ in range(3):
+        assert chunk.kept_workspace(kept, None, None, 2, cpu) is a and chunk.kept_workspace(kept, None, None, 1, meta) is b
+    big = chunk.kept_workspace(kept, None, None, 3, cpu)
+    assert big.numel() == 4000 and [w.numel() for w in kept] == [2000, 1000, 4000]
+    assert chunk.kept_workspace(kept, None, None, 1, cpu) is big and kept[0] is a

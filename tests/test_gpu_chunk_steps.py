@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from lsvd_b200 import ChunkState, LatentCacheLayout, LatentDecodeAttention, LsvdError, _lib
+from lsvd_b200.chunk import attn_chunk_workspace_bytes
 from oracle import attention as oattn
 from test_gpu_chunk import _case, _check_maps, _close, _maps_case, _run, _run_maps, _want
 
@@ -155,3 +156,53 @@ def test_requests_with_fewer_tokens_than_rows_see_nothing(news, causal):
     lat[news[0]:news[0] + news[1]] = 0
     _close(_run(dict(c, b_seq_len=lens), latent=True, status=status, causal=causal), lat, tol)
     assert status.item() == _lib.ERR_BOUNDS
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_one_module_on_two_streams_with_workspaces_of_their_own(captured):
+    """Partial results of two steps at once, eager or as graphs that are replayed side by side."""
+    cases = [_case([9, 30], [900, 77], [64, 32], [48, 64], seed=s) for s in (1, 2)]
+    cases[1]["up_k"], cases[1]["up_v"] = cases[0]["up_k"], cases[0]["up_v"]
+    wants = [_want(c) for c in cases]
+    attn = LatentDecodeAttention(cases[0]["layout"], 64, cases[0]["up_k"].to(DEV), cases[0]["up_v"].to(DEV))
+    runs = []
+    for c in cases:
+        st = ChunkState(c["b_req_idx"].to(DEV), c["b_seq_len"].to(DEV), c["start"].to(DEV), c["req_to_token"].to(DEV), c["max_len"], 30)
+        q, caches = c["q"].to(DEV), [c[k].to(DEV) for k in ("cache_k", "scale_k", "cache_v", "scale_v")]
+        out = torch.full_like(q, 77.0)
+        ws = torch.empty(attn_chunk_workspace_bytes(st, c["layout"], q.shape[0]), dtype=torch.uint8, device=DEV)
+        runs.append((lambda q=q, caches=caches, st=st, out=out, ws=ws: attn.forward_chunk(q, *caches, st, out=out, workspace=ws), out))
+    torch.cuda.synchronize()
+    streams, calls = [torch.cuda.Stream() for _ in runs], []
+    for (call, _), s in zip(runs, streams):
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.stream(s):
+                call()
+                with torch.cuda.graph(graph, stream=s):
+                    call()
+            call = graph.replay
+        calls.append(call)
+    torch.cuda.synchronize()
+    for _, out in runs:
+        out.fill_(77.0)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for call, s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                call()
+    torch.cuda.synchronize()
+    assert not attn._chunk_workspaces
+    for (_, out), (o, _, tol, _) in zip(runs, wants):
+        _close(out.cpu(), o, tol)
+
+
+def test_kept_workspaces_grow_and_stay():
+    s = Steps(rows=2, num_pages=40, max_new=200)
+    kept = s.attn._chunk_workspaces
+    s.step([3, 1])
+    first = kept[-1]
+    s.step([1, 2])
+    assert len(kept) == 1 and kept[0].data_ptr() == first.data_ptr()
+    s.step([150, 100])
+    assert kept[0].data_ptr() == first.data_ptr() and all(b.numel() >= 2 * a.numel() for a, b in zip(kept, kept[1:]))
