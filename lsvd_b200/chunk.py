@@ -39,6 +39,15 @@ def _i32(name, t, *shape, device):
     return t.data_ptr()
 
 
+def _status(t, device):
+    """Address of a status word: the kernels write to it, so it has to be where they run."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.numel() < 1 or t.device != device:
+        raise ValueError(f"status_word must be an int32 tensor on {device}")
+    return t.data_ptr()
+
+
 def _table(name, t, device):
     if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.device != device or t.numel() == 0:
         raise ValueError(f"{name} must be a non-empty int32 table [rows, columns] with unit column stride on {device}")
@@ -94,7 +103,7 @@ def chunk_maps(b_req_idx, b_ready_cache_len, b_new_len, block_table, page_size: 
     a.b_seq_len = _i32("out.b_seq_len", out.b_seq_len, B, device=dev)
     a.mem_index = _i32("out.mem_index", out.mem_index, num_tokens, device=dev)
     a.position_ids = _i32("out.position_ids", out.position_ids, num_tokens, device=dev)
-    a.status_word = status_word.data_ptr() if status_word is not None else None
+    a.status_word = _status(status_word, dev)
     with torch.cuda.device(dev):
         _lib.check(_lib.load().lsvd_chunk_maps(C.byref(a), _stream_ptr(b_req_idx)))
     return out
@@ -236,6 +245,8 @@ def chunk_attention_int8_latent_absorb(
         raise ValueError("up-factors must be [sum r, head_dim]")
     if up_k.stride(1) != 1 or (up_v is not None and up_v.stride(1) != 1):
         raise ValueError("up-factors must have unit inner stride")
+    if up_k.device != dev or (up_v is not None and up_v.device != dev):
+        raise ValueError(f"up-factors must be on {dev}")
     hm, n_slots = layout.head_major, layout.num_slots_of(cache_latent_k, "k")
     for which, cache, scale, total in (("k", cache_latent_k, cache_latent_k_scale, layout.sum_k),
                                        ("v", cache_latent_v, cache_latent_v_scale, layout.sum_v)):
@@ -306,11 +317,11 @@ def chunk_attention_int8_latent_absorb(
         need = attn_chunk_workspace_bytes(state, layout, T)
         if workspace is None:
             workspace = alloc_tensor_func((max(need, 256),), dtype=torch.uint8, device=dev)
-        if workspace.device != dev:
-            raise ValueError(f"workspace must be on {dev}")
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         if status_word is None:
             status_word = getattr(state, "status_word", None)
-        a.status_word = status_word.data_ptr() if status_word is not None else None
+        a.status_word = _status(status_word, dev)
         _lib.check(_lib.load().lsvd_attn_chunk(C.byref(a), _stream_ptr(q)))
     return out if out is not None else out_latent

@@ -59,3 +59,13 @@ def test_kept_workspaces_of_two_devices(monkeypatch):
     big = chunk.kept_workspace(kept, None, None, 3, cpu)
     assert big.numel() == 4000 and [w.numel() for w in kept] == [2000, 1000, 4000]
     assert chunk.kept_workspace(kept, None, None, 1, cpu) is big and kept[0] is a
+
+
+def test_status_words_have_to_be_where_the_kernels_run():
+    gpu, cpu = torch.device("cuda", 0), torch.device("cpu")
+    assert chunk._status(None, gpu) is None
+    word = torch.zeros(1, dtype=torch.int32)
+    assert chunk._status(word, cpu) == word.data_ptr()
+    for bad, dev in ((word, gpu), (word.long(), cpu), (word[:0], cpu), (torch.zeros(1), cpu)):
+        with pytest.raises(ValueError):
+            chunk._status(bad, dev)

@@ -3,7 +3,7 @@ tokens -- through the slot maps, the attention and the layer."""
 import pytest
 import torch
 
-from lsvd_b200 import ChunkState, LatentCacheLayout, LatentDecodeAttention, LsvdError, _lib
+from lsvd_b200 import ChunkState, LatentCacheLayout, LatentDecodeAttention, LsvdError, _lib, chunk_attention_int8_latent_absorb
 from lsvd_b200.chunk import attn_chunk_workspace_bytes
 from oracle import attention as oattn
 from test_gpu_chunk import _case, _check_maps, _close, _maps_case, _run, _run_maps, _want
@@ -206,3 +206,25 @@ def test_kept_workspaces_grow_and_stay():
     assert len(kept) == 1 and kept[0].data_ptr() == first.data_ptr()
     s.step([150, 100])
     assert kept[0].data_ptr() == first.data_ptr() and all(b.numel() >= 2 * a.numel() for a, b in zip(kept, kept[1:]))
+
+
+def test_tensors_that_are_elsewhere_are_refused():
+    """Refused on the host: what the kernels read or write has to be on their device."""
+    c = _case([2, 1], [5, 9], [64, 32], [48, 64])
+    st = ChunkState(c["b_req_idx"].to(DEV), c["b_seq_len"].to(DEV), c["start"].to(DEV), c["req_to_token"].to(DEV), c["max_len"], 2)
+    caches = [c[k].to(DEV) for k in ("cache_k", "scale_k", "cache_v", "scale_v")]
+
+    def call(**kw):
+        a = dict(up_k=c["up_k"].to(DEV), up_v=c["up_v"].to(DEV), status_word=None, workspace=None)
+        a.update(kw)
+        return chunk_attention_int8_latent_absorb(c["q"].to(DEV), st, 2, 64, *caches, layout=c["layout"], **a)
+
+    call()
+    word = torch.zeros(1, dtype=torch.int32)
+    for bad in (dict(status_word=word), dict(status_word=word.to(DEV).long()), dict(up_k=c["up_k"]), dict(up_v=c["up_v"]),
+                dict(workspace=torch.empty(1 << 20, dtype=torch.uint8)), dict(workspace=torch.empty(2 << 20, dtype=torch.uint8, device=DEV)[::2])):
+        with pytest.raises(ValueError):
+            call(**bad)
+    s = Steps(rows=1, num_pages=2, max_new=4)
+    with pytest.raises(ValueError):
+        s.state.begin(torch.ones(1, dtype=torch.int32, device=DEV), status_word=word)
