@@ -39,6 +39,11 @@ def _i32(name, t, *shape, device):
     return t.data_ptr()
 
 
+def _bound(n) -> int:
+    """A bound as the C side holds it: one beyond 32 bits bounds nothing, and must not come out as its lower half."""
+    return min(int(n), 2 ** 31 - 1)
+
+
 def _status(t, device):
     """Address of a status word: the kernels write to it, so it has to be where they run."""
     if t is None:
@@ -92,7 +97,7 @@ def chunk_maps(b_req_idx, b_ready_cache_len, b_new_len, block_table, page_size: 
     a.block_table, a.block_table_stride = _table("block_table", block_table, dev)
     a.req_to_token, a.req_to_token_stride = _table("req_to_token", req_to_token, dev)
     a.max_blocks, a.table_rows, a.max_len = block_table.shape[1], block_table.shape[0], req_to_token.shape[1]
-    a.rebuild, a.max_new_in_batch = int(rebuild), int(max_new_in_batch)
+    a.rebuild, a.max_new_in_batch = int(rebuild), _bound(max_new_in_batch)
     if free_pages is not None:
         a.free_pages, a.num_free = _i32("free_pages", free_pages, free_pages.numel(), device=dev), free_pages.numel()
         a.free_head = _i32("free_head", free_head, 1, device=dev)
@@ -169,7 +174,7 @@ class ChunkState:
 
 def attn_chunk_workspace_bytes(state, layout: LatentCacheLayout, num_tokens: int) -> int:
     return int(_lib.load().lsvd_attn_chunk_workspace_bytes(state.batch_size, layout.num_heads, layout.sum_v, num_tokens,
-                                                           int(state.max_new_in_batch), int(state.max_len_in_batch)))
+                                                           _bound(state.max_new_in_batch), _bound(state.max_len_in_batch)))
 
 
 def kept_workspace(kept: list, state, layout: LatentCacheLayout, num_tokens: int, device) -> torch.Tensor:
@@ -265,7 +270,7 @@ def chunk_attention_int8_latent_absorb(
     r2t = state.req_manager.req_to_token_indexs
     a = _lib.AttnChunkArgs()
     a.batch, a.num_heads, a.head_dim, a.num_tokens = B, q_head_num, head_dim, T
-    a.max_len_in_batch, a.max_new_in_batch = int(state.max_len_in_batch), int(state.max_new_in_batch)
+    a.max_len_in_batch, a.max_new_in_batch = _bound(state.max_len_in_batch), _bound(state.max_new_in_batch)
     a.sm_scale = float(sm_scale) if sm_scale is not None else 0.0
     a.num_slots, a.cache_layout = n_slots, _lib.CACHE_HEAD_MAJOR if hm else _lib.CACHE_SLOT_MAJOR
     a.req_to_token, a.req_to_token_stride = _table("req_to_token", r2t, dev)
@@ -296,7 +301,7 @@ def chunk_attention_int8_latent_absorb(
     a.up_k, a.up_k_row_stride = up_k.data_ptr(), up_k.stride(0)
     if up_v is not None:
         a.up_v, a.up_v_row_stride = up_v.data_ptr(), up_v.stride(0)
-    a.causal, a.window, a.softcap = int(causal), int(window), float(softcap)
+    a.causal, a.window, a.softcap = int(bool(causal)), _bound(window), float(softcap)
     if window < 0 or softcap < 0:
         raise ValueError("window and softcap must not be negative")
     if alibi_slopes is not None:

@@ -69,3 +69,7 @@ def test_status_words_have_to_be_where_the_kernels_run():
     for bad, dev in ((word, gpu), (word.long(), cpu), (word[:0], cpu), (torch.zeros(1), cpu)):
         with pytest.raises(ValueError):
             chunk._status(bad, dev)
+
+
+def test_bounds_are_held_not_wrapped():
+    assert [chunk._bound(n) for n in (0, 5, -3, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1)] == [0, 5, -3, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1]

@@ -228,3 +228,16 @@ def test_tensors_that_are_elsewhere_are_refused():
     s = Steps(rows=1, num_pages=2, max_new=4)
     with pytest.raises(ValueError):
         s.state.begin(torch.ones(1, dtype=torch.int32, device=DEV), status_word=word)
+
+
+@pytest.mark.parametrize("news", [[3, 1], [40, 2]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_bounds_beyond_32_bits_bound_nothing(news, causal):
+    c = _case(news, [50, 90], [64, 32], [48, 64])
+    want = _run(c, causal=causal)
+    for large in (2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 63 - 1):
+        assert torch.equal(_run(c, causal=causal, window=large), want)
+    s = Steps(rows=2, num_pages=20, max_new=2 ** 32 + 1)
+    got, o, tol = s.step(news)
+    s.state.check()
+    assert ((got - o).abs() <= tol).all()
