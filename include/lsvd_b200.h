@@ -206,7 +206,9 @@ int lsvd_attn_decode_static(const lsvd_attn_decode_args* args, void* stream);
  * b_ready_cache_len and free_head_out the word free_head (a captured step then advances the lengths at every replay).
  * An entry is refused -- it takes no page, its length stays `ready`, its tokens get slot -1 and position 0, LSVD_ERR_BOUNDS
  * is reported -- when its row, a length or its tokens do not fit the tables, num_tokens or max_new_in_batch, when an earlier entry
- * adds tokens to the same row, or when the free pages run out (with every later entry that needs a page).  A page outside the cache gives slot -1.
+ * adds tokens to the same row, when the free pages run out (with every later entry that needs a page), or when, in a rebuild with a
+ * free list, it has no new tokens and more cached ones than the entry that adds tokens to its row.  A page outside the cache gives
+ * slot -1.
  * ------------------------------------------------------------------------------------------- */
 #define LSVD_MAX_BATCH 4096     /* entries of a batch in lsvd_chunk_maps */
 typedef struct lsvd_chunk_maps_args {

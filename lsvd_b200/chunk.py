@@ -75,7 +75,8 @@ def chunk_maps(b_req_idx, b_ready_cache_len, b_new_len, block_table, page_size: 
     the capacity of the token maps and ``num_slots`` the number of cache rows.  ``out`` receives the results;
     ``out.b_seq_len`` may be ``b_ready_cache_len`` and ``out.free_head`` may be ``free_head``, so that a captured step
     advances the lengths at every replay.  An entry that does not fit (its row, its length, ``num_tokens``, more new tokens
-    than a ``max_new_in_batch`` above zero, the free pages, or a row that an earlier entry adds tokens to) gets no page and slot -1 for its tokens, its length stays, and
+    than a ``max_new_in_batch`` above zero, the free pages, a row that an earlier entry adds tokens to, or, in
+    a rebuild, no new tokens and more cached ones than the entry that adds tokens to its row) gets no page and slot -1 for its tokens, its length stays, and
     ``LSVD_ERR_BOUNDS`` is written to ``status_word``.
     """
     _require_cuda(b_req_idx, b_ready_cache_len, b_new_len, block_table, req_to_token, free_pages, free_head)

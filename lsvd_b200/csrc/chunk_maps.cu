@@ -165,6 +165,11 @@ __global__ void __launch_bounds__(kMapsThreads) chunk_maps_kernel(const __grid_c
       while (s.key[at & s.hash_mask] != row[i]) ++at;      // it was entered above
       if (s.first[at & s.hash_mask] != b) ok[i] = false;
       if (ok[i] && paged) v[i] = pages_of(ready[i] + add[i], P) - pages_of(ready[i], P);
+    } else if (ok[i] && paged && p.rebuild) {
+      // its slots are rewritten from columns of the table: none of them may be one that another entry's pages go to
+      uint32_t at = (static_cast<uint32_t>(row[i]) * 2654435761u) >> 7;
+      while (s.key[at & s.hash_mask] != row[i] && s.key[at & s.hash_mask] != kHashEmpty) ++at;      // (half the table is empty)
+      if (s.key[at & s.hash_mask] == row[i] && ready[i] > p.b_ready_cache_len[s.first[at & s.hash_mask]]) ok[i] = false;
     }
   }
   int32_t need[kMapsPer];

@@ -165,21 +165,29 @@ def chunk_maps(req, ready, new, table, page, r2t, num_tokens, num_slots, free=No
     """Slots of a step's new tokens, entry by entry (lists of Python integers; ``table`` and ``r2t`` are changed in place).
 
     Returns (start, seq, mem_index, position_ids, head, refused) with ``refused`` the entries that got nothing: their row or
-    length does not fit the tables, their tokens do not fit ``num_tokens`` or are more than ``max_new`` (0: any), an earlier entry adds tokens to the same row, or
-    the free pages have run out.
+    length does not fit the tables, their tokens do not fit ``num_tokens`` or are more than ``max_new`` (0: any), an earlier entry adds tokens to the same row, the free pages have
+    run out, or (``rebuild``) it has no new tokens and more cached ones than the entry that adds tokens to its row.
     """
     up = lambda tokens: -(-tokens // page)
     start, seq, refused, seen, dry = [0], [], [], set(), False
     mem, pos = [-1] * num_tokens, [0] * num_tokens
     h = head
+    fits = lambda row, old, n: 0 <= row < len(table) and old >= 0 and n >= 0 and old + n <= len(r2t[0]) and old + n <= len(table[0]) * page
+    adds, at = {}, 0
+    for row, old, n in zip(req, ready, new):
+        at += max(n, 0)
+        if n > 0 and fits(row, old, n) and at <= num_tokens and (max_new == 0 or n <= max_new):
+            adds.setdefault(row, old)
     for b, (row, old, n) in enumerate(zip(req, ready, new)):
         first = start[-1]
         start.append(first + max(n, 0))
-        ok = 0 <= row < len(table) and old >= 0 and n >= 0 and old + n <= len(r2t[0]) and old + n <= len(table[0]) * page
+        ok = fits(row, old, n)
         ok = ok and start[-1] <= num_tokens and (max_new == 0 or n <= max_new)
         if ok and n > 0:
             ok = row not in seen
             seen.add(row)
+        elif ok and rebuild and free is not None:
+            ok = old <= adds.get(row, old)
         need = up(old + n) - up(old) if ok and free is not None else 0
         if need and (dry or not 0 <= head <= len(free) or h + need > len(free)):
             dry, ok = True, False

@@ -241,3 +241,20 @@ def test_bounds_beyond_32_bits_bound_nothing(news, causal):
     got, o, tol = s.step(news)
     s.state.check()
     assert ((got - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("swap", [False, True])
+@pytest.mark.parametrize("ready,refused", [(5, False), (4, False), (21, True)])
+def test_rebuild_of_a_row_that_also_grows(ready, refused, swap):
+    """An entry without new tokens is rebuilt beside the one that adds tokens to the same row, unless its length reaches into
+    the columns that the new pages go to."""
+    c = _maps_case(3, 16, [30, 0, 2], [5, ready, 9])
+    c["req"][1] = c["req"][0]
+    order = [1, 0, 2] if swap else [0, 1, 2]
+    for k in ("req", "ready", "new"):
+        c[k] = [c[k][i] for i in order]
+    _check_maps(c, rebuild=True, refused=[order.index(1)] if refused else [])
+    _check_maps(c)                                         # without a rebuild it reads no column
+    if refused:                                            # without a free list no column is written
+        c["free"], c["head"] = None, 0
+        _check_maps(c, rebuild=True)
