@@ -214,10 +214,17 @@ def chunk_absorb(q16, cache_k, scale_k, cache_v, scale_v, up_k16, up_v16, k_off,
     Keys are rebuilt (no absorbed query): x = sm_scale s_k (z_k B_k) . q, capped, biased, masked; o_lat = sum p s_v z_v,
     o = B_v^T o_lat.  Returns (o [T, H, D], o_lat [T, sum r_v], their bounds); rows of no request are NaN.
 
-    The bounds follow from the kernels' roundings, each half a step: the absorbed query in fp16 (2^-11 of every term of a
-    score: dx), fp32 arithmetic on scores (2^-19 of the largest score, capped, or bias, whatever the cap), weights p s_v in fp16 (2^-11 of
-    every term), sums in fp32 (2^-20), the result in fp16 (2^-11, or half a step of 2^-24 below the normal range).  A score
-    off by dx changes a weight by e^dx and the sum of weights by as much: 2 dx of every term.
+    The bounds follow from the kernels' roundings; |.| stands for the same sum over absolute values, 2^-22 for a step of a product
+    with fp32 accumulators (16 terms, not rounded to nearest):
+      q~ = B_k q          D / 16 + 2 steps of |B_k| |q|; held as two fp16 numbers, 2^-22 of an entry and 2^-33 of the row's largest
+      score               those times |z|, and r_k / 8 + 2 steps of |q~| |z| (two products)
+      scales, cap, bias   2^-19 of the largest score or bias, whatever the cap
+      x - R, 2^x          2^-18: |x - R| < 64 in units of log2 where a weight counts
+    together dx, the largest over the keys that a row sees; a weight changes by e^dx and the sum of weights by as much: 2 dx of every term.
+      weights             two fp16 numbers, 2^-21 of each and 2^-30 of the row's largest
+      sums over L keys    L / 16 + 16 steps of 2^-23 of |w| |z|, as much for the weights' sum; 2^-20 for factors and the quotient
+      up-projection       2^-17 of |o_lat| |B_v| (r_v sums, two fp16 numbers) and 2^-25 |B_v|
+      result              to fp16: 2^-11, or half a step of 2^-24 below the normal range
     """
     T, H, D = q16.shape
     sm = 1.0 / math.sqrt(D) if sm_scale is None else sm_scale
@@ -245,7 +252,9 @@ def chunk_absorb(q16, cache_k, scale_k, cache_v, scale_v, up_k16, up_v16, k_off,
             kb, zk, sk = f(up_k16[k_off[h]:k_off[h + 1]]), f(cache_k[rows, k_off[h]:k_off[h + 1]]), f(scale_k[rows, h])
             zv, sv = f(cache_v[rows, v_off[h]:v_off[h + 1]]), f(scale_v[rows, h])
             x = (f(q16[a:e, h]) @ (zk @ kb).t()) * sk * sm
-            dx = 2.0 ** -11 * ((f(q16[a:e, h]) @ kb.t()).abs() @ zk.abs().t()) * sk.abs() * sm
+            qt, step = (f(q16[a:e, h]) @ kb.t()).abs(), 2.0 ** -22
+            dq = (D / 16 + 2) * step * (f(q16[a:e, h]).abs() @ kb.abs().t()) + step * qt + 2.0 ** -33 * qt.amax(1, keepdim=True)
+            dx = ((dq + (kb.shape[0] / 8 + 2) * step * qt) @ zk.abs().t()) * sk.abs() * sm
             big = x.abs()
             if softcap > 0:
                 x = softcap * torch.tanh(x / softcap)
@@ -255,7 +264,7 @@ def chunk_absorb(q16, cache_k, scale_k, cache_v, scale_v, up_k16, up_v16, k_off,
                 x = x - bias
                 big = torch.maximum(big, bias)
             none = torch.zeros((), dtype=torch.float64)
-            dx = torch.where(sees, dx + 2.0 ** -19 * big, none).amax(1, keepdim=True) if L else torch.zeros(n, 1, dtype=torch.float64)
+            dx = torch.where(sees, dx + 2.0 ** -19 * big + 2.0 ** -18, none).amax(1, keepdim=True) if L else torch.zeros(n, 1, dtype=torch.float64)
             x = x.masked_fill(~sees, float("-inf"))
             if L:
                 x = x - x.amax(1, keepdim=True).clamp_min(-1e300)
@@ -264,12 +273,13 @@ def chunk_absorb(q16, cache_k, scale_k, cache_v, scale_v, up_k16, up_v16, k_off,
             p = torch.where(total > 0, p / total, none)
             w = torch.where(p > 0, p * sv, none)
             y = w @ zv
-            off = (w.abs() @ zv.abs()) * (2 * dx * torch.exp(2 * dx) + 2.0 ** -11 + 2.0 ** -20)
+            off = (w.abs() @ zv.abs()) * (2 * dx * torch.exp(2 * dx) + 2.0 ** -20 + 2.0 ** -21 + 2 * (L / 16 + 16) * 2.0 ** -23)
+            if L:
+                off = off + 2.0 ** -30 * w.abs().amax(1, keepdim=True) * ((w != 0).double() @ zv.abs())
             lat[a:e, v_off[h]:v_off[h + 1]] = y
             lat_tol[a:e, v_off[h]:v_off[h + 1]] = half(y, off)
             if up_v16 is not None:
                 bv = f(up_v16[v_off[h]:v_off[h + 1]])
                 o[a:e, h] = y @ bv
-                # the latent result may pass through fp16 on its way
-                o_tol[a:e, h] = half(y @ bv, (off + 2.0 ** -11 * (y.abs() + off) + 2.0 ** -25) @ bv.abs() * (1 + 2.0 ** -20))
+                o_tol[a:e, h] = half(y @ bv, (off + 2.0 ** -17 * (y.abs() + off) + 2.0 ** -25) @ bv.abs())
     return o, lat, o_tol, lat_tol

@@ -110,3 +110,12 @@ def test_caps_of_any_size(news, cap):
     if cap >= 1e8:
         _, lat, _, _ = _want(c)
         assert rounding_ratio(_run(c, latent=True, softcap=cap), lat) <= 1.05
+
+
+@pytest.mark.parametrize("news,olds", [([3], [5000]), ([100], [3000]), ([1] * 20, [(i * 97) % 700 + 200 for i in range(20)])])
+def test_error_over_splits_of_the_keys(news, olds):
+    c = _case(news, olds, [64, 32], [48, 64])
+    o, lat, _, _ = _want(c)
+    for hm in (False, True):
+        assert rounding_ratio(_run(c, hm), o) <= 1.05
+        assert rounding_ratio(_run(c, hm, latent=True), lat) <= 1.05
