@@ -534,7 +534,7 @@ static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_ne
   c.stream_stride = std::min(kStreamMost, longest);
   chunk_split(static_cast<int64_t>(num_heads) * batch, 4 * 3 * sms, 256, 128, max_len, &c.stream_splits, &c.stream_split_len);
   const int64_t of_tokens = num_tokens / kChunkTileRows + std::min<int64_t>(batch, num_tokens / (c.tile_min + 1));
-  const int64_t of_requests = static_cast<int64_t>(batch) * ((longest + kChunkTileRows - 1) / kChunkTileRows);
+  const int64_t of_requests = static_cast<int64_t>(batch) * ((static_cast<int64_t>(longest) + kChunkTileRows - 1) / kChunkTileRows);
   c.tiles = static_cast<int>(std::max<int64_t>(1, std::min(of_tokens, of_requests)));
   chunk_split(static_cast<int64_t>(num_heads) * c.tiles, 2 * sms, 512, 64, max_len, &c.tile_splits, &c.tile_split_len);
   if (!c.stream) c.stream_splits = 0;

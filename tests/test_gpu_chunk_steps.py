@@ -258,3 +258,17 @@ def test_rebuild_of_a_row_that_also_grows(ready, refused, swap):
     if refused:                                            # without a free list no column is written
         c["free"], c["head"] = None, 0
         _check_maps(c, rebuild=True)
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [5, 0, 2]])
+def test_a_step_may_have_a_bound_of_its_own(news):
+    """The state's bound sizes the grids; a step that is known to bring less may lower it for itself."""
+    s = Steps(rows=3, num_pages=30, max_new=200)
+    s.step([100, 20, 3])
+    s.state.max_new_in_batch = max(news)
+    got, want, tol = s.step(news)
+    assert ((got - want).abs() <= tol).all()
+    s.state.max_new_in_batch = 200
+    got, want, tol = s.step([3, 90, 1])
+    s.state.check()
+    assert ((got - want).abs() <= tol).all()
