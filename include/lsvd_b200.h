@@ -302,7 +302,7 @@ typedef struct lsvd_attn_chunk_args {
   const int32_t* mem_index;      /* device int32 [num_tokens] or NULL: cache slots of the rows' tokens, as lsvd_chunk_maps     */
                                  /* gives them.  A row whose token has none (negative: its request was refused) sees nothing.  */
 } lsvd_attn_chunk_args;
-/* Bytes of workspace for this problem on the current device (0: bad sizes). */
+/* Bytes of workspace for this problem on the current device (0: none is needed, or bad sizes). */
 size_t lsvd_attn_chunk_workspace_bytes(int32_t batch, int32_t num_heads, int32_t sum_rank_v, int32_t num_tokens,
                                        int32_t max_new_in_batch, int32_t max_len_in_batch);
 int lsvd_attn_chunk(const lsvd_attn_chunk_args* args, void* stream);

@@ -507,6 +507,7 @@ struct ChunkPlan {
   bool stream, tile;                       // which forms are launched
   int stream_splits, stream_split_len, stream_stride;
   int tiles, tile_splits, tile_split_len, tile_min;
+  bool tile_rows;                          // the tile form needs rows for partial results: it is split, or a piece is folded
 };
 
 static void chunk_split(int64_t blocks, int64_t want, int least, int unit, int max_len, int* splits, int* len) {
@@ -539,6 +540,7 @@ static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_ne
   chunk_split(static_cast<int64_t>(num_heads) * c.tiles, 2 * sms, 512, 64, max_len, &c.tile_splits, &c.tile_split_len);
   if (!c.stream) c.stream_splits = 0;
   if (!c.tile) c.tile_splits = 0;
+  c.tile_rows = c.tile && (c.tile_splits > 1 || max_len > kFoldKeys);
   return c;
 }
 
@@ -546,11 +548,12 @@ struct ChunkWorkspace {
   size_t stream_ml, stream_o, tile_ml, tile_o, total;
 };
 
-// The stream form always has room for partial results (its up-projection is the merge's), the tile form when it is split.
+// The stream form always has room for partial results (its up-projection is the merge's), the tile form when it is split or its
+// rows may have more keys than one accumulator sums.
 static ChunkWorkspace chunk_workspace(const ChunkPlan& c, int batch, int num_heads, int sum_rv, int num_tokens) {
   auto align = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t srows = static_cast<size_t>(c.stream_splits) * batch * c.stream_stride;
-  const size_t trows = c.tile_splits > 1 ? static_cast<size_t>(c.tile_splits) * num_tokens : 0;
+  const size_t trows = c.tile_rows ? static_cast<size_t>(c.tile_splits) * num_tokens : 0;
   ChunkWorkspace w{};
   w.stream_o = align(srows * num_heads * sizeof(float2));
   w.tile_ml = w.stream_o + align(srows * sum_rv * sizeof(float));
@@ -615,7 +618,7 @@ extern "C" int lsvd_attn_chunk(const lsvd_attn_chunk_args* a, void* stream) {
   const bool stream_partials = c.stream && (c.stream_splits > 1 || a->out != nullptr);
   const bool merge = stream_partials || c.tile_splits > 1;
   const ChunkWorkspace w = chunk_workspace(c, a->batch, a->num_heads, sum_rv, a->num_tokens);
-  if (merge && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned(a->workspace, 256))) return LSVD_ERR_WORKSPACE;
+  if ((merge || c.tile_rows) && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned(a->workspace, 256))) return LSVD_ERR_WORKSPACE;
 
   p.q = static_cast<const __half*>(a->q);
   p.q_stride_t = a->q_stride_t;

@@ -11,6 +11,7 @@ constexpr float kChunkLog2e = 1.4426950408889634f;
 constexpr int kStreamRows = 8;      // query rows of a block of the stream form
 constexpr int kStreamMost = 2 * kStreamRows;      // of a request of the stream form: one or two blocks
 constexpr int kChunkTileRows = 256;  // and of the tile form
+constexpr int kFoldKeys = 8192;      // keys that an accumulator in tensor memory sums before it is folded into the workspace
 
 // Weights are 2^(x - R + kWeightShift) with R, the row's reference, the largest x + exponent of |V scale| among the keys that the row
 // SEES when R was last moved (x: score in units of log2).  R moves when that has grown by more than kLazy, so |weight * scale| stays
@@ -67,6 +68,8 @@ struct ChunkParams {
   int32_t stream_splits, stream_split_len, stream_stride;
   int32_t tile_splits, tile_split_len;
   int32_t stream_partials;   // the stream form leaves its results to the merge (the tile form: when it is split)
+  // (a block of the tile form with more than kFoldKeys keys also folds its sums into its rows of tile_o as it goes, and keeps the
+  // reference that they are relative to in tile_ml)
   int32_t tile_min;          // the tile form takes requests of more rows than this
   ChunkHead head[LSVD_MAX_HEADS];
 };

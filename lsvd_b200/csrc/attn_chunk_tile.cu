@@ -27,8 +27,13 @@
 // O is rescaled only when a row's reference moves (attn_chunk.cuh): a reference is looked for where a tile's largest score and largest
 // V scale together are past it, over the keys that the row sees.  Each weight enters the product as two fp16 numbers, its
 // first eleven bits and the rest: one rounding to fp16 instead, 2^-11 of every term, made the error against 64 bits 1.2 to 1.4 times that
-// of rounding the exact result, the second half costs 4 to 15 % (a prompt of 8191 tokens, 32 heads, ranks 64 + 64: 897 -> 1000 us).  o_lat meets the up-factor as two
-// fp16 numbers, what fp16 keeps of it and the rest.
+// of rounding the exact result, the second half costs 4 to 15 % (a prompt of 8191 tokens, 32 heads, ranks 64 + 64: 897 -> 1000 us).
+// o_lat meets the up-factor as two fp16 numbers, what fp16 keeps of it and the rest.
+//
+// The tensor cores cut off what an addition to an accumulator leaves: the error grows by about 2^-23.6 of the sum with each of the 8
+// products of a tile where all terms have one sign (8192 keys 0.8e-4, half the error of the fp16 result; 66000 keys 6.6e-4), by a
+// quarter of that for sums of both signs.  Every 8192 keys the softmax warps therefore add O to fp32 sums in the workspace, to nearest,
+// and start it again from zero.  That costs 1 to 2 % where nothing is folded (code), and 3 to 4 % instead at 4096 keys.
 #include <algorithm>
 
 #include "attn_chunk.cuh"
@@ -50,6 +55,8 @@ constexpr int kTileSmem = 208 * 1024 + 1024;     // q~ (or o_lat), widened stage
 constexpr int kTileMaxStages = 4;
 constexpr int kCodeStages = 4;                   // stages of codes on their way (one where four do not fit)
 constexpr int kTileSlotRing = 8;
+constexpr int kFoldTiles = kFoldKeys / kTileKeys;
+static_assert((kFoldTiles & (kFoldTiles - 1)) == 0, "tiles between folds");
 constexpr int kTileCols = 512;                   // tensor memory, 256 columns a group: S0 0..63, S1 64..127, O 128..255
 constexpr int kGroupCols = 256;
 constexpr int kColO = 128;
@@ -145,6 +152,9 @@ __device__ __forceinline__ bool tile_wait(TileShared& s, uint64_t* bar, uint32_t
   report_status(status_word, LSVD_ERR_TIMEOUT);
   return false;
 }
+
+// What sums that were folded at a row's reference `at` count at its present one.
+__device__ __forceinline__ float folded_factor(float at, float now) { return at == now ? 1.f : ex2(at - now); }
 
 // 16-byte piece `chunk` (0..7) of row `row` in a swizzled [row][128 bytes] tile.
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4)); }
@@ -630,172 +640,207 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
     const int outer_lo = __reduce_min_sync(0xffffffffu, keys.hi > keys.lo ? keys.lo : 0x7fffffff);
     const int outer_hi = __reduce_max_sync(0xffffffffu, keys.hi);
 
-    for (int j = 0; go && j < ntiles; ++j) {
-      const int st = j & (stages - 1), k0 = kbeg + j * kTileKeys;
-      const uint32_t s_addr = lane_addr + (j & 1) * kTileKeys;
-      go = tile_wait(s, &s.full[st], (j / stages) & 1, p.status_word) && tile_wait(s, &s.s_full[grp][j & 1], (j >> 1) & 1, p.status_word);
-      if (!__all_sync(0xffffffffu, go)) {
-        go = false;
-        break;
-      }
-      tc_fence_after();
-      const bool nothing = k0 >= outer_hi || k0 + kTileKeys <= outer_lo;      // of this warp's rows
-      const uint32_t live0 = s.live[st][0], live1 = s.live[st][1];
-      const bool masked = k0 < inner_lo || k0 + kTileKeys > inner_hi || (live0 & live1) != 0xffffffffu;
-      float2 x[kTileKeys / 2];
-      float top = -INFINITY;
-      if (!nothing) {
-        // (half by half: the scales of the second half are not fetched before the first half's scores are in)
-        const float4* sk = reinterpret_cast<const float4*>(s.sk[st]);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t raw[32];
-          __syncwarp();
-          tmem_ld32(s_addr + 32 * half, raw);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 c = sk[8 * half + i];
-            x[16 * half + 2 * i] = mul2(make_float2(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), make_float2(c.x, c.y));
-            x[16 * half + 2 * i + 1] = mul2(make_float2(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), make_float2(c.z, c.w));
-          }
-        }
-        if (kCap || kBias) {
-          const float2 ff = make_float2(f, f);
-#pragma unroll
-          for (int i = 0; i < kTileKeys / 2; ++i) x[i] = mul2(x[i], ff);
-        }
-        if (kCap) {
-          const float2 cu = make_float2(p.cap_u, p.cap_u);
-          float far = 0.f;
-#pragma unroll
-          for (int i = 0; i < kTileKeys / 2; ++i) far = max3(far, fabsf(x[i].x), fabsf(x[i].y));
-          if (__any_sync(0xffffffffu, far * p.cap_u >= kCapSeries)) {
-#pragma unroll
-            for (int i = 0; i < kTileKeys / 2; ++i) x[i] = capped_log2(x[i], mul2(x[i], cu), p.cap_log2e);
-          } else {
-#pragma unroll
-            for (int i = 0; i < kTileKeys / 2; ++i) x[i] = capped_series(x[i], mul2(x[i], cu));
-          }
-        }
-        if (kBias) {
-          const float away = static_cast<float>(pos - k0);
-#pragma unroll
-          for (int i = 0; i < kTileKeys / 2; ++i)
-            x[i] = make_float2(fmaf(-slope, fabsf(away - static_cast<float>(2 * i)), x[i].x),
-                               fmaf(-slope, fabsf(away - static_cast<float>(2 * i + 1)), x[i].y));
-        }
-        if (masked) {
-          const int a = min(max(keys.lo - k0, 0), 64), b = min(max(keys.hi - k0, 0), 64);
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {            // bits of the keys that the row sees, 32 at a time
-            const int from = min(max(a - 32 * w, 0), 32), upto = min(max(b - 32 * w, 0), 32);
-            const uint32_t mask = (w == 0 ? live0 : live1) & (upto >= 32 ? ~0u : (1u << upto) - 1u) & (from >= 32 ? 0u : ~0u << from);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if (!((mask >> (2 * i)) & 1u)) x[16 * w + i].x = -INFINITY;
-              if (!((mask >> (2 * i + 1)) & 1u)) x[16 * w + i].y = -INFINITY;
-            }
-          }
-        }
-        float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kTileKeys / 2; i += 2) {
-          t0 = max3(t0, x[i].x, x[i].y);
-          t1 = max3(t1, x[i + 1].x, x[i + 1].y);
-        }
-        top = fmaxf(t0, t1);
-        if (!kCap && !kBias) top *= f;
-      }
-      // top + e_top bounds what a row sees here: only where that is past a row's reference are the rows' own values looked for
-      if (__any_sync(0xffffffffu, R == -INFINITY ? top > -INFINITY : top + s.e_top[st] > R + kLazy)) {
-        float need = -INFINITY;
-        if (!nothing) {
-          const float4* se = reinterpret_cast<const float4*>(s.se[st]);
-          const float2 ff = make_float2(f, f);
-#pragma unroll
-          for (int i = 0; i < kTileKeys / 4; ++i) {
-            const float4 e = se[i];
-            const float2 a = (kCap || kBias) ? add2(x[2 * i], make_float2(e.x, e.y)) : fma2(x[2 * i], ff, make_float2(e.x, e.y));
-            const float2 b = (kCap || kBias) ? add2(x[2 * i + 1], make_float2(e.z, e.w)) : fma2(x[2 * i + 1], ff, make_float2(e.z, e.w));
-            need = max3(need, a.x, a.y);
-            need = max3(need, b.x, b.y);
-          }
-        }
-        const bool first = R == -INFINITY;
-        const bool grown = first ? need > -INFINITY : need > R + kLazy;
-        if (__any_sync(0xffffffffu, grown && !first)) {        // (so j > 0)
-          const float by = grown && !first ? ex2(R - need) : 1.f;
-          l *= by;
-          go = tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
-          if (!__all_sync(0xffffffffu, go)) {
-            go = false;
-            break;
-          }
-          tc_fence_after();
-          __syncwarp();
+    for (int j0 = 0; go && j0 < ntiles; j0 += kFoldTiles) {
+      const int jend = min(ntiles, j0 + kFoldTiles);
+      if (j0 > 0) {
+        // the sums so far go to the workspace, added to nearest, and O starts again from zero
+        go = __all_sync(0xffffffffu, tile_wait(s, &s.o_done[grp], (j0 - 1) & 1, p.status_word));
+        if (!go) break;
+        tc_fence_after();
+        const int64_t part = static_cast<int64_t>(split) * p.num_tokens + token;
+        const bool again = j0 > kFoldTiles && tid < rows;
+        const float by = again ? folded_factor(p.tile_ml[part * p.num_heads + h].x, R) : 0.f;
+        float4* sums = reinterpret_cast<float4*>(p.tile_o + part * p.sum_rv + H.v_col);
+        __syncwarp();
 #pragma unroll 1
-          for (int col = 0; col < rv; col += 16) {
-            uint32_t v[16];
-            tmem_ld16(lane_addr + kColO + col, v);
+        for (int col = 0; col < rv; col += 16) {
+          uint32_t v[16];
+          tmem_ld16(lane_addr + kColO + col, v);
+          if (tid < rows) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
-            tmem_st16(lane_addr + kColO + col, v);
-          }
-        }
-        if (grown) R = need;
-      }
-      __syncwarp();
-      if (nothing) {
-        uint32_t z[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = 0u;
-#pragma unroll
-        for (int i = 0; i < kTileKeys; i += 16) tmem_st16(s_addr + i, z);
-      } else {
-        // exponentials in place (the unit that bounds the kernel works without a pause), then the weights
-        const float base = R == -INFINITY ? 0.f : R - kWeightShift;
-        const float2 nb = make_float2(-base, -base), ff = make_float2(f, f);
-        float2 sum[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < kTileKeys / 2; ++i) {
-          const float2 y = (kCap || kBias) ? add2(x[i], nb) : fma2(x[i], ff, nb);
-          x[i] = make_float2(ex2(y.x), ex2(y.y));
-          sum[i & 3] = add2(sum[i & 3], x[i]);
-        }
-        const float4* sv = reinterpret_cast<const float4*>(s.sv[st]);
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {         // (16-column stores cost spills)
-          uint32_t w[8], rest[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 p0 = x[8 * part + 2 * i], p1 = x[8 * part + 2 * i + 1];
-            const float4 c = sv[4 * part + i];
-            float2 w0 = mul2(p0, make_float2(c.x, c.y)), w1 = mul2(p1, make_float2(c.z, c.w));
-            if (masked) {             // a masked key's weight is zero whatever its scale holds
-              if (p0.x == 0.f) w0.x = 0.f;
-              if (p0.y == 0.f) w0.y = 0.f;
-              if (p1.x == 0.f) w1.x = 0.f;
-              if (p1.y == 0.f) w1.y = 0.f;
+            for (int i = 0; i < 4; ++i) {
+              float4 y = again ? sums[(col >> 2) + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+              y.x = fmaf(y.x, by, __uint_as_float(v[4 * i]));
+              y.y = fmaf(y.y, by, __uint_as_float(v[4 * i + 1]));
+              y.z = fmaf(y.z, by, __uint_as_float(v[4 * i + 2]));
+              y.w = fmaf(y.w, by, __uint_as_float(v[4 * i + 3]));
+              sums[(col >> 2) + i] = y;
             }
-            pack_weights(w0, w[2 * i], rest[2 * i]);
-            pack_weights(w1, w[2 * i + 1], rest[2 * i + 1]);
           }
           __syncwarp();
-          tmem_st8(s_addr + 8 * part, w);
-          tmem_st8(s_addr + kTileKeys / 2 + 8 * part, rest);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0u;
+          tmem_st16(lane_addr + kColO + col, v);
         }
-        sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-        l += sum[0].x + sum[0].y;
+        if (tid < rows) p.tile_ml[part * p.num_heads + h].x = R;
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      // Phases are told apart by parity alone: before the last product is let go, the one in front of it is seen to have ended.
-      if (j > 0 && j + 1 == ntiles) go = go && tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
-      go = __all_sync(0xffffffffu, go);
-      if (go && lane == 0) mbar_arrive(&s.p_full[grp][j & 1]);
+      for (int j = j0; go && j < jend; ++j) {
+        const int st = j & (stages - 1), k0 = kbeg + j * kTileKeys;
+        const uint32_t s_addr = lane_addr + (j & 1) * kTileKeys;
+        go = tile_wait(s, &s.full[st], (j / stages) & 1, p.status_word) && tile_wait(s, &s.s_full[grp][j & 1], (j >> 1) & 1, p.status_word);
+        if (!__all_sync(0xffffffffu, go)) {
+          go = false;
+          break;
+        }
+        tc_fence_after();
+        const bool nothing = k0 >= outer_hi || k0 + kTileKeys <= outer_lo;      // of this warp's rows
+        const uint32_t live0 = s.live[st][0], live1 = s.live[st][1];
+        const bool masked = k0 < inner_lo || k0 + kTileKeys > inner_hi || (live0 & live1) != 0xffffffffu;
+        float2 x[kTileKeys / 2];
+        float top = -INFINITY;
+        if (!nothing) {
+          // (half by half: the scales of the second half are not fetched before the first half's scores are in)
+          const float4* sk = reinterpret_cast<const float4*>(s.sk[st]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t raw[32];
+            __syncwarp();
+            tmem_ld32(s_addr + 32 * half, raw);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 c = sk[8 * half + i];
+              x[16 * half + 2 * i] = mul2(make_float2(__uint_as_float(raw[4 * i]), __uint_as_float(raw[4 * i + 1])), make_float2(c.x, c.y));
+              x[16 * half + 2 * i + 1] = mul2(make_float2(__uint_as_float(raw[4 * i + 2]), __uint_as_float(raw[4 * i + 3])), make_float2(c.z, c.w));
+            }
+          }
+          if (kCap || kBias) {
+            const float2 ff = make_float2(f, f);
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 2; ++i) x[i] = mul2(x[i], ff);
+          }
+          if (kCap) {
+            const float2 cu = make_float2(p.cap_u, p.cap_u);
+            float far = 0.f;
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 2; ++i) far = max3(far, fabsf(x[i].x), fabsf(x[i].y));
+            if (__any_sync(0xffffffffu, far * p.cap_u >= kCapSeries)) {
+#pragma unroll
+              for (int i = 0; i < kTileKeys / 2; ++i) x[i] = capped_log2(x[i], mul2(x[i], cu), p.cap_log2e);
+            } else {
+#pragma unroll
+              for (int i = 0; i < kTileKeys / 2; ++i) x[i] = capped_series(x[i], mul2(x[i], cu));
+            }
+          }
+          if (kBias) {
+            const float away = static_cast<float>(pos - k0);
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 2; ++i)
+              x[i] = make_float2(fmaf(-slope, fabsf(away - static_cast<float>(2 * i)), x[i].x),
+                                 fmaf(-slope, fabsf(away - static_cast<float>(2 * i + 1)), x[i].y));
+          }
+          if (masked) {
+            const int a = min(max(keys.lo - k0, 0), 64), b = min(max(keys.hi - k0, 0), 64);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {            // bits of the keys that the row sees, 32 at a time
+              const int from = min(max(a - 32 * w, 0), 32), upto = min(max(b - 32 * w, 0), 32);
+              const uint32_t mask = (w == 0 ? live0 : live1) & (upto >= 32 ? ~0u : (1u << upto) - 1u) & (from >= 32 ? 0u : ~0u << from);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                if (!((mask >> (2 * i)) & 1u)) x[16 * w + i].x = -INFINITY;
+                if (!((mask >> (2 * i + 1)) & 1u)) x[16 * w + i].y = -INFINITY;
+              }
+            }
+          }
+          float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kTileKeys / 2; i += 2) {
+            t0 = max3(t0, x[i].x, x[i].y);
+            t1 = max3(t1, x[i + 1].x, x[i + 1].y);
+          }
+          top = fmaxf(t0, t1);
+          if (!kCap && !kBias) top *= f;
+        }
+        // top + e_top bounds what a row sees here: only where that is past a row's reference are the rows' own values looked for
+        if (__any_sync(0xffffffffu, R == -INFINITY ? top > -INFINITY : top + s.e_top[st] > R + kLazy)) {
+          float need = -INFINITY;
+          if (!nothing) {
+            const float4* se = reinterpret_cast<const float4*>(s.se[st]);
+            const float2 ff = make_float2(f, f);
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 4; ++i) {
+              const float4 e = se[i];
+              const float2 a = (kCap || kBias) ? add2(x[2 * i], make_float2(e.x, e.y)) : fma2(x[2 * i], ff, make_float2(e.x, e.y));
+              const float2 b = (kCap || kBias) ? add2(x[2 * i + 1], make_float2(e.z, e.w)) : fma2(x[2 * i + 1], ff, make_float2(e.z, e.w));
+              need = max3(need, a.x, a.y);
+              need = max3(need, b.x, b.y);
+            }
+          }
+          const bool first = R == -INFINITY;
+          const bool grown = first ? need > -INFINITY : need > R + kLazy;
+          if (__any_sync(0xffffffffu, grown && !first)) {        // (so j > 0)
+            const float by = grown && !first ? ex2(R - need) : 1.f;
+            l *= by;
+            go = tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
+            if (!__all_sync(0xffffffffu, go)) {
+              go = false;
+              break;
+            }
+            tc_fence_after();
+            __syncwarp();
+#pragma unroll 1
+            for (int col = 0; col < rv; col += 16) {
+              uint32_t v[16];
+              tmem_ld16(lane_addr + kColO + col, v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
+              tmem_st16(lane_addr + kColO + col, v);
+            }
+          }
+          if (grown) R = need;
+        }
+        __syncwarp();
+        if (nothing) {
+          uint32_t z[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) z[i] = 0u;
+#pragma unroll
+          for (int i = 0; i < kTileKeys; i += 16) tmem_st16(s_addr + i, z);
+        } else {
+          // exponentials in place (the unit that bounds the kernel works without a pause), then the weights
+          const float base = R == -INFINITY ? 0.f : R - kWeightShift;
+          const float2 nb = make_float2(-base, -base), ff = make_float2(f, f);
+          float2 sum[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < kTileKeys / 2; ++i) {
+            const float2 y = (kCap || kBias) ? add2(x[i], nb) : fma2(x[i], ff, nb);
+            x[i] = make_float2(ex2(y.x), ex2(y.y));
+            sum[i & 3] = add2(sum[i & 3], x[i]);
+          }
+          const float4* sv = reinterpret_cast<const float4*>(s.sv[st]);
+#pragma unroll
+          for (int part = 0; part < 4; ++part) {         // (16-column stores cost spills)
+            uint32_t w[8], rest[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 p0 = x[8 * part + 2 * i], p1 = x[8 * part + 2 * i + 1];
+              const float4 c = sv[4 * part + i];
+              float2 w0 = mul2(p0, make_float2(c.x, c.y)), w1 = mul2(p1, make_float2(c.z, c.w));
+              if (masked) {             // a masked key's weight is zero whatever its scale holds
+                if (p0.x == 0.f) w0.x = 0.f;
+                if (p0.y == 0.f) w0.y = 0.f;
+                if (p1.x == 0.f) w1.x = 0.f;
+                if (p1.y == 0.f) w1.y = 0.f;
+              }
+              pack_weights(w0, w[2 * i], rest[2 * i]);
+              pack_weights(w1, w[2 * i + 1], rest[2 * i + 1]);
+            }
+            __syncwarp();
+            tmem_st8(s_addr + 8 * part, w);
+            tmem_st8(s_addr + kTileKeys / 2 + 8 * part, rest);
+          }
+          sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+          l += sum[0].x + sum[0].y;
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        // Phases are told apart by parity alone: before the last product is let go, the one in front of it is seen to have ended.
+        if (j > 0 && j + 1 == jend) go = go && tile_wait(s, &s.o_done[grp], (j - 1) & 1, p.status_word);
+        go = __all_sync(0xffffffffu, go);
+        if (go && lane == 0) mbar_arrive(&s.p_full[grp][j & 1]);
+      }
     }
 
     // ---- results -------------------------------------------------------------------------------------------------------
@@ -807,6 +852,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
       const float by = p.tile_splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       const bool to_up = p.out != nullptr && p.tile_splits == 1;
       const int64_t part = static_cast<int64_t>(split) * p.num_tokens + token;
+      const bool folded = ntiles > kFoldTiles && tid < rows;
+      const float by_folded = folded ? folded_factor(p.tile_ml[part * p.num_heads + h].x, R) : 0.f;
       if (p.tile_splits > 1 && tid < rows) p.tile_ml[part * p.num_heads + h] = make_float2(R, l);
 #pragma unroll 1
       for (int c = 0; c < rv; c += 16) {
@@ -814,6 +861,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
         float y[16];
         __syncwarp();
         if (ntiles > 0) tmem_ld16(lane_addr + kColO + c, v);
+        if (folded) {
+          const float4* sums = reinterpret_cast<const float4*>(p.tile_o + part * p.sum_rv + H.v_col + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 y = sums[i];
+            v[4 * i] = __float_as_uint(fmaf(y.x, by_folded, __uint_as_float(v[4 * i])));
+            v[4 * i + 1] = __float_as_uint(fmaf(y.y, by_folded, __uint_as_float(v[4 * i + 1])));
+            v[4 * i + 2] = __float_as_uint(fmaf(y.z, by_folded, __uint_as_float(v[4 * i + 2])));
+            v[4 * i + 3] = __float_as_uint(fmaf(y.w, by_folded, __uint_as_float(v[4 * i + 3])));
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) y[i] = (ntiles > 0 && by != 0.f) ? __uint_as_float(v[i]) * by : 0.f;
         if (p.tile_splits > 1) {

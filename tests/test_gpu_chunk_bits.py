@@ -3,14 +3,16 @@
 
 Threshold.  The last rounding, to nearest, is off by r = rms(fp16(o) - o), about 2^-12.2 of rms(o): half a step is 2^-12 to 2^-11 of a
 value, uniform in it (factor 1 / sqrt 3).  A kernel whose other roundings are those of 32-bit arithmetic and of numbers held in
-22 bits (2^-21 of a term, 2^-18 with the sums) adds e below r / 16 in quadrature: rms <= 1.002 r.  One rounding of every weight or of
+22 bits (2^-21 of a term, 2^-17 with the sums over some thousand keys) adds e below r / 16 in quadrature: rms <= 1.002 r.  One rounding of every weight or of
 every query entry to 11 bits adds as much again as r, spread over the terms: 1.2 r and more.  So: rms <= 1.05 r."""
 import pytest
 import torch
 
+from lsvd_b200 import ChunkState, LatentCacheLayout, chunk_attention_int8_latent_absorb
 from test_gpu_chunk import _case, _run, _slopes, _want
 
 pytestmark = pytest.mark.gpu
+DEV = "cuda"
 
 
 def rounding_ratio(got, want):
@@ -119,3 +121,51 @@ def test_error_over_splits_of_the_keys(news, olds):
     for hm in (False, True):
         assert rounding_ratio(_run(c, hm), o) <= 1.05
         assert rounding_ratio(_run(c, hm, latent=True), lat) <= 1.05
+
+
+def _exact_long(q, cache_k, scale_k, cache_v, scale_v, up_k, ranks, slots, old, begin=None):
+    """Latent result of one request's new tokens in 64 bits, on the GPU (keys rebuilt, dense masks)."""
+    T, H, D = q.shape
+    out = torch.empty(T, H * ranks, dtype=torch.float64, device=DEV)
+    L = old + T
+    pos, t = torch.arange(old, L, device=DEV)[:, None], torch.arange(L, device=DEV)[None, :]
+    hide = t > pos if begin is None else (t > pos) | (t < begin[:, None])
+    for h in range(H):
+        c = slice(h * ranks, (h + 1) * ranks)
+        keys = scale_k[slots, h].double()[:, None] * (cache_k[slots, c].double() @ up_k[c].double())
+        x = (q[:, h].double() @ keys.t() / D ** 0.5).masked_fill_(hide, float("-inf"))
+        out[:, c] = torch.softmax(x, 1) @ (scale_v[slots, h].double()[:, None] * cache_v[slots, c].double())
+    return out
+
+
+@pytest.mark.parametrize("heads,new,old", [(100, 264, 66000), (128, 20, 130000), (32, 40, 8180), (128, 17, 16367), (64, 4, 66000)])
+@pytest.mark.parametrize("begins", [False, True])
+def test_long_sums_keep_their_bits(heads, new, old, begins):
+    """Pieces of up to 66000 keys of one block: an accumulator of the tensor cores cuts off what its additions leave, so that its error
+    grows with their number (8 for 64 keys), and is folded into fp32 sums every 8192 keys.  The largest scores come late, so that
+    references move between the folds; with ``begins`` the rows begin at positions in other tiles, some behind the first fold.
+
+    Threshold: 1024 additions cut off 2^-23 each on average at most, 2^-13 of sums whose terms have one sign (the worst case, here
+    nearly so); the last rounding's rms is 2^-12.6 of values like these: sqrt(1 + 2^-0.8) = 1.25.  Without folds 66000 keys come to 4."""
+    ranks, D = 16, 32
+    g = torch.Generator(device=DEV).manual_seed(heads + new)
+    L = old + new
+    rand = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    lay = LatentCacheLayout([ranks] * heads)
+    codes = lambda: torch.randint(-128, 128, (L, heads * ranks), generator=g, device=DEV, dtype=torch.int8)
+    ck, cv = codes(), codes()
+    sk = (0.004 + 0.008 * torch.arange(L, device=DEV)[:, None] / L).expand(L, heads).half().contiguous()
+    sv = (0.01 + 0.01 * torch.rand(L, heads, generator=g, device=DEV)).half()
+    cv = (cv.short() // 2 + 60).clamp(-128, 127).to(torch.int8)      # mostly positive: sums that keep growing
+    q, up_k = rand(new, heads, D).half(), (rand(heads * ranks, D) / 8).half()
+    slots = torch.randperm(L, generator=g, device=DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    begin = torch.tensor([(i * 977) % (old + 1) for i in range(new)], **i32) if begins else None
+    state = ChunkState(torch.zeros(1, **i32), torch.tensor([L], **i32), torch.tensor([0, new], **i32), slots.int()[None], L, new)
+    got = chunk_attention_int8_latent_absorb(q, state, heads, D, ck, sk, cv, sv, up_k, layout=lay, key_begin=begin)
+    want = _exact_long(q, ck, sk, cv, sv, up_k, ranks, slots, old, begin)
+    assert rounding_ratio(got, want) <= 1.25
+    up_v = (rand(heads * ranks, D) / 8).half()
+    out = chunk_attention_int8_latent_absorb(q, state, heads, D, ck, sk, cv, sv, up_k, up_v, layout=lay, key_begin=begin)
+    o = torch.stack([want[:, h * ranks:(h + 1) * ranks] @ up_v[h * ranks:(h + 1) * ranks].double() for h in range(heads)], 1)
+    assert rounding_ratio(out, o) <= 1.25
