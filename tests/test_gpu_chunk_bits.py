@@ -138,16 +138,17 @@ def _exact_long(q, cache_k, scale_k, cache_v, scale_v, up_k, ranks, slots, old, 
     return out
 
 
-@pytest.mark.parametrize("heads,new,old", [(100, 264, 66000), (128, 20, 130000), (32, 40, 8180), (128, 17, 16367), (64, 4, 66000)])
+@pytest.mark.parametrize("heads,new,old,ranks", [(100, 264, 66000, 16), (128, 20, 130000, 16), (32, 40, 8180, 16), (128, 17, 16367, 16),
+                                                 (64, 4, 66000, 16), (64, 300, 40000, 112), (74, 300, 8300, 128)])
 @pytest.mark.parametrize("begins", [False, True])
-def test_long_sums_keep_their_bits(heads, new, old, begins):
+def test_long_sums_keep_their_bits(heads, new, old, ranks, begins):
     """Pieces of up to 66000 keys of one block: an accumulator of the tensor cores cuts off what its additions leave, so that its error
     grows with their number (8 for 64 keys), and is folded into fp32 sums every 8192 keys.  The largest scores come late, so that
     references move between the folds; with ``begins`` the rows begin at positions in other tiles, some behind the first fold.
 
     Threshold: 1024 additions cut off 2^-23 each on average at most, 2^-13 of sums whose terms have one sign (the worst case, here
     nearly so); the last rounding's rms is 2^-12.6 of values like these: sqrt(1 + 2^-0.8) = 1.25.  Without folds 66000 keys come to 4."""
-    ranks, D = 16, 32
+    D = 32
     g = torch.Generator(device=DEV).manual_seed(heads + new)
     L = old + new
     rand = lambda *s: torch.randn(*s, generator=g, device=DEV)
