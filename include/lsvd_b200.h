@@ -297,7 +297,8 @@ typedef struct lsvd_attn_chunk_args {
   int32_t causal, window;        /* window 0: none                                                                 */
   float softcap;                 /* 0: none; otherwise at least 1e-6 (smaller: LSVD_ERR_UNSUPPORTED), finite       */
   const float* alibi_slopes;     /* device fp32 [num_heads] or NULL                                                */
-  const int32_t* b_prefix_len;   /* device int32 [batch] or NULL                                                   */
+  const int32_t* b_prefix_len;   /* device int32 [batch] or NULL; a prefix has to be added in one step: rows see     */
+                                 /* what is cached when their step runs                                            */
   const int32_t* key_begin;      /* device int32 [num_tokens] or NULL                                              */
   const int32_t* mem_index;      /* device int32 [num_tokens] or NULL: cache slots of the rows' tokens, as lsvd_chunk_maps     */
                                  /* gives them.  A row whose token has none (negative: its request was refused) sees nothing.  */

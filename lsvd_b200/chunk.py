@@ -215,7 +215,8 @@ def chunk_attention_int8_latent_absorb(
     keys ``t <= pos`` of its request, and
 
       * ``window > 0``: only ``t > pos - window``;
-      * ``b_prefix_len [B]`` int32: also every ``t`` below it (a prefix whose tokens see one another);
+      * ``b_prefix_len [B]`` int32: also every ``t`` below it (a prefix whose tokens see one another; all of them have to be
+        added in one step, since an earlier piece cannot see what is not cached yet);
       * ``key_begin [num_tokens]`` int32: only ``t >= key_begin`` (first position of the token's document);
       * ``causal=False``: every key of the request (with a window: ``|pos - t| < window``).
 

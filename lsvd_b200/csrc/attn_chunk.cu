@@ -10,9 +10,9 @@
 // (|code| <= 128) and meet q~ and the weights on the tensor cores (mma m16n8k16, fp32 accumulators).  With few rows the bytes
 // of the cache would bound it, r_k + r_v + 4 bytes per key and head; what does is the instruction stream of a tile (widening,
 // two products of 16-row fragments that few rows fill, softmax) at twelve warps an SM.  Measured: 16 single tokens over 4096 keys, 32
-// heads, mean ranks 64 + 64: 201 us (268 MB, 1.3 TB/s); five tokens of eight requests 139 us.  Sixteen rows a
-// block, with the lower half of the fragments for rows 9 to 16, cost the few-row cases 230 against 215 us; the value loop is rolled for
-// the instruction cache (215 -> 201 us).
+// heads, mean ranks 64 + 64: 200 us (268 MB, 1.3 TB/s); five tokens of eight requests over 4091 keys 136 us.  Before the value loop
+// was rolled for the instruction cache (215 -> 201 us for the single tokens), sixteen rows a block, with the lower half of the
+// fragments for rows 9 to 16, took them 230 us against 215.
 //
 // Roundings.  q~ enters the products as two fp16 numbers, what fp16 keeps of it and the rest, relative to its row's largest entry (a
 // power of two taken out, so no entry overflows and small ones keep their bits down to 2^-23 of the largest).  The weights
@@ -519,12 +519,11 @@ static void chunk_split(int64_t blocks, int64_t want, int least, int unit, int m
 }
 
 // Requests of up to 16 new tokens go to the stream form (from 9 on as two blocks, each with its own pass over the keys), longer ones
-// to the tile form: eight requests over 4091 keys with 8, 9 and 16 new tokens each take 147, 233 and
-// 238 us so, 369 in the tile form.  A single
-// request of a step that may bring more than 16 always goes to the tile form (one launch).  The keys are split where the rows alone are too few
-// blocks: stream form, four rounds of the resident blocks (three per SM), pieces of 256 keys or more (at two, three, four, six
-// and eight rounds: eight requests of five tokens 140, 147, 152, 171, 192 us, 16 single tokens 257, 228, 225, 245, 257 us); tile
-// form, two rounds (one per SM), 512 keys or more.
+// to the tile form: eight requests over 4091 keys with 8, 9 and 16 new tokens each take 139, 226 and 230 us so, 392 from 9 on in the
+// tile form.  A single request of a step that may bring more than 16 always goes to the tile form (one launch).  The keys are split
+// where the rows alone are too few blocks: stream form, four rounds of the resident blocks (three per SM), pieces of 256 keys or more
+// (at two, three, four, six and eight rounds: eight requests of five tokens 128, 131, 136, 151, 169 us, 16 single tokens 232, 206, 200,
+// 210, 217 us); tile form, two rounds (one per SM), 512 keys or more.
 static ChunkPlan chunk_plan(int batch, int num_heads, int num_tokens, int max_new, int max_len) {
   ChunkPlan c{};
   const int64_t sms = std::max(1, device_sm_count());

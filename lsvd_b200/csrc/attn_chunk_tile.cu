@@ -10,19 +10,21 @@
 // the int8 codes to fp16 (exact) and store them in the 128-byte-swizzled layouts that the products read, one that issues the
 // products.  The codes are widened once for both groups; the score product of tile j + 2 runs while the softmax is at tile j + 1.
 //
-// What bounds it.  The 16384 exponentials of 64 keys take 1024 cycles of an SM (16 a cycle), the products 768 at ranks of
-// 64 + 64; a step takes about 2900 (clocks read inside the kernel).  With three load warps the softmax warps waited a quarter to a
-// third of it and the load warps hardly ever; with four the dependent chains of the softmax, two warps a scheduler, are what is left
-// (fixed-latency waits lead the stalls, 41 % of the issue slots are used).  What moved it, for a prompt of 8191 tokens, 32 heads, ranks 64 + 64:
+// What bounds it.  The 16384 exponentials of 64 keys take 1024 cycles of an SM (16 a cycle), the products 1024 at ranks of
+// 64 + 64; a prompt of 8191 tokens takes 2.0 us more for each such step of an SM than one of 4096, some 3900 cycles.  The dependent
+// chains of the softmax, two warps a scheduler, are what is left (fixed-latency waits lead the stalls, 43 % of the issue slots are
+// used).  What moved it, for a prompt of 8191 tokens, 32 heads, ranks 64 + 64, each at its time:
 //   * code size: the load warps' passes fully unrolled (compile-time widths) took 1.38 ms, as loops shared by K and V 0.97 ms:
 //     with all roles unrolled a third of the instruction fetches missed the SM's cache;
 //   * the prologue (q~ = B_k q) and the epilogue (o = B_v^T o_lat) with their factors read by every warp from global memory
 //     were 65 of 250 thousand cycles of an average block; with the factors in shared memory 0.88 ms;
-//   * four load warps instead of three 0.83 ms (five 0.85, seven 0.84);
-//   * both halves of q~ in the products, and of o_lat in the up-projection, 0.90 ms: the error against 64 bits went from 1.8 times
-//     that of a rounding of the result alone to 1.3 times.
-// Tried and slower: two threads a row with sixteen softmax warps (1.05 ms), the scores read twice instead of kept in registers
-// between the maximum and the weights (1.08 ms).  128 rows a block (mma m16n8k16) took 2.6 ms.
+//   * four load warps instead of three 0.83 ms (five 0.85, seven 0.84): with three the softmax warps waited a quarter to a third of
+//     a step for them;
+//   * both halves of q~ in the products, and of o_lat in the up-projection, 0.90 ms; both halves of the weights 1.00 ms; references
+//     over the keys that a row sees 1.01 ms; folds 1.03 ms.  With them the error against 64 bits is that of rounding the result
+//     alone, before them 1.8 times that.
+// Tried and slower: two threads a row with sixteen softmax warps (1.05 against 0.83 ms), the scores read twice instead of kept in
+// registers between the maximum and the weights (1.08 ms).  128 rows a block (mma m16n8k16) took 2.6 ms.
 //
 // O is rescaled only when a row's reference moves (attn_chunk.cuh): a reference is looked for where a tile's largest score and largest
 // V scale together are past it, over the keys that the row sees.  Each weight enters the product as two fp16 numbers, its
@@ -796,7 +798,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tile_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < kTileKeys; i += 16) tmem_st16(s_addr + i, z);
         } else {
-          // exponentials in place (the unit that bounds the kernel works without a pause), then the weights
+          // exponentials in place, one after another without a pause between them, then the weights
           const float base = R == -INFINITY ? 0.f : R - kWeightShift;
           const float2 nb = make_float2(-base, -base), ff = make_float2(f, f);
           float2 sum[4];

@@ -296,7 +296,7 @@ extern "C" int lsvd_chunk_maps(const lsvd_chunk_maps_args* a, void* stream) {
   while (hash < 2 * a->batch) hash *= 2;
   const size_t smem = static_cast<size_t>(a->batch) * (6 * 4 + 8) + static_cast<size_t>(hash) * 8;
   LSVD_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(chunk_maps_kernel), static_cast<int>(smem)));
-  // (one block and eight, replayed: 64 tokens 10.3 and 12.3 us, 2400 tokens 20.5 and 14.3, 98304 tokens 55 and 18)
+  // (one block and eight, replayed: 64 tokens 8.2 and 8.2 us, 2400 tokens 10.2 and 10.2, 98304 tokens 100 and 21)
   const int ctas = a->num_tokens > 2 * kMapsThreads || a->rebuild ? kMapsCluster : 1;
   LSVD_CUDA_TRY(launch_chained(chunk_maps_kernel, dim3(ctas), dim3(kMapsThreads), smem, static_cast<cudaStream_t>(stream), ctas, true,
                                *a, hash));
