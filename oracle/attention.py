@@ -165,8 +165,9 @@ def chunk_maps(req, ready, new, table, page, r2t, num_tokens, num_slots, free=No
     """Slots of a step's new tokens, entry by entry (lists of Python integers; ``table`` and ``r2t`` are changed in place).
 
     Returns (start, seq, mem_index, position_ids, head, refused) with ``refused`` the entries that got nothing: their row or
-    length does not fit the tables, their tokens do not fit ``num_tokens`` or are more than ``max_new`` (0: any), an earlier entry adds tokens to the same row, the free pages have
-    run out, or (``rebuild``) it has no new tokens and more cached ones than the entry that adds tokens to its row.
+    length does not fit the tables, their tokens do not fit ``num_tokens`` or are more than ``max_new`` (0: any), an earlier
+    entry adds tokens to the same row, the free pages have run out, or (``rebuild`` with a free list) it has no new tokens and
+    more cached ones than the entry that adds tokens to its row.
     """
     up = lambda tokens: -(-tokens // page)
     start, seq, refused, seen, dry = [0], [], [], set(), False
